@@ -344,6 +344,61 @@ int rbk_attn_bwd(rbk_ctx* ctx, void* dqkv, float* dbias_qkv, const void* qkv, co
                  const float* lse, int B, int S, int H, int dh, float scale, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Query / key normalisation with the rotary position embedding
+ * ------------------------------------------------------------------------ */
+
+/* A half tensor [B, S, H, dh] by strides: element (b, s, h, c) at
+ * p[b * sb + s * ss + h * sh + c].  Strides are multiples of 8 elements and p
+ * is 16-byte aligned, so a head may be a column block of a fused q | k | v row
+ * as well as a plane of a [B, H, S, dh] tensor. */
+typedef struct rbk_heads {
+    void* p;
+    int64_t sb, ss, sh;
+} rbk_heads;
+
+/* For every token (b, s) and every head x of its queries and keys:
+ *   xhat = x / sqrt(mean(x^2) + eps),  z = gain * xhat  (gain NULL: ones),
+ *   y = z with the first `rot` channels rotated by the token's position p:
+ *   pair i < rot / 2 = (a, b) -> (a cos t - b sin t, a sin t + b cos t),
+ *   t = p * inv_freq[i]; the pair is channels (i, i + rot / 2), or with
+ *   interleaved != 0 channels (2 i, 2 i + 1).  One FP16 rounding, of y.
+ * The angle is taken modulo a turn in 64-bit fixed point, so it is as exact at
+ * position 2^31 - 1 as at 1.
+ *   dh a multiple of 8, 8 <= dh <= 256; rot a multiple of 16 (8 when
+ *   interleaved), 0 <= rot <= dh; B, S >= 0; Hq, Hk >= 0 (Hk = 0: queries only).
+ * No counterpart in the reference, whose positions are learned embeddings. */
+typedef struct rbk_qk_args {
+    int B, S, Hq, Hk, dh;
+    int rot, interleaved;
+    float eps;               /* > 0                                              */
+    double theta;            /* inv_freq[i] = theta^(-2 i / rot) when inv_freq is NULL */
+    const double* inv_freq;  /* host [rot / 2], radians per position, or NULL    */
+    const int* positions;    /* device [B * S], or NULL: token (b, s) has pos0 + s */
+    int pos0;
+    const void *gq, *gk;     /* half [dh] gains of queries and keys, or NULL     */
+    rbk_heads q, k;          /* the heads before the normalisation               */
+    rbk_heads oq, ok;        /* forward: y (may be q, k themselves); backward: dx */
+    /* backward only */
+    rbk_heads dyq, dyk;      /* gradients of y (dx may be dy itself)             */
+    float *dgq, *dgk;        /* FP32 [dh] gradients of the gains, or NULL        */
+    int accumulate;          /* 1: dgq, dgk += ; 0: they are set                 */
+    /* Scratch of the backward: RBK_QK_BWD_WS_BYTES of device memory, or NULL for
+     * the ctx scratch.  A caller that captures the call into a CUDA graph passes
+     * its own: the ctx scratch may move when another call needs more. */
+    void* ws;
+} rbk_qk_args;
+
+#define RBK_QK_BWD_WS_BYTES (1024 * 256 * 4)
+
+/* q, k -> oq, ok (the heads that rbk_attn_fwd reads, when they are column
+ * blocks of its qkv rows). */
+int rbk_qk_norm_rope_fwd(rbk_ctx* ctx, const rbk_qk_args* args, void* stream);
+/* dyq, dyk -> oq, ok = dq, dk, and dgq, dgk.  Nothing but q, k is needed from
+ * the forward: the row statistics are computed again from the rows, which the
+ * pass reads anyway.  Sums in a fixed order: two runs give the same bits. */
+int rbk_qk_norm_rope_bwd(rbk_ctx* ctx, const rbk_qk_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
  * Model: the RubidiumTransformer drop-in (src/model.h:112-139)
  * ------------------------------------------------------------------------ */
 

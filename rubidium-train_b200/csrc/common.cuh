@@ -109,6 +109,10 @@ struct ProfScope {
 // only when the current arena is too small.
 int ctx_scratch(rbk_ctx* ctx, size_t bytes, void** out);
 
+// The ctx exists and its device is the calling thread's current one: a launch on
+// another device's stream, or with another device's scratch, is refused.
+int check_device(rbk_ctx* ctx, const char* who);
+
 // out[c] += sum_r part[r*C + c], deterministic (ctx.cu).
 int column_reduce(float* out, const float* part, int R, int C, cudaStream_t st);
 

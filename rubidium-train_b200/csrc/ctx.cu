@@ -61,6 +61,14 @@ int ctx_scratch(rbk_ctx* ctx, size_t bytes, void** out) {
     return RBK_OK;
 }
 
+int check_device(rbk_ctx* ctx, const char* who) {
+    RBK_REQUIRE(ctx, "%s: ctx is NULL", who);
+    int dev;
+    RBK_CUDA(cudaGetDevice(&dev));
+    RBK_REQUIRE(dev == ctx->device, "%s: the current device (%d) is not the context's (%d)", who, dev, ctx->device);
+    return RBK_OK;
+}
+
 // out[c] += sum_r part[r*C + c]   (deterministic, fixed order over r)
 __global__ void column_reduce_kernel(float* __restrict__ out, const float* __restrict__ part, int R, int C) {
     const int c = blockIdx.x * blockDim.x + threadIdx.x;

@@ -48,6 +48,19 @@ class TailArgs(C.Structure):
     ]
 
 
+class Heads(C.Structure):
+    """rbk_heads (include/rbk.h)."""
+    _fields_ = [("p", vp), ("sb", i64), ("ss", i64), ("sh", i64)]
+
+
+class QkArgs(C.Structure):
+    """rbk_qk_args (include/rbk.h)."""
+    _fields_ = [("B", i32), ("S", i32), ("Hq", i32), ("Hk", i32), ("dh", i32), ("rot", i32), ("interleaved", i32),
+                ("eps", f32), ("theta", C.c_double), ("inv_freq", vp), ("positions", vp), ("pos0", i32), ("gq", vp),
+                ("gk", vp), ("q", Heads), ("k", Heads), ("oq", Heads), ("ok", Heads), ("dyq", Heads), ("dyk", Heads),
+                ("dgq", vp), ("dgk", vp), ("accumulate", i32), ("ws", vp)]
+
+
 class Config(C.Structure):
     _fields_ = [("V", i32), ("T", i32), ("D", i32), ("H", i32), ("L", i32), ("FF", i32)]
 
@@ -103,6 +116,8 @@ _SIGS = {
     "rbk_gemm_wgrad": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, vp]),
     "rbk_attn_fwd": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, f32, vp]),
     "rbk_attn_bwd": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, vp]),
+    "rbk_qk_norm_rope_fwd": (i32, [vp, C.POINTER(QkArgs), vp]),
+    "rbk_qk_norm_rope_bwd": (i32, [vp, C.POINTER(QkArgs), vp]),
     "rbk_model_create": (i32, [C.POINTER(vp), C.POINTER(Config), C.POINTER(ModelOpts)]),
     "rbk_model_destroy": (i32, [vp]),
     "rbk_model_buffer": (i32, [vp, i32, C.POINTER(vp), C.POINTER(i64)]),

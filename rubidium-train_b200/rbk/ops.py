@@ -12,7 +12,7 @@ import threading
 
 import torch
 
-from ._lib import GemmDesc, Scaler, TailArgs, call, lib
+from ._lib import GemmDesc, Heads, QkArgs, Scaler, TailArgs, call, lib
 
 EPI_STORE_F16, EPI_BIAS_GELU, EPI_GELU_BWD, EPI_ACC_F32, EPI_STORE_F32 = range(5)
 LN_REFERENCE_FORMULA = 1
@@ -72,6 +72,16 @@ def _p(t):
 def _need(t, dtype, name):
     if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous CUDA {dtype} tensor, got {t.dtype} on {t.device}")
+
+
+def _need_here(t, dtype, name, shape=None):
+    """A CUDA tensor of the current device, type and shape (any strides)."""
+    if t.dtype != dtype or not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA {dtype} tensor, got {t.dtype} on {t.device}")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 # ----------------------------------------------------------------- LayerNorm --
@@ -273,3 +283,90 @@ def attn_bwd(qkv, o, dout, lse, B, S, H, dh, scale=None, dbias=None):
     call("rbk_attn_bwd", ctx().handle, _p(dqkv), _p(dbias), _p(qkv), _p(o), _p(dout), _p(lse), B, S, H, dh,
          C.c_float(scale), _s())
     return dqkv
+
+
+# ------------------------------------------------- query / key norm, rotation --
+
+RBK_QK_BWD_WS_BYTES = 1024 * 256 * 4
+
+
+def _heads(t, name, shape=None):
+    _need_here(t, torch.float16, name, shape)
+    if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
+        raise ValueError(f"{name}: expected [B, S, H, dh] heads with contiguous channels, got shape {tuple(t.shape)}, "
+                         f"strides {t.stride()}")
+    return Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out):
+    a = QkArgs()
+    a.B, a.S, a.Hq, a.dh = q.shape
+    a.q = _heads(q, "q")
+    if k is not None:
+        a.Hk = k.shape[2]
+        a.k = _heads(k, "k", (a.B, a.S, a.Hk, a.dh))
+    a.rot = a.dh if rot is None else rot
+    a.interleaved, a.eps, a.theta, a.pos0 = int(interleaved), eps, theta, pos0
+    if inv_freq is not None:
+        if len(inv_freq) != a.rot // 2:
+            raise ValueError(f"inv_freq: expected {a.rot // 2} values, got {len(inv_freq)}")
+        freq = (C.c_double * max(1, len(inv_freq)))(*[float(x) for x in inv_freq])
+        a.inv_freq, a.kept = C.cast(freq, C.c_void_p), freq
+    if positions is not None:
+        _need_here(positions, torch.int32, "positions", (a.B, a.S))
+        if not positions.is_contiguous():
+            raise ValueError("positions: expected a contiguous tensor")
+        a.positions = positions.data_ptr()
+    for name, g in (("gq", gq), ("gk", gk)):
+        if g is not None:
+            _need_here(g, torch.float16, name, (a.dh,))
+            if not g.is_contiguous():
+                raise ValueError(f"{name}: expected a contiguous tensor")
+            setattr(a, name, g.data_ptr())
+    if out is None:
+        # queries and keys side by side, as the projection's rows hold them
+        both = torch.empty(a.B, a.S, a.Hq + a.Hk, a.dh, dtype=torch.float16, device=q.device)
+        out = both[:, :, :a.Hq], (both[:, :, a.Hq:] if k is not None else None)
+    oq, ok = out
+    a.oq = _heads(oq, "out[0]", q.shape)
+    if k is not None:
+        a.ok = _heads(ok, "out[1]", k.shape)
+    return a, oq, ok
+
+
+def qk_norm_rope_fwd(q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000.0, inv_freq=None, rot=None,
+                     interleaved=False, eps=1e-6, out=None):
+    """Per-head RMS norm of queries and keys, then the rotary position embedding (rbk_qk_norm_rope_fwd).
+
+    q [B, S, Hq, dh], k [B, S, Hk, dh] (or None): half, any strides with contiguous channels.  gq, gk: half
+    [dh] gains.  positions: int32 [B, S], or None for pos0 + s.  inv_freq: rot / 2 host numbers, or None for
+    theta^(-2 i / rot).  rot: leading channels that turn (default dh).  out: (yq, yk), e.g. the q and k blocks of
+    the qkv rows that attn_fwd reads, or (q, k) themselves; by default one new tensor.  Returns (yq, yk)."""
+    a, yq, yk = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
+    call("rbk_qk_norm_rope_fwd", ctx().handle, C.byref(a), _s())
+    return yq, yk
+
+
+def qk_norm_rope_bwd(dyq, dyk, q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000.0, inv_freq=None,
+                     rot=None, interleaved=False, eps=1e-6, out=None, dgq=None, dgk=None):
+    """Its backward (rbk_qk_norm_rope_bwd): q, k as the forward read them.  Returns (dq, dk, dgq, dgk); given
+    FP32 [dh] dgq, dgk accumulate, else both are new.  out: (dq, dk), may be (dyq, dyk)."""
+    a, dq, dk = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
+    a.dyq = _heads(dyq, "dyq", q.shape)
+    if k is not None:
+        a.dyk = _heads(dyk, "dyk", k.shape)
+    if (dgq is None) != (dgk is None) and k is not None:
+        raise ValueError("dgq and dgk: give both or neither")
+    a.accumulate = int(dgq is not None)
+    if dgq is None:
+        both = torch.empty(2, a.dh, dtype=torch.float32, device=q.device)
+        dgq, dgk = both[0], (both[1] if k is not None else None)
+    for name, g in (("dgq", dgq), ("dgk", dgk)):
+        if g is not None:
+            _need(g, torch.float32, name)
+            _need_here(g, torch.float32, name, (a.dh,))
+            setattr(a, name, g.data_ptr())
+    ws = torch.empty(RBK_QK_BWD_WS_BYTES, dtype=torch.uint8, device=q.device)
+    a.ws = ws.data_ptr()
+    call("rbk_qk_norm_rope_bwd", ctx().handle, C.byref(a), _s())
+    return dq, dk, dgq, dgk

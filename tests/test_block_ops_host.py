@@ -1,0 +1,104 @@
+"""Argument checks and references of the decoder-block operators that need no GPU: a call is refused for its
+arguments before it looks at its context or a device."""
+import ctypes as C
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import qk_ref   # noqa: E402
+
+P = 1 << 20     # an aligned address that no refused call reads
+
+
+def refused(name, args, match):
+    from rbk import lib
+    st = getattr(lib(), name)(None, C.byref(args), None)
+    msg = lib().rbk_last_error().decode()
+    assert st == -1 and match in msg, (st, msg)
+
+
+def qk(**kw):
+    from rbk._lib import Heads, QkArgs
+    a = QkArgs()
+    a.B, a.S, a.Hq, a.Hk, a.dh, a.rot, a.eps, a.theta = 2, 4, 3, 1, 64, 64, 1e-6, 1e4
+    for n in ("q", "k", "oq", "ok", "dyq", "dyk"):
+        setattr(a, n, Heads(P, 1024, 256, 64))
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("name", ["rbk_qk_norm_rope_fwd", "rbk_qk_norm_rope_bwd"])
+def test_qk_refusals(name):
+    from rbk._lib import Heads
+    for kw, match in [
+        (dict(B=-1), "negative"), (dict(Hk=-1), "negative"), (dict(B=65536, S=65536), "tokens"),
+        (dict(dh=0, rot=0), "dh"), (dict(dh=60, rot=0), "dh"), (dict(dh=264, rot=0), "dh"),
+        (dict(rot=80), "rot"), (dict(rot=-16), "rot"), (dict(rot=24), "rot"), (dict(rot=4, interleaved=1), "rot"),
+        (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(theta=0.0), "theta"),
+        (dict(theta=float("inf")), "theta"), (dict(gq=P + 2), "gains"), (dict(gk=P + 8), "gains"),
+        (dict(q=Heads(None, 1024, 256, 64)), "q is NULL"), (dict(k=Heads(P + 2, 1024, 256, 64)), "k must be 16-byte"),
+        (dict(q=Heads(P, 1024, 252, 64)), "strides of q"), (dict(ok=Heads(P, 1024, 256, 63)), "strides of ok"),
+        (dict(oq=Heads(P, 1024, 256, 0)), "zero stride"), (dict(oq=Heads(P, 0, 256, 64)), "zero stride"),
+    ]:
+        refused(name, qk(**kw), match)
+    freq = (C.c_double * 32)(*([0.5] * 31 + [float("inf")]))
+    refused(name, qk(inv_freq=C.cast(freq, C.c_void_p)), "inv_freq[31]")
+    refused(name, qk(), "ctx is NULL")                       # nothing else is wrong with these arguments
+    refused(name, qk(Hk=0, k=Heads(), ok=Heads(), dyk=Heads()), "ctx is NULL")
+
+
+def test_qk_bwd_refusals():
+    from rbk._lib import Heads
+    refused("rbk_qk_norm_rope_bwd", qk(dyq=Heads(None, 0, 0, 0)), "dyq is NULL")
+    refused("rbk_qk_norm_rope_bwd", qk(ws=P + 4), "ws")
+
+
+def test_qk_gradient_formula_against_differences():
+    """The reference's gradient, in float64, against central differences of its forward."""
+    torch.manual_seed(0)
+    B, S, H, dh = 1, 2, 2, 16
+    for rot, inter in ((16, False), (8, True)):
+        x, dy = (torch.randn(B, S, H, dh, dtype=torch.float64) for _ in range(2))
+        gain = 1 + 0.3 * torch.randn(dh, dtype=torch.float64)
+        ang = qk_ref.angles(B, S, rot, 100.0, None, 3)
+
+        def f(x, gain):
+            return float((qk_ref.fwd(x, gain, ang, rot, inter, 1e-3)[0] * dy).sum())
+
+        dx, dg, _, _ = qk_ref.bwd(dy, x, gain, ang, rot, inter, 1e-3)
+        step = 1e-6                                          # truncation ~ step^2, cancellation ~ 1e-16 / step
+        for t, d in ((x, dx), (gain, dg)):
+            for i in range(0, t.numel(), 7):
+                e = torch.zeros_like(t)
+                e.view(-1)[i] = step
+                lo, hi = (f(x - e, gain), f(x + e, gain)) if t is x else (f(x, gain - e), f(x, gain + e))
+                assert abs((hi - lo) / (2 * step) - float(d.view(-1)[i])) < 1e-7
+
+
+def test_args_layouts_match_header(tmp_path):
+    """The ctypes mirrors of the block operators' argument structs have the C compiler's field offsets."""
+    import os
+    import shutil
+    import subprocess
+    if shutil.which("gcc") is None:
+        pytest.skip("no gcc")
+    from rbk import _lib
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    structs = [("rbk_heads", _lib.Heads), ("rbk_qk_args", _lib.QkArgs)]
+    lines, want = [], []
+    for cname, cls in structs:
+        for f, _ in cls._fields_:
+            lines.append(f'printf("%zu\\n", offsetof({cname}, {f}));')
+            want.append(getattr(cls, f).offset)
+        lines.append(f'printf("%zu\\n", sizeof({cname}));')
+        want.append(C.sizeof(cls))
+    src = tmp_path / "off.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "rbk.h"\nint main(void) {\n' +
+                   "\n".join(lines) + "\nreturn 0;\n}\n")
+    exe = tmp_path / "off"
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), "-I/usr/local/cuda/include", str(src), "-o", str(exe)],
+                   check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == want
