@@ -302,6 +302,55 @@ int rbk_gemm_wgrad(rbk_ctx* ctx, float* dW, float* dbias, const void* dY, const 
                    void* stream);
 
 /* ------------------------------------------------------------------------
+ * Gated feed-forward block
+ * ------------------------------------------------------------------------ */
+
+enum { RBK_ACT_SILU = 0, RBK_ACT_GELU = 1 /* the tanh form */ };
+
+/* gate = x Wg^T + bg, up = x Wu^T + bu, h = act(gate) * up,
+ * y = h Wd^T + bd + residual.  All tensors half, row-major; D and F multiples of
+ * 8, every pointer 16-byte aligned, row strides (elements) multiples of 8.
+ * The two projections, the activation and the product are one kernel (tcgen05
+ * tiles that hold the gate's and the up projection's columns side by side), the
+ * down projection is the second; up to 32 rows, where reading the weights is the
+ * cost, both are kernels that stream them.  h is rounded to half once. */
+typedef struct rbk_ffn_args {
+    int N, D, F;             /* N >= 0 rows                                      */
+    int act;                 /* RBK_ACT_*                                        */
+    const void* x; int ldx;  /* [N, D]                                           */
+    const void* wgu;         /* [2F, D]: the rows of Wg, then those of Wu        */
+    const void* bgu;         /* [2F] or NULL                                     */
+    const void* wd;          /* [D, F]                                           */
+    const void* bd;          /* [D] or NULL                                      */
+    const void* residual; int ldr;   /* [N, D] or NULL; may be y                 */
+    void* y; int ldy;        /* [N, D]                                           */
+    void* gu;                /* [N, 2F]: gate | up for the backward, or NULL     */
+    void* h;                 /* [N, F]: scratch, or kept for the backward        */
+} rbk_ffn_args;
+int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* args, void* stream);
+
+/* From dy and the forward's x and gu:
+ *   dh = dy Wd,  dgu = [dh * up * act'(gate) | dh * act(gate)]   (one kernel)
+ *   dx = dgu Wgu,  dWgu += dgu^T x,  dbgu += column sums of dgu,
+ *   dWd += dy^T h,  dbd += column sums of dy        (rbk_gemm_dgrad / _wgrad)
+ * dgu is rounded to half once; the weight gradients are FP32 and accumulate.
+ * recompute_h: h is written by the first kernel from gu (it need not have been
+ * kept); else the forward's h is read, and only by dWd.  dx, dwgu, dbgu, dwd and
+ * dbd may be NULL (dbgu needs dwgu, dbd needs dwd); x is read for dwgu only. */
+typedef struct rbk_ffn_bwd_args {
+    int N, D, F;
+    int act;
+    const void* dy; int lddy;
+    const void* x; int ldx;
+    const void *gu, *wgu, *wd;
+    void* h; int recompute_h;    /* h may be NULL when it is neither wanted nor needed */
+    void* dgu;                   /* [N, 2F], may be gu                           */
+    void* dx; int lddx;
+    float *dwgu, *dbgu, *dwd, *dbd;
+} rbk_ffn_bwd_args;
+int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
  * LoRA adapters, kernel level (the model level runs the same GEMMs inside
  * rbk_model_forward / _backward once rbk_model_lora_enable has been called)
  * ------------------------------------------------------------------------ */

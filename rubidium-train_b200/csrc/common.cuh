@@ -116,6 +116,13 @@ int check_device(rbk_ctx* ctx, const char* who);
 // out[c] += sum_r part[r*C + c], deterministic (ctx.cu).
 int column_reduce(float* out, const float* part, int R, int C, cudaStream_t st);
 
+// The gated feed-forward block's tcgen05 tiles (gemm.cu): h[N, F] = act(x Wg^T + bg) * (x Wu^T + bu),
+// gu[N, 2F] (or NULL) the two projections; and dgu[N, 2F] (may be gu) from dy and gu, h (or NULL) again.
+int glu_fwd_tiles(rbk_ctx* ctx, void* h, void* gu, const void* x, int ldx, const void* wgu, const void* bgu, int N, int D,
+                  int F, int act, cudaStream_t st);
+int glu_bwd_tiles(rbk_ctx* ctx, void* dgu, void* h, const void* dy, int lddy, const void* wd, const void* gu, int N, int D,
+                  int F, int act, cudaStream_t st);
+
 // Ticket slots (see rbk_ctx::tickets).
 enum TicketSlot {
     kTicketSum = 0,
@@ -211,6 +218,25 @@ __device__ __forceinline__ float gelu_grad_f(float x) {
     const float c = 0.7978845608028654f, a = 0.044715f;
     const float t = tanhf(c * (x + a * x * x * x));
     return 0.5f * (1.0f + t) + 0.5f * x * (1.0f - t * t) * c * (1.0f + 3.0f * a * x * x);
+}
+
+// The gate activations z sigma(r(z)): SiLU with r = z, the tanh form of GELU with
+// r = 2 sqrt(2 / pi) (z + 0.044715 z^3), since (1 + tanh(r / 2)) / 2 = sigma(r).
+// The exponential and the quotient are the fast ones, right to about 2^-21: what
+// they feed is rounded to FP16 (2^-11).
+__device__ __forceinline__ float glu_sigma(float z, int act) {
+    const float c = 1.5957691216057308f, a = 0.044715f;
+    const float r = act == RBK_ACT_GELU ? c * z * (1.0f + a * z * z) : z;
+    return __fdividef(1.0f, 1.0f + __expf(-r));
+}
+__device__ __forceinline__ float glu_act(float z, int act) { return z * glu_sigma(z, act); }
+// a = act(z), da = act'(z) = s + z s (1 - s) r'(z)
+__device__ __forceinline__ void glu_act_grad(float z, int act, float& a, float& da) {
+    const float c = 1.5957691216057308f, a3 = 3.0f * 0.044715f;
+    const float s = glu_sigma(z, act);
+    a = z * s;
+    const float dr = act == RBK_ACT_GELU ? c * (1.0f + a3 * z * z) : 1.0f;
+    da = s + a * (1.0f - s) * dr;
 }
 
 }  // namespace rbk

@@ -100,6 +100,17 @@ __device__ __forceinline__ void gelu_grad2(float& g0, float& g1, float x0, float
     f2unpack(mul2(f2pack(g0, g1), d), g0, g1);
 }
 
+// Epilogues of the gated feed-forward block (ffn.cu), on the CTA-pair kernel only.
+//   kEpiGlu:    a tile's 256 accumulator columns are 128 columns of the gate x Wg^T and the same 128 of
+//               the up projection x Wu^T (even / odd CTA's rows of B); h = act(gate) * up leaves with
+//               them, or alone.
+//   kEpiGluBwd: acc = dh = dy Wd;  dgate = dh up act'(gate), dup = dh act(gate), and h again.
+constexpr int kEpiGlu = 5, kEpiGluBwd = 6;
+__host__ __device__ constexpr bool is_glu(int epi) { return epi == kEpiGlu || epi == kEpiGluBwd; }
+__host__ __device__ constexpr bool is_f16(int epi) {
+    return epi == RBK_EPI_STORE_F16 || epi == RBK_EPI_BIAS_GELU || epi == RBK_EPI_GELU_BWD || is_glu(epi);
+}
+
 template <int BN>
 struct Cfg {
     static constexpr int STAGES = BN == 256 ? 4 : BN == 192 ? 5 : 6;
@@ -137,6 +148,11 @@ struct Params {
     float* part_rows;   // [splits - 1][M] row-sum partials (dbias_rows)
     int ldp;            // row pitch of a plane (N rounded up to 4)
     int c_zero;         // ACC_F32 into a C known to hold zeros: the owner stores without reading C
+    // gated feed-forward epilogues: N is F; bias / aux are the gate's, bias2 / aux2 the up projection's
+    const half* bias2;
+    const half* aux2;
+    int act;
+    int store_gu, store_h;
 };
 
 // How an ACC_F32 unit of split `split` writes its tile.  kAccStore: the owner of a tile whose C
@@ -671,6 +687,102 @@ __device__ __forceinline__ void epilogue_chunk_tma(const Params& p, int m0, int 
     ++sc;
 }
 
+// v[j] += bias[n + j] where n + j < N (bias of 32 columns, the same in every lane).
+__device__ __forceinline__ void add_bias32(float* v, const half* bias, int n, int N) {
+    if (n + 32 <= N) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+            float b[8];
+            h8_to_f(__ldg(reinterpret_cast<const uint4*>(bias + n + j)), b);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[j + q] += b[q];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (n + j < N) v[j] += __half2float(bias[n + j]);
+    }
+}
+
+// Gated feed-forward, one 32 x 32 chunk: g, u the gate's and the up projection's accumulators.  The warp's
+// three tiles take gate, up and h.
+__device__ __forceinline__ void glu_chunk(const Params& p, int m0, int n, const uint32_t* rg, const uint32_t* ru,
+                                          uint8_t* st, uint32_t st_s, int lane, const CUtensorMap* tmG,
+                                          const CUtensorMap* tmU, const CUtensorMap* tmH) {
+    if (n >= p.N || m0 >= p.M) return;                     // warp-uniform
+    float g[32], u[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        g[j] = __uint_as_float(rg[j]);
+        u[j] = __uint_as_float(ru[j]);
+    }
+    if (p.bias) {
+        add_bias32(g, p.bias, n, p.N);
+        add_bias32(u, p.bias2, n, p.N);
+    }
+    if (lane == 0) bulk_wait_read0();                      // the tiles' previous tensor stores have read them
+    __syncwarp();
+    if (p.store_gu) {
+        row_to_sw(st, lane, g);
+        row_to_sw(st + 2048, lane, u);
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) g[j] = glu_act(g[j], p.act) * u[j];
+    row_to_sw(st + 4096, lane, g);
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) {
+        if (p.store_gu) {
+            tma_store_2d(tmG, st_s, n, m0);
+            tma_store_2d(tmU, st_s + 2048, n, m0);
+        }
+        tma_store_2d(tmH, st_s + 4096, n, m0);
+        bulk_commit();
+    }
+}
+
+// Its backward: r the accumulators of dh, pg / pu this chunk's saved gate and up values (prefetch_h).
+__device__ __forceinline__ void glu_bwd_chunk(const Params& p, int m0, int n, const uint32_t* r, uint8_t* st,
+                                              uint32_t st_s, int lane, const uint4* pg, const uint4* pu,
+                                              const CUtensorMap* tmG, const CUtensorMap* tmU,
+                                              const CUtensorMap* tmH) {
+    if (n >= p.N || m0 >= p.M) return;                     // warp-uniform
+    if (lane == 0) bulk_wait_read0();
+    __syncwarp();
+    stage_in_sw(st, pg, lane);
+    stage_in_sw(st + 2048, pu, lane);
+    __syncwarp();
+    // 8 columns at a time: the own row's gate and up pieces are replaced by dgate and dup
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        uint4* sg = reinterpret_cast<uint4*>(st + swoff(lane, k));
+        uint4* su = reinterpret_cast<uint4*>(st + 2048 + swoff(lane, k));
+        float g[8], u[8], h[8];
+        h8_to_f(*sg, g);
+        h8_to_f(*su, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = __uint_as_float(r[8 * k + j]);
+            float a, da;
+            glu_act_grad(g[j], p.act, a, da);
+            h[j] = a * u[j];
+            g[j] = d * u[j] * da;
+            u[j] = d * a;
+        }
+        *sg = f_to_h8(g);
+        *su = f_to_h8(u);
+        if (p.store_h) *reinterpret_cast<uint4*>(st + 4096 + swoff(lane, k)) = f_to_h8(h);
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_2d(tmG, st_s, n, m0);
+        tma_store_2d(tmU, st_s + 2048, n, m0);
+        if (p.store_h) tma_store_2d(tmH, st_s + 4096, n, m0);
+        bulk_commit();
+    }
+}
+
 // FP32 epilogues (ACC_F32, STORE_F32) of one 32 x 32 chunk through bulk tensor operations: two
 // 32-row x 16-column halves (64-byte rows, the same 64-byte swizzle as the FP16 tiles) leave
 // through the warp's 2 KB tile, each half as one tensor reduce-add into C (ACC_F32) or one tensor
@@ -776,9 +888,9 @@ __device__ __forceinline__ void add_f16x2(float& c0, float& c1, uint32_t a) {
 constexpr int kRowWarps = 5;                    // ROW: row warp w owns operand stage w
 template <int EPI, bool ROW>
 struct PairEpi {
-    static constexpr bool TMA = EPI == RBK_EPI_STORE_F16 || EPI == RBK_EPI_BIAS_GELU || EPI == RBK_EPI_GELU_BWD;
-    static constexpr int STAGES = TMA ? kPairStages : kPairStages - 1;
-    static constexpr int WARP_STAGE = kTmaStageBytes;
+    static constexpr bool TMA = is_f16(EPI);
+    static constexpr int STAGES = TMA && !is_glu(EPI) ? kPairStages : kPairStages - 1;
+    static constexpr int WARP_STAGE = is_glu(EPI) ? 3 * 2048 : kTmaStageBytes;   // gate, up and h tiles
     static constexpr int PART_BYTES = ROW ? kRowWarps * BM * 4 : 0;     // per-warp row partials
     static constexpr int SMEM = 1024 + STAGES * (BM * BK * 2 + 128 * BK * 2) + kEpiWarps * WARP_STAGE +
                                 PART_BYTES + 256;
@@ -800,7 +912,8 @@ __global__ void __launch_bounds__(PairEpi<EPI, ROW>::THREADS, 1)
     constexpr int BN = 256, HALF_N = 128;
     constexpr int A_BYTES = BM * BK * 2, B_BYTES = HALF_N * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
     constexpr int STAGES = PairEpi<EPI, ROW>::STAGES;
-    constexpr bool kTma = EPI == RBK_EPI_STORE_F16 || EPI == RBK_EPI_BIAS_GELU || EPI == RBK_EPI_GELU_BWD;
+    constexpr bool kTma = is_f16(EPI);
+    constexpr int TILE_N = EPI == kEpiGlu ? HALF_N : BN;             // columns of C of a tile
     constexpr int kWarpStage = PairEpi<EPI, ROW>::WARP_STAGE;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = su32(smem_raw);
@@ -865,7 +978,9 @@ __global__ void __launch_bounds__(PairEpi<EPI, ROW>::THREADS, 1)
             for (int u = pair; u < p.units && !*abort_flag; u += num_pairs) {
                 int mb, nb, kb0, kb1;
                 decode_unit(p, u, mb, nb, kb0, kb1);
-                const int m0 = mb * 2 * BM + (int)rank * BM, n0 = nb * BN + (int)rank * HALF_N;
+                const int m0 = mb * 2 * BM + (int)rank * BM;
+                // kEpiGlu: rows nb * 128 .. of the gate's half of B in the even CTA, of the up half in the odd
+                const int n0 = EPI == kEpiGlu ? nb * TILE_N + (int)rank * p.N : nb * BN + (int)rank * HALF_N;
                 bool ok = true;
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag)) { ok = false; break; }
@@ -1048,7 +1163,7 @@ __global__ void __launch_bounds__(PairEpi<EPI, ROW>::THREADS, 1)
         // ------------------------------ epilogue (both CTAs) -----------------
         const int q = warp & 3;
         const int half_id = (warp - 2) / 4;
-        constexpr int kChunks = BN / 32;
+        constexpr int kChunks = TILE_N / 32;
         const int c0 = half_id * (kChunks / 2), c1 = half_id ? kChunks : kChunks / 2;
         uint8_t* my_stage = gbase + (epi_stage - base) + (warp - 2) * kWarpStage;
         const uint32_t my_stage_s = epi_stage + (warp - 2) * kWarpStage;
@@ -1065,8 +1180,12 @@ __global__ void __launch_bounds__(PairEpi<EPI, ROW>::THREADS, 1)
             constexpr bool kOwn = EPI == RBK_EPI_ACC_F32;        // C values the owner adds to, one chunk ahead
             const bool own = kOwn && mode == kAccOwner;
             const int lda = p.ld_aux ? p.ld_aux : p.ldc;
-            uint4 pf[4];
+            uint4 pf[4], pu[EPI == kEpiGluBwd ? 4 : 1];
             float4 cpf[kOwn ? 8 : 1];
+            if constexpr (EPI == kEpiGluBwd) {
+                prefetch_h(pf, p.aux, lda, m0, nb * BN + c0 * 32, p, lane);
+                prefetch_h(pu, p.aux2, lda, m0, nb * BN + c0 * 32, p, lane);
+            }
             if (kAux && p.aux) prefetch_h(pf, p.aux, lda, m0, nb * BN + c0 * 32, p, lane);
             if constexpr (kOwn) {
                 if (own) load_c_row(cpf, p, m0, nb * BN + c0 * 32, lane);
@@ -1076,12 +1195,25 @@ __global__ void __launch_bounds__(PairEpi<EPI, ROW>::THREADS, 1)
             const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + buf * BN;
 #pragma unroll 1
             for (int c = c0; c < c1; ++c) {
-                uint32_t r[32];
+                uint32_t r[32], ru[EPI == kEpiGlu ? 32 : 1];
                 tmem_ld32(tbase + c * 32, r);
+                if constexpr (EPI == kEpiGlu) tmem_ld32(tbase + HALF_N + c * 32, ru);
                 uint4 cur[4] = {pf[0], pf[1], pf[2], pf[3]};
                 if (kAux && p.aux && c + 1 < c1) prefetch_h(pf, p.aux, lda, m0, nb * BN + (c + 1) * 32, p, lane);
+                if constexpr (EPI == kEpiGluBwd) {
+                    uint4 curu[4] = {pu[0], pu[1], pu[2], pu[3]};
+                    if (c + 1 < c1) {
+                        prefetch_h(pf, p.aux, lda, m0, nb * BN + (c + 1) * 32, p, lane);
+                        prefetch_h(pu, p.aux2, lda, m0, nb * BN + (c + 1) * 32, p, lane);
+                    }
+                    tmem_wait_ld();
+                    glu_bwd_chunk(p, m0, nb * BN + c * 32, r, my_stage, my_stage_s, lane, cur, curu, &tmC, &tmX, &tmP);
+                    continue;
+                }
                 tmem_wait_ld();
-                if constexpr (kTma) {
+                if constexpr (EPI == kEpiGlu) {
+                    glu_chunk(p, m0, nb * TILE_N + c * 32, r, ru, my_stage, my_stage_s, lane, &tmC, &tmX, &tmP);
+                } else if constexpr (kTma) {
                     epilogue_chunk_tma<EPI>(p, m0, nb * BN + c * 32, r, my_stage, my_stage_s, lane, cur, &tmC, &tmX, sc);
                 } else {
                     float4 cv[kOwn ? 8 : 1];
@@ -1148,7 +1280,7 @@ int launch_pair(rbk_ctx* ctx, const rbk_gemm_desc* d, Params& p, cudaStream_t st
     CUtensorMap ta, tb, tc_, tx, tp;
     // FP16 outputs: 32 x 32 store boxes over the logical [M, N] (ldc / ld_aux pitches); FP32
     // outputs: 16 x 32 boxes (64-byte rows), the split planes of deterministic mode a 3-D map
-    constexpr bool kTma = EPI == RBK_EPI_STORE_F16 || EPI == RBK_EPI_BIAS_GELU || EPI == RBK_EPI_GELU_BWD;
+    constexpr bool kTma = is_f16(EPI);
     memset(&tc_, 0, sizeof(tc_));
     memset(&tx, 0, sizeof(tx));
     memset(&tp, 0, sizeof(tp));
@@ -1196,6 +1328,39 @@ int launch_pair(rbk_ctx* ctx, const rbk_gemm_desc* d, Params& p, cudaStream_t st
     return RBK_OK;
 }
 
+// The gated feed-forward tiles: maps of gate, up and h (dgate, dup and h) instead of one C.
+template <int EPI>
+int launch_glu(rbk_ctx* ctx, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tg,
+               const CUtensorMap& tu, const CUtensorMap& th, const Params& p, cudaStream_t st) {
+    constexpr int SMEM = PairEpi<EPI, false>::SMEM;
+    static_assert(SMEM <= 232448, "shared memory budget");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(PairEpi<EPI, false>::THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    static int configured_device = -1, max_pairs = 0;
+    if (configured_device != ctx->device) {
+        RBK_CUDA(cudaFuncSetAttribute(gemm_pair_kernel<EPI, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        cfg.gridDim = dim3(ctx->num_sms & ~1);
+        int n = 0;
+        RBK_CUDA(cudaOccupancyMaxActiveClusters(&n, gemm_pair_kernel<EPI, false>, &cfg));
+        max_pairs = n > 0 ? n : ctx->num_sms / 2;
+        configured_device = ctx->device;
+    }
+    cfg.gridDim = dim3(2 * (p.units < max_pairs ? p.units : max_pairs));
+    cfg.numAttrs = set_pdl(attr, 1);
+    RBK_CUDA(cudaLaunchKernelEx(&cfg, gemm_pair_kernel<EPI, false>, ta, tb, tg, tu, th, p));
+    RBK_LAUNCHED("gemm_pair_kernel (gated)");
+    return RBK_OK;
+}
+
 // CTA pairs unless RBK_GEMM_SINGLE=1 (the 1-CTA kernel for every N = 256 problem).
 static bool pair_tiles() {
     static const int v = [] {
@@ -1205,7 +1370,65 @@ static bool pair_tiles() {
     return v != 0;
 }
 
+// Fields that the gated tiles and the others share: one split, tiles of 256 rows x tile_n columns.
+static Params glu_params(rbk_ctx* ctx, int M, int F, int K, int tile_n, int act) {
+    Params p = {};
+    p.M = M; p.N = F; p.K = K;
+    p.m_blocks = (M + 2 * BM - 1) / (2 * BM);
+    p.n_blocks = (F + tile_n - 1) / tile_n;
+    p.k_blocks = p.kb_per_split = (K + BK - 1) / BK;
+    p.splits = 1;
+    p.units = p.m_blocks * p.n_blocks;
+    p.alpha = 1.0f;
+    p.act = act;
+    p.err = ctx->tickets + kGemmError;
+    return p;
+}
+static int half_map(CUtensorMap* tm, const void* ptr, int cols, int rows, int64_t ld) {
+    if (!ptr) return memset(tm, 0, sizeof(*tm)), RBK_OK;
+    return make_tmap(tm, ptr, cols, rows, ld, 32, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 }  // namespace gemm
+
+int glu_fwd_tiles(rbk_ctx* ctx, void* h, void* gu, const void* x, int ldx, const void* wgu, const void* bgu, int N, int D,
+                  int F, int act, cudaStream_t st) {
+    using namespace gemm;
+    Params p = glu_params(ctx, N, F, D, 128, act);
+    p.bias = (const half*)bgu;
+    p.bias2 = bgu ? p.bias + F : nullptr;
+    p.store_gu = gu != nullptr;
+    half* g = (half*)gu;
+    CUtensorMap ta, tb, tg, tu, th;
+    RBK_TRY(make_tmap(&ta, x, D, N, ldx, 64, 128));
+    RBK_TRY(make_tmap(&tb, wgu, D, 2 * (uint64_t)F, D, 64, 128));
+    RBK_TRY(half_map(&tg, g, F, N, 2 * (int64_t)F));
+    RBK_TRY(half_map(&tu, g ? g + F : nullptr, F, N, 2 * (int64_t)F));
+    RBK_TRY(half_map(&th, h, F, N, F));
+    ProfScope prof(ctx, st, kCatGemm, 4.0 * N * (double)D * F, 0);
+    return launch_glu<kEpiGlu>(ctx, ta, tb, tg, tu, th, p, st);
+}
+
+int glu_bwd_tiles(rbk_ctx* ctx, void* dgu, void* h, const void* dy, int lddy, const void* wd, const void* gu, int N, int D,
+                  int F, int act, cudaStream_t st) {
+    using namespace gemm;
+    Params p = glu_params(ctx, N, F, D, 256, act);
+    p.b_mn = 1;                                             // B(n = f, k = d) = Wd[d, f]
+    p.aux = (const half*)gu;
+    p.aux2 = p.aux + F;
+    p.ld_aux = 2 * F;
+    p.store_h = h != nullptr;
+    half* g = (half*)dgu;
+    CUtensorMap ta, tb, tg, tu, th;
+    RBK_TRY(make_tmap(&ta, dy, D, N, lddy, 64, 128));
+    RBK_TRY(make_tmap(&tb, wd, F, D, F, 64, 64));
+    RBK_TRY(half_map(&tg, g, F, N, 2 * (int64_t)F));
+    RBK_TRY(half_map(&tu, g + F, F, N, 2 * (int64_t)F));
+    RBK_TRY(half_map(&th, h, F, N, F));
+    ProfScope prof(ctx, st, kCatGemm, 2.0 * N * (double)D * F, 1);
+    return launch_glu<kEpiGluBwd>(ctx, ta, tb, tg, tu, th, p, st);
+}
+
 }  // namespace rbk
 
 using namespace rbk;
@@ -1296,6 +1519,8 @@ int rbk_gemm(rbk_ctx* ctx, const rbk_gemm_desc* d, void* stream) {
     p.err = ctx->tickets + kGemmError;
     p.part = nullptr;
     p.part_rows = nullptr;
+    p.bias2 = p.aux2 = nullptr;
+    p.act = p.store_gu = p.store_h = 0;
     p.ldp = (d->N + 3) & ~3;
     p.c_zero = epi == RBK_EPI_ACC_F32 && ctx->gemm_c_zero;
     const bool det = epi == RBK_EPI_ACC_F32 && p.splits > 1 && ctx->deterministic;

@@ -61,6 +61,19 @@ class QkArgs(C.Structure):
                 ("dgq", vp), ("dgk", vp), ("accumulate", i32), ("ws", vp)]
 
 
+class FfnArgs(C.Structure):
+    """rbk_ffn_args (include/rbk.h)."""
+    _fields_ = [("N", i32), ("D", i32), ("F", i32), ("act", i32), ("x", vp), ("ldx", i32), ("wgu", vp), ("bgu", vp),
+                ("wd", vp), ("bd", vp), ("residual", vp), ("ldr", i32), ("y", vp), ("ldy", i32), ("gu", vp), ("h", vp)]
+
+
+class FfnBwdArgs(C.Structure):
+    """rbk_ffn_bwd_args (include/rbk.h)."""
+    _fields_ = [("N", i32), ("D", i32), ("F", i32), ("act", i32), ("dy", vp), ("lddy", i32), ("x", vp), ("ldx", i32),
+                ("gu", vp), ("wgu", vp), ("wd", vp), ("h", vp), ("recompute_h", i32), ("dgu", vp), ("dx", vp),
+                ("lddx", i32), ("dwgu", vp), ("dbgu", vp), ("dwd", vp), ("dbd", vp)]
+
+
 class Config(C.Structure):
     _fields_ = [("V", i32), ("T", i32), ("D", i32), ("H", i32), ("L", i32), ("FF", i32)]
 
@@ -118,6 +131,8 @@ _SIGS = {
     "rbk_attn_bwd": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, vp]),
     "rbk_qk_norm_rope_fwd": (i32, [vp, C.POINTER(QkArgs), vp]),
     "rbk_qk_norm_rope_bwd": (i32, [vp, C.POINTER(QkArgs), vp]),
+    "rbk_gated_ffn_fwd": (i32, [vp, C.POINTER(FfnArgs), vp]),
+    "rbk_gated_ffn_bwd": (i32, [vp, C.POINTER(FfnBwdArgs), vp]),
     "rbk_model_create": (i32, [C.POINTER(vp), C.POINTER(Config), C.POINTER(ModelOpts)]),
     "rbk_model_destroy": (i32, [vp]),
     "rbk_model_buffer": (i32, [vp, i32, C.POINTER(vp), C.POINTER(i64)]),

@@ -12,7 +12,7 @@ import threading
 
 import torch
 
-from ._lib import GemmDesc, Heads, QkArgs, Scaler, TailArgs, call, lib
+from ._lib import FfnArgs, FfnBwdArgs, GemmDesc, Heads, QkArgs, Scaler, TailArgs, call, lib
 
 EPI_STORE_F16, EPI_BIAS_GELU, EPI_GELU_BWD, EPI_ACC_F32, EPI_STORE_F32 = range(5)
 LN_REFERENCE_FORMULA = 1
@@ -370,3 +370,90 @@ def qk_norm_rope_bwd(dyq, dyk, q, k, gq=None, gk=None, positions=None, pos0=0, t
     a.ws = ws.data_ptr()
     call("rbk_qk_norm_rope_bwd", ctx().handle, C.byref(a), _s())
     return dq, dk, dgq, dgk
+
+
+# ------------------------------------------------------ gated feed-forward --
+
+ACT_SILU, ACT_GELU = range(2)
+_ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU}
+
+
+def _rows(t, name, shape):
+    """A half [N, D] tensor with contiguous rows; returns its row stride."""
+    _need_here(t, torch.float16, name, shape)
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: expected contiguous rows, got strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _whole(t, dtype, name, shape):
+    _need_here(t, dtype, name, shape)
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor, got strides {t.stride()}")
+
+
+def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save=True, out=None):
+    """y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd + residual (rbk_gated_ffn_fwd).
+
+    x [N, D], wgu [2F, D] (gate rows, then up rows), wd [D, F], biases [2F] and [D]: half.  act: "silu" or "gelu"
+    (tanh form).  Returns (y, gu, h): gu [N, 2F] the two projections, for gated_ffn_bwd (None with save False),
+    and h [N, F] the product.  out: y, may be residual."""
+    a = FfnArgs()
+    a.N, a.D = x.shape
+    a.F = wd.shape[1]
+    a.act = _ACTS[act]
+    a.ldx = _rows(x, "x", (a.N, a.D))
+    _whole(wgu, torch.float16, "wgu", (2 * a.F, a.D))
+    _whole(wd, torch.float16, "wd", (a.D, a.F))
+    y = torch.empty(a.N, a.D, dtype=torch.float16, device=x.device) if out is None else out
+    a.ldy = _rows(y, "out", (a.N, a.D))
+    a.x, a.wgu, a.wd, a.y = x.data_ptr(), wgu.data_ptr(), wd.data_ptr(), y.data_ptr()
+    if bgu is not None:
+        _whole(bgu, torch.float16, "bgu", (2 * a.F,))
+        a.bgu = bgu.data_ptr()
+    if bd is not None:
+        _whole(bd, torch.float16, "bd", (a.D,))
+        a.bd = bd.data_ptr()
+    if residual is not None:
+        a.ldr = _rows(residual, "residual", (a.N, a.D))
+        a.residual = residual.data_ptr()
+    h = torch.empty(a.N, a.F, dtype=torch.float16, device=x.device)
+    a.h = h.data_ptr()
+    gu = torch.empty(a.N, 2 * a.F, dtype=torch.float16, device=x.device) if save else None
+    if save:
+        a.gu = gu.data_ptr()
+    call("rbk_gated_ffn_fwd", ctx().handle, C.byref(a), _s())
+    return y, gu, h
+
+
+def gated_ffn_bwd(dy, x, gu, wgu, wd, act="silu", h=None, want_dx=True, dwgu=None, dbgu=None, dwd=None, dbd=None,
+                  dgu=None):
+    """Its backward (rbk_gated_ffn_bwd) from the saved gu.  h: the forward's, or None to have it computed again.
+    dwgu [2F, D], dbgu [2F], dwd [D, F], dbd [D]: FP32, accumulate; those left out are not computed.  dgu: may be gu.
+    Returns (dx or None, dgu, h)."""
+    a = FfnBwdArgs()
+    a.N, a.D = dy.shape
+    a.F = wd.shape[1]
+    a.act = _ACTS[act]
+    a.lddy, a.ldx = _rows(dy, "dy", (a.N, a.D)), _rows(x, "x", (a.N, a.D))
+    _whole(gu, torch.float16, "gu", (a.N, 2 * a.F))
+    _whole(wgu, torch.float16, "wgu", (2 * a.F, a.D))
+    _whole(wd, torch.float16, "wd", (a.D, a.F))
+    a.dy, a.x, a.gu, a.wgu, a.wd = (t.data_ptr() for t in (dy, x, gu, wgu, wd))
+    a.recompute_h = int(h is None)
+    h = torch.empty(a.N, a.F, dtype=torch.float16, device=dy.device) if h is None else h
+    _whole(h, torch.float16, "h", (a.N, a.F))
+    dgu = torch.empty_like(gu) if dgu is None else dgu
+    _whole(dgu, torch.float16, "dgu", gu.shape)
+    a.h, a.dgu = h.data_ptr(), dgu.data_ptr()
+    dx = None
+    if want_dx:
+        dx = torch.empty(a.N, a.D, dtype=torch.float16, device=dy.device)
+        a.dx, a.lddx = dx.data_ptr(), a.D
+    for name, t, shape in (("dwgu", dwgu, (2 * a.F, a.D)), ("dbgu", dbgu, (2 * a.F,)), ("dwd", dwd, (a.D, a.F)),
+                           ("dbd", dbd, (a.D,))):
+        if t is not None:
+            _whole(t, torch.float32, name, shape)
+            setattr(a, name, t.data_ptr())
+    call("rbk_gated_ffn_bwd", ctx().handle, C.byref(a), _s())
+    return dx, dgu, h

@@ -6,6 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+import ffn_ref   # noqa: E402
 import qk_ref   # noqa: E402
 
 P = 1 << 20     # an aligned address that no refused call reads
@@ -77,6 +78,79 @@ def test_qk_gradient_formula_against_differences():
                 assert abs((hi - lo) / (2 * step) - float(d.view(-1)[i])) < 1e-7
 
 
+def ffn(**kw):
+    from rbk._lib import FfnArgs
+    a = FfnArgs()
+    a.N, a.D, a.F, a.ldx, a.ldy, a.ldr = 4, 64, 128, 64, 64, 64
+    a.x = a.wgu = a.bgu = a.wd = a.bd = a.residual = a.y = a.gu = a.h = P
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_ffn_fwd_refusals():
+    n = "rbk_gated_ffn_fwd"
+    for kw, match in [
+        (dict(N=-1), "negative"), (dict(D=0), "multiples of 8"), (dict(D=60), "multiples of 8"),
+        (dict(F=-8), "multiples of 8"), (dict(F=12), "multiples of 8"), (dict(act=2), "act"), (dict(act=-1), "act"),
+        (dict(x=None), "x is NULL"), (dict(wgu=None), "wgu is NULL"), (dict(wd=None), "wd is NULL"),
+        (dict(y=None), "y is NULL"), (dict(h=None), "h is NULL"), (dict(x=P + 2), "x must be 16-byte"),
+        (dict(bgu=P + 8), "bgu must be"), (dict(bd=P + 8), "bd must be"), (dict(gu=P + 8), "gu must be"),
+        (dict(residual=P + 4), "residual must be"), (dict(ldx=56), "stride of x"), (dict(ldx=68), "stride of x"),
+        (dict(ldy=0), "stride of y"), (dict(ldr=8), "stride of residual"),
+    ]:
+        refused(n, ffn(**kw), match)
+    refused(n, ffn(), "ctx is NULL")
+    refused(n, ffn(bgu=None, bd=None, residual=None, ldr=0, gu=None), "ctx is NULL")
+
+
+def test_ffn_bwd_refusals():
+    from rbk._lib import FfnBwdArgs
+
+    def args(**kw):
+        a = FfnBwdArgs()
+        a.N, a.D, a.F, a.lddy, a.ldx, a.lddx = 4, 64, 128, 64, 64, 64
+        for k in ("dy", "x", "gu", "wgu", "wd", "h", "dgu", "dx", "dwgu", "dbgu", "dwd", "dbd"):
+            setattr(a, k, P)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    n = "rbk_gated_ffn_bwd"
+    for kw, match in [
+        (dict(N=-2), "negative"), (dict(D=4), "multiples of 8"), (dict(act=7), "act"), (dict(dwgu=None), "dbgu needs"),
+        (dict(dwd=None), "dbd needs"), (dict(dy=None), "dy is NULL"), (dict(x=None), "x is NULL"),
+        (dict(gu=None), "gu is NULL"), (dict(wgu=None), "wgu is NULL"), (dict(wd=None), "wd is NULL"),
+        (dict(h=None), "h is NULL"), (dict(dgu=None), "dgu is NULL"), (dict(dgu=P + 8), "dgu must be"),
+        (dict(lddy=60), "stride of dy"), (dict(lddx=32), "stride of dx"), (dict(dwgu=P + 4), "dwgu must be"),
+    ]:
+        refused(n, args(**kw), match)
+    refused(n, args(), "ctx is NULL")
+    refused(n, args(dwgu=None, dbgu=None, dwd=None, dbd=None, dx=None, x=None, wgu=None, h=None), "ctx is NULL")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_ffn_gradient_formula_against_differences(act):
+    """The reference's gradient, in float64, against central differences of its forward."""
+    torch.manual_seed(1)
+    N, D, F = 3, 8, 16
+    x, wgu, wd, dy = (torch.randn(*s, dtype=torch.float64) for s in ((N, D), (2 * F, D), (D, F), (N, D)))
+
+    def y(x, wgu, wd):
+        return float((ffn_ref.fwd(x, wgu, wd, None, None, None, act)["y"][0] * dy).sum())
+
+    g = ffn_ref.bwd(dy, x, x @ wgu.T, wgu, wd, act)
+    args = [x, wgu, wd]
+    for i, name in enumerate(("dx", "dwgu", "dwd")):
+        for j in range(0, args[i].numel(), 5):
+            e = torch.zeros_like(args[i])
+            e.view(-1)[j] = 1e-6
+            up = [t + e if k == i else t for k, t in enumerate(args)]
+            lo = [t - e if k == i else t for k, t in enumerate(args)]
+            want = (y(*up) - y(*lo)) / 2e-6
+            assert abs(want - float(g[name][0].reshape(-1)[j])) < 1e-6 * (1 + abs(want))
+
+
 def test_args_layouts_match_header(tmp_path):
     """The ctypes mirrors of the block operators' argument structs have the C compiler's field offsets."""
     import os
@@ -86,7 +160,8 @@ def test_args_layouts_match_header(tmp_path):
         pytest.skip("no gcc")
     from rbk import _lib
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    structs = [("rbk_heads", _lib.Heads), ("rbk_qk_args", _lib.QkArgs)]
+    structs = [("rbk_heads", _lib.Heads), ("rbk_qk_args", _lib.QkArgs), ("rbk_ffn_args", _lib.FfnArgs),
+               ("rbk_ffn_bwd_args", _lib.FfnBwdArgs)]
     lines, want = [], []
     for cname, cls in structs:
         for f, _ in cls._fields_:

@@ -1,0 +1,196 @@
+"""rbk_gated_ffn_fwd / _bwd against float64, element by element, within the bounds of ffn_ref.py."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import ffn_ref as ref   # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from rbk import ops as o
+    torch.cuda.set_device(0)
+    return o
+
+
+def within(name, got, want, bound):
+    over = (got.double() - want).abs() - bound
+    assert bool((over <= 0).all()), f"{name}: off by up to {float(over.max())} more than the bound"
+
+
+def case(N, D, F, bias=False, res=False, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + 31 * N + D + 7 * F)
+
+    def r(*shape, scale=1.0):
+        return (scale * torch.randn(*shape, device="cuda", generator=g)).half()
+
+    return dict(x=r(N, D), wgu=r(2 * F, D, scale=D ** -0.5), wd=r(D, F, scale=F ** -0.5),
+                bgu=r(2 * F, scale=0.3) if bias else None, bd=r(D, scale=0.3) if bias else None,
+                residual=r(N, D) if res else None, dy=r(N, D))
+
+
+SIZES = [(1, 8, 8), (1, 64, 128), (2, 72, 24), (7, 520, 40), (8, 256, 264), (9, 64, 1000), (16, 136, 16), (17, 776, 520),
+         (31, 8, 2056), (32, 1024, 72), (33, 8, 8), (33, 64, 24), (64, 264, 136), (129, 72, 520), (257, 512, 1032),
+         (300, 776, 256), (1000, 136, 2056), (2500, 256, 640)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("N,D,F", SIZES)
+def test_forward(ops, N, D, F, act):
+    bias, res = N % 2 == 1, F % 16 == 8
+    c = case(N, D, F, bias, res)
+    want = ref.fwd(c["x"], c["wgu"], c["wd"], c["bgu"], c["bd"], c["residual"], act)
+    how = dict(bgu=c["bgu"], bd=c["bd"], residual=c["residual"], act=act)
+    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], **how)
+    for name, t in (("gu", gu), ("h", h), ("y", y)):
+        within(name, t, *want[name])
+    y2, none, h2 = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], save=False, **how)
+    assert none is None and torch.equal(y, y2) and torch.equal(h, h2)
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("N,D,F", SIZES)
+def test_backward(ops, N, D, F, act):
+    c = case(N, D, F, seed=1)
+    gu = (c["x"].float() @ c["wgu"].float().T).half()
+    want = ref.bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], act)
+    grads = dict(dwgu=torch.zeros(2 * F, D, device="cuda"), dbgu=torch.zeros(2 * F, device="cuda"),
+                 dwd=torch.zeros(D, F, device="cuda"), dbd=torch.zeros(D, device="cuda"))
+    dx, dgu, h = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], act=act, **grads)
+    for name, t in dict(grads, dx=dx, dgu=dgu, h=h).items():
+        within(name, t, *want[name])
+    # the forward's h kept, gradients over the saved activations, nothing else asked for
+    over = gu.clone()
+    dx2, dgu2, _ = ops.gated_ffn_bwd(c["dy"], c["x"], over, c["wgu"], c["wd"], act=act, h=h, dgu=over)
+    assert dgu2 is over and torch.equal(dgu2, dgu) and torch.equal(dx2, dx)
+    assert ops.device_error() == 0
+
+
+def test_backward_accumulates_and_reads_the_kept_product(ops):
+    N, D, F = 200, 128, 264
+    c = case(N, D, F, seed=2)
+    gu = (c["x"].float() @ c["wgu"].float().T).half()
+    h = torch.randn(N, F, device="cuda").half()            # not the one gu would give: it must be what dwd reads
+    dwd = torch.full((D, F), 3.0, device="cuda")
+    dx, _, h2 = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], h=h, want_dx=False, dwd=dwd)
+    assert dx is None and h2 is h
+    want = 3.0 + c["dy"].double().T @ h.double()
+    within("dwd", dwd, want, (N + 2) * ref.E * (3.0 + c["dy"].double().abs().T @ h.double().abs()))
+
+
+@pytest.mark.parametrize("N", [5, 100])
+def test_strides_and_what_lies_beside(ops, N):
+    """Row strides of x, residual and y; y over the residual; neighbours of the rows stay as they were."""
+    D, F = 136, 72
+    c = case(N, D, F, True, True, seed=3)
+    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], bgu=c["bgu"], bd=c["bd"], residual=c["residual"])
+    wide = torch.full((N, D + 24), 9.0, device="cuda", dtype=torch.float16)
+    xs, ys = wide.clone()[:, 8:8 + D], wide[:, 16:16 + D]
+    xs.copy_(c["x"])
+    ys.copy_(c["residual"])
+    y2, gu2, h2 = ops.gated_ffn_fwd(xs, c["wgu"], c["wd"], bgu=c["bgu"], bd=c["bd"], residual=ys, out=ys)
+    assert y2 is ys and torch.equal(y2, y) and torch.equal(gu2, gu) and torch.equal(h2, h)
+    assert bool((wide[:, :16] == 9.0).all()) and bool((wide[:, 16 + D:] == 9.0).all())
+    dys = wide.clone()[:, 8:8 + D]
+    dys.copy_(c["dy"])
+    grads = [dict(dwgu=torch.zeros(2 * F, D, device="cuda"), dwd=torch.zeros(D, F, device="cuda")) for _ in range(2)]
+    a = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], **grads[0])
+    b = ops.gated_ffn_bwd(dys, xs, gu, c["wgu"], c["wd"], **grads[1])
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+@pytest.mark.parametrize("N", [6, 70])
+def test_a_row_that_is_not_finite_spoils_itself_only(ops, N):
+    D, F = 64, 136
+    c = case(N, D, F, seed=4)
+    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"])
+    x = c["x"].clone()
+    x[2, 5] = float("nan")
+    x[4, 0] = float("inf")
+    y2, gu2, h2 = ops.gated_ffn_fwd(x, c["wgu"], c["wd"])
+    keep = torch.ones(N, dtype=torch.bool, device="cuda")
+    keep[2] = keep[4] = False
+    for a, b in ((y, y2), (gu, gu2), (h, h2)):
+        assert torch.equal(a[keep], b[keep]) and not bool(b[~keep].isfinite().all(1).any())
+
+
+def test_extreme_gates(ops):
+    """Pre-activations of FP16's largest size: act(-big) is 0, act(big) is big, their slopes 0 and 1."""
+    N, D, F = 3, 8, 16
+    x = torch.ones(N, D, device="cuda", dtype=torch.float16)
+    wgu = torch.zeros(2 * F, D, device="cuda", dtype=torch.float16)
+    wgu[:F // 2, 0], wgu[F // 2:F, 0], wgu[F:, 0] = 60000.0, -60000.0, 0.5
+    wd = torch.zeros(D, F, device="cuda", dtype=torch.float16)
+    wd[0] = 2.0 ** -6
+    dy = torch.ones(N, D, device="cuda", dtype=torch.float16)
+    for act in ("silu", "gelu"):
+        y, gu, h = ops.gated_ffn_fwd(x, wgu, wd, act=act)
+        assert bool((h[:, :F // 2] == 30000).all()) and bool((h[:, F // 2:] == 0).all())
+        dx, dgu, h2 = ops.gated_ffn_bwd(dy, x, gu, wgu, wd, act=act)
+        assert torch.equal(h, h2)
+        d = 2.0 ** -6
+        assert bool((dgu[:, :F // 2] == d * 0.5).all()) and bool((dgu[:, F // 2:F] == 0).all())
+        assert bool((dgu[:, F:F + F // 2] == d * 60000).all()) and bool((dgu[:, F + F // 2:] == 0).all())
+
+
+def test_no_rows(ops):
+    x = torch.empty(0, 64, device="cuda", dtype=torch.float16)
+    wgu, wd = torch.ones(256, 64, device="cuda").half(), torch.ones(64, 128, device="cuda").half()
+    y, gu, h = ops.gated_ffn_fwd(x, wgu, wd)
+    assert y.shape == (0, 64) and gu.shape == (0, 256) and h.shape == (0, 128)
+    dw = torch.ones(256, 64, device="cuda")
+    dx, dgu, _ = ops.gated_ffn_bwd(x, x, gu, wgu, wd, dwgu=dw)
+    assert dx.shape == (0, 64) and bool((dw == 1).all())
+
+
+@pytest.mark.parametrize("N", [3, 200])
+def test_repeats_bits_on_streams_and_in_graphs(ops, N):
+    D, F = 256, 520
+    c = case(N, D, F, True, True, seed=5)
+
+    def both():
+        y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], bgu=c["bgu"], bd=c["bd"], residual=c["residual"])
+        return (y, gu, h) + ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"])
+
+    want = both()
+    assert all(torch.equal(a, b) for a, b in zip(both(), want))
+    graphs = []
+    for _ in range(2):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            both()
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=side):
+                out = both()
+        graphs.append((side, gr, out))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for side, gr, out in graphs:
+            with torch.cuda.stream(side):
+                for t in out:
+                    t.zero_()
+                gr.replay()
+    torch.cuda.synchronize()
+    for _, _, out in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert ops.device_error() == 0
+
+
+def test_refused_tensors(ops):
+    c = case(4, 64, 128)
+    with pytest.raises(ValueError):
+        ops.gated_ffn_fwd(c["x"].float(), c["wgu"], c["wd"])
+    with pytest.raises(ValueError):
+        ops.gated_ffn_fwd(c["x"], c["wgu"][:128], c["wd"])
+    with pytest.raises(ValueError):
+        ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"].T)
+    with pytest.raises(ValueError):
+        ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], bd=c["x"][0].float())
+    with pytest.raises(KeyError):
+        ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], act="relu")
+    with pytest.raises(RuntimeError, match="multiples of 8"):
+        ops.gated_ffn_fwd(c["x"][:, :60], c["wgu"][:, :60].contiguous(), c["wd"][:60].contiguous())
