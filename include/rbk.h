@@ -245,6 +245,34 @@ typedef struct rbk_tail_args {
  * (src/cuda_kernels.cuh:186). */
 int rbk_adam_tail(rbk_ctx* ctx, const rbk_tail_args* args, void* stream);
 
+/* One gradient tensor: n elements at g, FP32, or half when `half` is set, at any
+ * alignment of its type.  out: where the clipped values go: g itself, a range of
+ * its own, or NULL (the tensor counts in the norm and is not written). */
+typedef struct rbk_grad {
+    const void* g;
+    void* out;
+    int64_t n;               /* >= 0                                              */
+    int64_t half;            /* 0: FP32, 1: half                                  */
+} rbk_grad;
+
+/* Global gradient norm and clipping over `count` tensors:
+ *   *norm = sqrt(sum of squares of all elements) / scale   (device FP32)
+ *   out = g * min(1, max_norm / *norm)
+ * scale is scaler->scale (the gradients of a scaled loss keep their scale: the tail
+ * divides it out), or 1 when scaler is NULL.  max_norm <= 0: no clipping, out = g.
+ * Where the norm is at most max_norm, nothing is written in place; where a gradient
+ * is infinite or NaN they all pass unchanged, so the tail finds the overflow and skips
+ * its step.  Squares are summed in FP64, in a fixed order: no finite gradient overflows
+ * the sum, and two runs give the same bits.
+ * Written ranges must not overlap each other or another tensor (RBK_ERR_INVALID);
+ * `tensors` is a host array, read during the call only.  ws: RBK_CLIP_WS_BYTES of
+ * device memory, or NULL for the ctx scratch (see rbk_qk_args.ws).
+ * rbk_adam_tail's own max_norm clips each tensor by itself, as the reference does
+ * (src/model.cu:493-523); this is the norm over all of them, for it to follow. */
+#define RBK_CLIP_WS_BYTES (16 << 10)
+int rbk_clip_grad_norm(rbk_ctx* ctx, const rbk_grad* tensors, int count, float max_norm, const rbk_scaler* scaler,
+                       float* norm, void* ws, void* stream);
+
 /* ------------------------------------------------------------------------
  * GEMM (tcgen05 / TMEM, TMA-fed)
  * ------------------------------------------------------------------------ */

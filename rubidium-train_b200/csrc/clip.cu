@@ -1,0 +1,299 @@
+// clip.cu — the global gradient norm over many tensors, and clipping by it.
+//
+//   norm = sqrt(sum over all tensors of g^2) / scale,   out = g min(1, max_norm / norm)
+//
+// Memory bound: the gradients are read for the norm, and where clipping bites (or out is not g) read again
+// and written.  Two launches, ordered by programmatic dependent launch: every block of the first leaves the
+// FP64 sum of its chunks, every block of the second adds those sums in the same order and scales its chunks.
+// The tensors' addresses travel as kernel parameters, so the call copies nothing to the device and can be
+// captured into a graph.
+//
+// A tensor is cut into chunks of 32 KB whose borders lie on 16-byte boundaries of g: whatever g's alignment, all
+// its vectors but the first and the last are whole.
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "common.cuh"
+
+namespace rbk {
+namespace clip {
+
+constexpr int kThreads = 256;
+constexpr int kChunkBytes = 32 << 10;
+constexpr int kVec = kChunkBytes / 16 / kThreads;        // 16-byte vectors of a chunk per thread
+constexpr int kMaxBlocks = RBK_CLIP_WS_BYTES / 8;        // FP64 sums, of all launches of a call
+
+struct Tensor {
+    const char* g;
+    char* out;
+    long long n;
+    int first;                                           // its first chunk
+    int half;
+};
+// As many tensors as a launch's parameters hold: 900 is 28.8 KB of the 32764 bytes.
+template <int CAP>
+struct Table {
+    Tensor t[CAP];
+    int count, chunks;
+};
+
+// The tensor of chunk c: the last one whose first chunk is <= c.
+template <int CAP>
+__device__ __forceinline__ int tensor_of(const Table<CAP>& tab, int c) {
+    int lo = 0, hi = tab.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab.t[mid].first <= c) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Sum of squares of one 16-byte vector.  FP32 squares go to FP64 one by one: a square may be beyond FP32's
+// range.  FP16 squares are exact in FP32 (22 bits) and eight of them stay far below its largest value.
+__device__ __forceinline__ double squares(const uint4& v, int half) {
+    if (half) {
+        float f[8];
+        h8_to_f(v, f);
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = fmaf(f[i], f[i], s);
+        return s;
+    }
+    const double a = __uint_as_float(v.x), b = __uint_as_float(v.y), c = __uint_as_float(v.z), d = __uint_as_float(v.w);
+    return fma(a, a, b * b) + fma(c, c, d * d);
+}
+
+// Vector i (16 bytes) of the aligned span that holds the tensor; elements outside it read as zero.
+// `skip` = elements between that span's start and g.
+__device__ __forceinline__ uint4 load_vec(const Tensor& t, long long i, int skip) {
+    const int ve = t.half ? 8 : 4;
+    const long long e = i * ve - skip;
+    if (e >= 0 && e + ve <= t.n) return *reinterpret_cast<const uint4*>(t.g + e * (t.half ? 2 : 4));
+    uint4 v = make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < ve; ++j) {
+        if (e + j < 0 || e + j >= t.n) continue;
+        if (t.half) reinterpret_cast<unsigned short*>(&v)[j] = reinterpret_cast<const unsigned short*>(t.g)[e + j];
+        else reinterpret_cast<uint32_t*>(&v)[j] = reinterpret_cast<const uint32_t*>(t.g)[e + j];
+    }
+    return v;
+}
+__device__ __forceinline__ int skip_of(const Tensor& t) {
+    return (int)(reinterpret_cast<uintptr_t>(t.g) & 15u) / (t.half ? 2 : 4);
+}
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// The block's sum of v in thread 0, warps in order.
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double sw[kThreads / 32];
+    v = warp_sum_d(v);
+    if ((threadIdx.x & 31) == 0) sw[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double s = 0.0;
+    if (threadIdx.x == 0)
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) s += sw[w];
+    return s;
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Table<CAP> tab, double* part) {
+    grid_dependency_sync();
+    double acc = 0.0;
+    for (int c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
+        const Tensor& t = tab.t[tensor_of(tab, c)];
+        const int skip = skip_of(t);
+        const long long v0 = (long long)(c - t.first) * (kChunkBytes / 16) + threadIdx.x;
+        uint4 v[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = load_vec(t, v0 + i * kThreads, skip);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) acc += squares(v[i], t.half);
+    }
+    acc = block_sum(acc);
+    if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+// One 16-byte vector times coef, to out (whose alignment is its own).
+__device__ __forceinline__ void store_vec(const Tensor& t, long long i, int skip, uint4 v, float coef) {
+    const int ve = t.half ? 8 : 4;
+    const long long e = i * ve - skip;
+    if (e + ve <= 0 || e >= t.n) return;
+    if (t.half) {
+        float f[8];
+        h8_to_f(v, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= coef;
+        v = f_to_h8(f);
+    } else {
+        v.x = __float_as_uint(__uint_as_float(v.x) * coef);
+        v.y = __float_as_uint(__uint_as_float(v.y) * coef);
+        v.z = __float_as_uint(__uint_as_float(v.z) * coef);
+        v.w = __float_as_uint(__uint_as_float(v.w) * coef);
+    }
+    char* o = t.out + e * (t.half ? 2 : 4);
+    if (e >= 0 && e + ve <= t.n && (reinterpret_cast<uintptr_t>(o) & 15u) == 0) {
+        *reinterpret_cast<uint4*>(o) = v;
+        return;
+    }
+    for (int j = 0; j < ve; ++j) {
+        if (e + j < 0 || e + j >= t.n) continue;
+        if (t.half) reinterpret_cast<unsigned short*>(o)[j] = reinterpret_cast<const unsigned short*>(&v)[j];
+        else reinterpret_cast<uint32_t*>(o)[j] = reinterpret_cast<const uint32_t*>(&v)[j];
+    }
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<CAP> tab, const double* part,
+                                                         int parts, float max_norm, const rbk_scaler* scaler,
+                                                         float* norm_out) {
+    __shared__ float coef_s;
+    grid_dependency_sync();
+    double s = 0.0;
+    for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
+    s = block_sum(s);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(s) / (scaler ? (double)scaler->scale : 1.0);
+        // 1 too for a NaN (no comparison holds) and an infinite norm
+        const bool bites = max_norm > 0.0f && norm > (double)max_norm && norm <= 1.7976931348623157e308;
+        coef_s = bites ? (float)((double)max_norm / norm) : 1.0f;
+        if (norm_out && blockIdx.x == 0) *norm_out = (float)norm;
+    }
+    __syncthreads();
+    const float coef = coef_s;
+    for (int c = tab.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+        const Tensor& t = tab.t[tensor_of(tab, c)];
+        if (!t.out || (t.out == t.g && coef == 1.0f)) continue;
+        const int skip = skip_of(t);
+        const long long v0 = (long long)(c - t.first) * (kChunkBytes / 16) + threadIdx.x;
+        uint4 v[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = load_vec(t, v0 + i * kThreads, skip);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) store_vec(t, v0 + i * kThreads, skip, v[i], coef);
+    }
+}
+
+// Written ranges overlap nothing but the gradient they replace.
+static bool disjoint(const rbk_grad* t, int count) {
+    struct Range {
+        uintptr_t a, b;
+        bool written;
+    };
+    std::vector<Range> r;
+    r.reserve(2 * (size_t)count);
+    for (int i = 0; i < count; ++i) {
+        const uintptr_t bytes = (uintptr_t)t[i].n * (t[i].half ? 2 : 4), g = (uintptr_t)t[i].g, o = (uintptr_t)t[i].out;
+        if (!bytes) continue;
+        r.push_back({g, g + bytes, o == g});
+        if (o && o != g) r.push_back({o, o + bytes, true});
+    }
+    const auto by_start = [](const Range& x, const Range& y) { return x.a < y.a; };
+    if (!std::is_sorted(r.begin(), r.end(), by_start)) std::sort(r.begin(), r.end(), by_start);
+    uintptr_t end = 0, end_written = 0;                  // of the ranges before
+    for (const Range& x : r) {
+        if (x.a < (x.written ? end : end_written)) return false;
+        end = std::max(end, x.b);
+        if (x.written) end_written = std::max(end_written, x.b);
+    }
+    return true;
+}
+
+static int check(const rbk_grad* t, int count, float max_norm, const float* norm, const void* ws) {
+    const char* who = "rbk_clip_grad_norm";
+    RBK_REQUIRE(count >= 0, "%s: negative count", who);
+    RBK_REQUIRE(t || !count, "%s: tensors is NULL", who);
+    RBK_REQUIRE(norm, "%s: norm is NULL", who);
+    RBK_REQUIRE(max_norm == max_norm, "%s: max_norm is NaN", who);
+    RBK_REQUIRE(aligned16(ws), "%s: ws must be 16-byte aligned", who);
+    long long chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        RBK_REQUIRE(t[i].n >= 0, "%s: tensor %d has a negative size", who, i);
+        RBK_REQUIRE(t[i].half == 0 || t[i].half == 1, "%s: tensor %d: half must be 0 or 1", who, i);
+        RBK_REQUIRE(t[i].g || !t[i].n, "%s: tensor %d is NULL", who, i);
+        const uintptr_t es = t[i].half ? 2 : 4;
+        RBK_REQUIRE((uintptr_t)t[i].g % es == 0 && (uintptr_t)t[i].out % es == 0,
+                    "%s: tensor %d is not aligned to its type", who, i);
+        RBK_REQUIRE(t[i].n < (1LL << 40), "%s: tensor %d is too large", who, i);
+        chunks += t[i].n * (long long)es / kChunkBytes + 2;
+        RBK_REQUIRE(chunks < (1LL << 31), "%s: the tensors are too large", who);
+    }
+    try {
+        RBK_REQUIRE(disjoint(t, count), "%s: a written range overlaps another tensor", who);
+    } catch (const std::bad_alloc&) {
+        set_error("%s: out of host memory", who);
+        return RBK_ERR_NOMEM;
+    }
+    return RBK_OK;
+}
+
+// The next tensors that fit one launch, from *at on.
+template <int CAP>
+static void fill(Table<CAP>& tab, const rbk_grad* t, int count, int* at) {
+    tab.count = tab.chunks = 0;
+    for (; *at < count && tab.count < CAP; ++*at) {
+        const rbk_grad& s = t[*at];
+        if (!s.n) continue;
+        const int es = s.half ? 2 : 4;
+        Tensor& d = tab.t[tab.count++];
+        d.g = (const char*)s.g;
+        d.out = (char*)s.out;
+        d.n = s.n;
+        d.half = (int)s.half;
+        d.first = tab.chunks;
+        const long long bytes = (long long)((uintptr_t)s.g & 15u) + s.n * es;
+        tab.chunks += (int)((bytes + kChunkBytes - 1) / kChunkBytes);
+    }
+}
+
+template <int CAP>
+static int run(rbk_ctx* ctx, const rbk_grad* t, int count, float max_norm, const rbk_scaler* scaler, float* norm,
+               double* part, cudaStream_t st) {
+    static_assert(sizeof(Table<CAP>) <= 32000, "kernel parameters");
+    Table<CAP> tab;
+    // each launch of the first kernel has its own stretch of the sums
+    const int launches = std::max(1, (count + CAP - 1) / CAP);
+    const int per = std::max(1, std::min(4 * ctx->num_sms, kMaxBlocks / launches));
+    RBK_REQUIRE(launches * per <= kMaxBlocks, "rbk_clip_grad_norm: more than %d tensors", kMaxBlocks * CAP);
+    int parts = 0;
+    for (int at = 0; at < count;) {
+        fill(tab, t, count, &at);
+        if (!tab.chunks) continue;
+        const int grid = std::min(per, tab.chunks);
+        RBK_CUDA(launch_pdl(squares_kernel<CAP>, dim3(grid), dim3(kThreads), 0, st, tab, part + parts));
+        RBK_LAUNCHED("squares_kernel");
+        parts += grid;
+    }
+    int at = 0;
+    do {
+        fill(tab, t, count, &at);
+        const int grid = std::max(1, std::min(4 * ctx->num_sms, tab.chunks));
+        RBK_CUDA(launch_pdl(scale_kernel<CAP>, dim3(grid), dim3(kThreads), 0, st, tab, (const double*)part, parts,
+                            max_norm, scaler, norm));
+        RBK_LAUNCHED("scale_kernel");
+    } while (at < count);
+    return RBK_OK;
+}
+
+}  // namespace clip
+}  // namespace rbk
+
+using namespace rbk;
+
+extern "C" int rbk_clip_grad_norm(rbk_ctx* ctx, const rbk_grad* tensors, int count, float max_norm,
+                                  const rbk_scaler* scaler, float* norm, void* ws, void* stream) {
+    RBK_TRY(clip::check(tensors, count, max_norm, norm, ws));
+    RBK_TRY(check_device(ctx, "rbk_clip_grad_norm"));
+    if (!ws) RBK_TRY(ctx_scratch(ctx, RBK_CLIP_WS_BYTES, &ws));
+    double bytes = 0.0;
+    for (int i = 0; i < count; ++i) bytes += (tensors[i].out ? 3.0 : 1.0) * tensors[i].n * (tensors[i].half ? 2 : 4);
+    ProfScope prof(ctx, as_stream(stream), kCatOther, bytes);
+    // a table of the size that is needed: the parameters are copied with each launch
+    if (count <= 120) return clip::run<120>(ctx, tensors, count, max_norm, scaler, norm, (double*)ws, as_stream(stream));
+    return clip::run<900>(ctx, tensors, count, max_norm, scaler, norm, (double*)ws, as_stream(stream));
+}

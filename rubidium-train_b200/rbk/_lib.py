@@ -74,6 +74,11 @@ class FfnBwdArgs(C.Structure):
                 ("lddx", i32), ("dwgu", vp), ("dbgu", vp), ("dwd", vp), ("dbd", vp)]
 
 
+class Grad(C.Structure):
+    """rbk_grad (include/rbk.h)."""
+    _fields_ = [("g", vp), ("out", vp), ("n", i64), ("half", i64)]
+
+
 class Config(C.Structure):
     _fields_ = [("V", i32), ("T", i32), ("D", i32), ("H", i32), ("L", i32), ("FF", i32)]
 
@@ -133,6 +138,7 @@ _SIGS = {
     "rbk_qk_norm_rope_bwd": (i32, [vp, C.POINTER(QkArgs), vp]),
     "rbk_gated_ffn_fwd": (i32, [vp, C.POINTER(FfnArgs), vp]),
     "rbk_gated_ffn_bwd": (i32, [vp, C.POINTER(FfnBwdArgs), vp]),
+    "rbk_clip_grad_norm": (i32, [vp, vp, i32, f32, vp, vp, vp, vp]),
     "rbk_model_create": (i32, [C.POINTER(vp), C.POINTER(Config), C.POINTER(ModelOpts)]),
     "rbk_model_destroy": (i32, [vp]),
     "rbk_model_buffer": (i32, [vp, i32, C.POINTER(vp), C.POINTER(i64)]),

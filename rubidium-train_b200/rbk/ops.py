@@ -84,6 +84,12 @@ def _need_here(t, dtype, name, shape=None):
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
+def _whole(t, dtype, name, shape):
+    _need_here(t, dtype, name, shape)
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor, got strides {t.stride()}")
+
+
 # ----------------------------------------------------------------- LayerNorm --
 
 def ln_fwd(x, gamma, beta, eps=1e-5):
@@ -188,6 +194,41 @@ def adam_tail(p32, g, m, v, p16, scaler_buf, lr, b1=0.9, b2=0.999, eps=1e-8, wd=
     a.t = t
     a.scaler = scaler_buf.data_ptr()
     call("rbk_adam_tail", ctx().handle, C.byref(a), _s())
+
+
+RBK_CLIP_WS_BYTES = 16 << 10
+
+
+def clip_grad_norm(grads, max_norm, scaler=None, out=None):
+    """Clip by the norm over all tensors (rbk_clip_grad_norm): returns the FP32 norm [1] of the gradients divided by
+    the loss scale, and multiplies them by min(1, max_norm / norm), in place or into `out`.
+
+    grads: contiguous FP32 or half tensors.  scaler: a new_scaler() buffer (None: no loss scale).  out: a tensor for each
+    of its gradient's type and size, or None in a place to count that gradient and not write it.  max_norm <= 0: only
+    the norm is computed (and `out` is a copy)."""
+    dev, n = torch.cuda.current_device(), len(grads)
+    norm = torch.empty(1, dtype=torch.float32, device="cuda")
+    vals = []
+    for i, g in enumerate(grads):
+        half = g.dtype == torch.float16
+        if not (half or g.dtype == torch.float32) or not g.is_cuda or g.get_device() != dev or not g.is_contiguous():
+            raise ValueError(f"grads[{i}]: expected a contiguous FP32 or half tensor on cuda:{dev}, got {g.dtype} on "
+                             f"{g.device}")
+        vals += g.data_ptr(), g.data_ptr(), g.numel(), half
+    if out is not None:
+        if len(out) != n:
+            raise ValueError(f"out: expected {n} tensors, got {len(out)}")
+        for i, (g, o) in enumerate(zip(grads, out)):
+            if o is not None and (o.dtype != g.dtype or o.numel() != g.numel() or o.get_device() != dev
+                                  or not o.is_contiguous()):
+                raise ValueError(f"out[{i}]: expected a contiguous {g.dtype} tensor of {g.numel()} elements on cuda:{dev}")
+            vals[4 * i + 1] = 0 if o is None else o.data_ptr()
+    if scaler is not None:
+        _whole(scaler, torch.int32, "scaler", (8,))
+    arr = (C.c_int64 * max(1, 4 * n))(*vals)
+    ws = torch.empty(RBK_CLIP_WS_BYTES, dtype=torch.uint8, device="cuda")
+    call("rbk_clip_grad_norm", ctx().handle, C.addressof(arr), n, max_norm, _p(scaler), _p(norm), _p(ws), _s())
+    return norm
 
 
 # --------------------------------------------------------------------- LoRA --
@@ -384,12 +425,6 @@ def _rows(t, name, shape):
     if t.shape[1] > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: expected contiguous rows, got strides {t.stride()}")
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _whole(t, dtype, name, shape):
-    _need_here(t, dtype, name, shape)
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor, got strides {t.stride()}")
 
 
 def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save=True, out=None):

@@ -151,6 +151,42 @@ def test_ffn_gradient_formula_against_differences(act):
             assert abs(want - float(g[name][0].reshape(-1)[j])) < 1e-6 * (1 + abs(want))
 
 
+def clip(tensors, max_norm=1.0, norm=P, ws=P, count=None):
+    from rbk import lib
+    from rbk._lib import Grad
+    arr = (Grad * max(1, len(tensors)))(*[Grad(*t) for t in tensors])
+    st = lib().rbk_clip_grad_norm(None, C.cast(arr, C.c_void_p), len(tensors) if count is None else count, max_norm,
+                                  None, norm, ws, None)
+    return st, lib().rbk_last_error().decode()
+
+
+@pytest.mark.parametrize("tensors,kw,match", [
+    ([], dict(count=-1), "negative count"), ([], dict(norm=None), "norm is NULL"), ([], dict(ws=P + 8), "ws"),
+    ([], dict(max_norm=float("nan")), "max_norm"), ([(P, P, -1, 0)], {}, "negative size"),
+    ([(P, P, 4, 2)], {}, "half must"), ([(None, None, 4, 0)], {}, "tensor 0 is NULL"),
+    ([(P, P, 4, 0), (P + 66, P + 66, 4, 0)], {}, "tensor 1 is not aligned"), ([(P, P + 101, 4, 1)], {}, "not aligned"),
+    ([(P, P, 1 << 41, 0)], {}, "too large"),
+    ([(P, P, 100, 0), (P, P, 100, 0)], {}, "overlaps"),                       # the same tensor twice
+    ([(P, P, 100, 0), (P + 396, P + 396, 9, 0)], {}, "overlaps"),             # one element shared
+    ([(P, P + 4, 100, 0)], {}, "overlaps"),                                   # shifted over itself
+    ([(P + 4000, P, 100, 0), (P + 300, None, 10, 1)], {}, "overlaps"),        # written over a tensor that is read
+    ([(P, None, 10, 0), (P + 4000, P + 2000, 9, 0), (P + 8000, P + 2032, 9, 0)], {}, "overlaps"),
+])
+def test_clip_refusals(tensors, kw, match):
+    st, msg = clip(tensors, **kw)
+    assert st == -1 and match in msg, (st, msg)
+
+
+@pytest.mark.parametrize("tensors", [
+    [], [(None, None, 0, 0)], [(P, P, 100, 0), (P + 400, P + 400, 7, 0)], [(P + 400, P + 400, 7, 1), (P, P, 100, 0)],
+    [(P, None, 100, 0), (P, None, 100, 0)], [(P, P + 400, 100, 0)], [(P + 2, P + 202, 100, 1)],
+])
+def test_clip_accepts(tensors):
+    """What is not refused for its tensors is refused for the missing context only."""
+    st, msg = clip(tensors)
+    assert st == -1 and "ctx is NULL" in msg
+
+
 def test_args_layouts_match_header(tmp_path):
     """The ctypes mirrors of the block operators' argument structs have the C compiler's field offsets."""
     import os
@@ -161,7 +197,7 @@ def test_args_layouts_match_header(tmp_path):
     from rbk import _lib
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     structs = [("rbk_heads", _lib.Heads), ("rbk_qk_args", _lib.QkArgs), ("rbk_ffn_args", _lib.FfnArgs),
-               ("rbk_ffn_bwd_args", _lib.FfnBwdArgs)]
+               ("rbk_ffn_bwd_args", _lib.FfnBwdArgs), ("rbk_grad", _lib.Grad)]
     lines, want = [], []
     for cname, cls in structs:
         for f, _ in cls._fields_:
