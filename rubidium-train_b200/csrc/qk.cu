@@ -12,25 +12,29 @@
 // Layout: a head is split over G lanes (the power of two >= dh / 16), a lane holding two
 // 16-byte chunks of it, chosen so that both members of every rotated pair are in the
 // same lane: no exchange is needed for the rotation.  A warp works on 32 / G heads of one
-// token at a time, so a token's angles are computed once for all of its heads.
+// token at a time, so a token's angles are computed once for all of its heads, each by one
+// of the lanes that need it (they get it by shuffle).  The loads of a warp's next heads are in
+// flight while it works on its present ones, across tokens too.
+#include <algorithm>
 #include <cmath>
 
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace rbk {
 namespace qk {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kMaxDh = 256;
+constexpr int kMaxParts = 32;                // warps that share a token's heads
 constexpr int kMaxRows = 1024;               // partial rows of the gain gradients (RBK_QK_BWD_WS_BYTES)
 
-struct Heads {
-    half* p;
-    long long sb, ss, sh;
+struct Heads {                               // strides in 16-byte vectors
+    uint4* p;
+    int sb, ss, sh;
 };
 struct Side {                                // the queries or the keys
     int H;
-    int units_per_token, heads_per_unit;     // a warp takes heads_per_unit heads of one token at a time
+    int parts, heads_per_part;               // a warp takes heads_per_part heads of one token at a time
     Heads x, o, dy;
     const half* gain;
 };
@@ -52,62 +56,70 @@ __device__ __forceinline__ void turn(int p, unsigned long long freq, float& c, f
     sincospif((float)(int)(t >> 32) * 4.656612873077393e-10f, &s, &c);      // 2^-31: half turns
 }
 
-// What a lane holds of a head: chunks (8 channels each) a and b.
+// What a lane holds of a head: chunks (8 channels, one vector each) a and b.
 struct Lane {
-    int a, b;                                // channel offsets
+    int a, b;
     bool has_a, has_b, rot_a, rot_b;
 };
 __device__ __forceinline__ Lane lane_of(const Params& p, int j) {
     Lane l;
     const int chunks = p.dh >> 3, rs = p.rot >> 4;
-    int ca, cb;
     if (p.interleaved) {
-        ca = 2 * j;
-        cb = ca + 1;
-        l.rot_a = ca < (p.rot >> 3);
-        l.rot_b = cb < (p.rot >> 3);
+        l.a = 2 * j;
+        l.b = l.a + 1;
+        l.rot_a = l.a < (p.rot >> 3);
+        l.rot_b = l.b < (p.rot >> 3);
     } else {
-        ca = j < rs ? j : 2 * j;
-        cb = j < rs ? j + rs : 2 * j + 1;
+        l.a = j < rs ? j : 2 * j;
+        l.b = j < rs ? j + rs : 2 * j + 1;
         l.rot_a = l.rot_b = j < rs;
     }
-    l.has_a = ca < chunks;
-    l.has_b = cb < chunks;
-    l.a = 8 * ca;
-    l.b = 8 * cb;
+    l.has_a = l.a < chunks;
+    l.has_b = l.b < chunks;
     return l;
 }
 
-// The rotation (sign = 1) or its transpose (sign = -1) on a lane's channels.
-__device__ __forceinline__ void rotate(const Params& p, const Lane& l, float* a, float* b, const float* c,
-                                       const float* s, float sign) {
-    if (p.interleaved) {
+using tc::lo2;
+using tc::hi2;
+using tc::pk2;
+using tc::padd2;
+using tc::psub2;
+using tc::pmul2;
+using tc::pfma2;
+
+// What a lane holds of a head: packed pairs of neighbouring channels, 0..3 of chunk a, 4..7 of chunk b.
+struct Row {
+    uint64_t v[8];
+};
+
+// The rotation, or with T its transpose, of a lane's channels by cs = cosines and sn = sines: packed like the
+// channels when pairs are half a rotation apart, (pair 2i, pair 2i + 1) when they are neighbours.
+template <bool INTER, bool T>
+__device__ __forceinline__ void rotate(const Lane& l, Row& r, const uint64_t* cs, const uint64_t* sn) {
+    if constexpr (INTER) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (l.rot_a) {
-                const float x = a[2 * i], y = a[2 * i + 1], sn = sign * s[i];
-                a[2 * i] = x * c[i] - y * sn;
-                a[2 * i + 1] = x * sn + y * c[i];
-            }
-            if (l.rot_b) {
-                const float x = b[2 * i], y = b[2 * i + 1], sn = sign * s[4 + i];
-                b[2 * i] = x * c[4 + i] - y * sn;
-                b[2 * i + 1] = x * sn + y * c[4 + i];
-            }
+        for (int i = 0; i < 8; ++i) {
+            if (i < 4 ? !l.rot_a : !l.rot_b) continue;
+            const float x = lo2(r.v[i]), y = hi2(r.v[i]);
+            const float c = i & 1 ? hi2(cs[i / 2]) : lo2(cs[i / 2]), s = i & 1 ? hi2(sn[i / 2]) : lo2(sn[i / 2]);
+            r.v[i] = T ? pk2(fmaf(y, s, x * c), fmaf(-x, s, y * c)) : pk2(fmaf(-y, s, x * c), fmaf(x, s, y * c));
         }
     } else if (l.rot_a) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = a[i], y = b[i], sn = sign * s[i];
-            a[i] = x * c[i] - y * sn;
-            b[i] = x * sn + y * c[i];
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t a = r.v[i], b = r.v[4 + i];
+            if (T) {
+                r.v[i] = pfma2(b, sn[i], pmul2(a, cs[i]));
+                r.v[4 + i] = psub2(pmul2(b, cs[i]), pmul2(a, sn[i]));
+            } else {
+                r.v[i] = psub2(pmul2(a, cs[i]), pmul2(b, sn[i]));
+                r.v[4 + i] = pfma2(a, sn[i], pmul2(b, cs[i]));
+            }
         }
     }
 }
 
-__device__ __forceinline__ uint4 load8(const half* p, bool on) {
-    return on ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
-}
+__device__ __forceinline__ uint4 load8(const uint4* p, bool on) { return on ? *p : make_uint4(0, 0, 0, 0); }
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
@@ -115,97 +127,143 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-template <int G, bool BWD>
-__global__ void __launch_bounds__(kThreads) qk_kernel(const __grid_constant__ Params p) {
+// Blocks of an SM: 24 warps at 80 registers forward, 16 at 128 backward.
+template <bool BWD>
+constexpr int kPerSm = BWD ? 2 : 3;
+
+template <int G, bool INTER, bool BWD>
+__global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_constant__ Params p) {
     constexpr int HPW = 32 / G;                                     // heads of a token per warp and step
+    constexpr int ANG = HPW >= 8 ? 1 : 8 / HPW;                     // angles that a lane computes of its slot's 8
     __shared__ float acc_s[BWD ? kWarps : 1][BWD ? kMaxDh : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int which = (int)blockIdx.x >= p.blocks0;
     const Side& sd = p.side[which];
-    const int block = which ? blockIdx.x - p.blocks0 : blockIdx.x;
-    const int blocks = which ? gridDim.x - p.blocks0 : p.blocks0;
+    const int w = (which ? blockIdx.x - p.blocks0 : blockIdx.x) * kWarps + warp;
+    const int stride = max(1, (int)(which ? gridDim.x - p.blocks0 : p.blocks0) * kWarps / sd.parts);   // tokens of a round
     const int g = lane / G, j = lane % G;
     const Lane l = lane_of(p, j);
+    unsigned long long freq[ANG];
+#pragma unroll
+    for (int i = 0; i < ANG; ++i) freq[i] = p.freq[8 * j + (g * ANG + i) % 8];
     grid_dependency_sync();
 
-    float ga[8], gb[8];
-    if (sd.gain) {
-        h8_to_f(load8(sd.gain + l.a, l.has_a), ga);
-        h8_to_f(load8(sd.gain + l.b, l.has_b), gb);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ga[i] = gb[i] = 1.0f;
+    Row gain;
+    {
+        const uint4 one = make_uint4(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u);
+        const uint4* gp = reinterpret_cast<const uint4*>(sd.gain);
+        tc::h8_to_p(gp ? load8(gp + l.a, l.has_a) : one, gain.v);
+        tc::h8_to_p(gp ? load8(gp + l.b, l.has_b) : one, gain.v + 4);
     }
-    float da[8] = {}, db[8] = {};
+    Row acc = {};                                                   // gain gradient
 
-    const long long units = (long long)p.tokens * sd.units_per_token;
-    for (long long u = (long long)block * kWarps + warp; u < units; u += (long long)blocks * kWarps) {
-        const int token = (int)(u / sd.units_per_token), part = (int)(u - (long long)token * sd.units_per_token);
-        const int bi = token / p.S, si = token - bi * p.S;
-        const int pos = p.pos ? p.pos[token] : p.pos0 + si;
-        float c[8], s[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) turn(pos, p.freq[8 * j + i], c[i], s[i]);
-        const half* xt = sd.x.p + bi * sd.x.sb + si * sd.x.ss;
-        half* ot = sd.o.p + bi * sd.o.sb + si * sd.o.ss;
-        const half* dt = BWD ? sd.dy.p + bi * sd.dy.sb + si * sd.dy.ss : nullptr;
-        const int h0 = part * sd.heads_per_unit, h1 = min(sd.H, h0 + sd.heads_per_unit);
-        for (int hb = h0; hb < h1; hb += HPW) {                     // the same trip count in every lane
-            const int h = hb + g;
-            const bool on = h < h1;
-            float a[8], b[8];
-            h8_to_f(load8(xt + h * sd.x.sh + l.a, on && l.has_a), a);
-            h8_to_f(load8(xt + h * sd.x.sh + l.b, on && l.has_b), b);
-            float ss = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
-            if constexpr (!BWD) {
-                const float rstd = rsqrtf(group_sum<G>(ss) * p.inv_dh + p.eps);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    a[i] = a[i] * rstd * ga[i];
-                    b[i] = b[i] * rstd * gb[i];
-                }
-                rotate(p, l, a, b, c, s, 1.0f);
-            } else {
-                float ea[8], eb[8];
-                h8_to_f(load8(dt + h * sd.dy.sh + l.a, on && l.has_a), ea);
-                h8_to_f(load8(dt + h * sd.dy.sh + l.b, on && l.has_b), eb);
-                rotate(p, l, ea, eb, c, s, -1.0f);
-                float wx = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) wx += ea[i] * ga[i] * a[i] + eb[i] * gb[i] * b[i];
-                const float rstd = rsqrtf(group_sum<G>(ss) * p.inv_dh + p.eps);
-                const float t = group_sum<G>(wx) * rstd * p.inv_dh;  // mean(w xhat)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    a[i] *= rstd;
-                    b[i] *= rstd;
-                    da[i] += ea[i] * a[i];
-                    db[i] += eb[i] * b[i];
-                    a[i] = rstd * (ea[i] * ga[i] - a[i] * t);
-                    b[i] = rstd * (eb[i] * gb[i] - b[i] * t);
-                }
-            }
-            if (on && l.has_a) *reinterpret_cast<uint4*>(ot + h * sd.o.sh + l.a) = f_to_h8(a);
-            if (on && l.has_b) *reinterpret_cast<uint4*>(ot + h * sd.o.sh + l.b) = f_to_h8(b);
+    // The heads in flight: token (bi, si), this lane's head and pointers to its chunk a.
+    const int part = w % sd.parts, h0 = part * sd.heads_per_part + g;
+    const int h1 = min(sd.H, (part + 1) * sd.heads_per_part) + g;   // of the group's heads: h - g < h1 - g
+    const int ab = l.b - l.a;
+    int token = w / sd.parts < stride ? w / sd.parts : p.tokens, h = 0, pos = 0;
+    const uint4 *xp = nullptr, *ep = nullptr;
+    uint4* op = nullptr;
+    uint4 xa, xb, ea, eb;
+    auto at = [&](const Heads& t, int bi, int si) {
+        return t.p + ((long long)bi * t.sb + (long long)si * t.ss + (long long)h0 * t.sh + l.a);
+    };
+    auto start = [&] {
+        const int bi = (int)((unsigned)token / (unsigned)p.S), si = token - bi * p.S;
+        pos = p.pos ? p.pos[token] : p.pos0 + si;
+        xp = at(sd.x, bi, si);
+        op = at(sd.o, bi, si);
+        if (BWD) ep = at(sd.dy, bi, si);
+        h = h0;
+    };
+    auto fetch = [&] {
+        const bool on = h < sd.H;
+        xa = load8(xp, on && l.has_a);
+        xb = load8(xp + ab, on && l.has_b);
+        if (BWD) {
+            ea = load8(ep, on && l.has_a);
+            eb = load8(ep + ab, on && l.has_b);
         }
+    };
+    if (token < p.tokens) {
+        start();
+        fetch();
+    }
+    bool fresh = true;
+    uint64_t cs[4], sn[4];
+    while (token < p.tokens) {
+        Row x, e;
+        tc::h8_to_p(xa, x.v);
+        tc::h8_to_p(xb, x.v + 4);
+        if (BWD) {
+            tc::h8_to_p(ea, e.v);
+            tc::h8_to_p(eb, e.v + 4);
+        }
+        const bool on = h < sd.H;
+        uint4* const o = op;
+        if (fresh) {                                                // a new token: its angles
+            float c[ANG], s[ANG];
+#pragma unroll
+            for (int i = 0; i < ANG; ++i) turn(pos, freq[i], c[i], s[i]);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const int s0 = i / ANG * G + j, s1 = (i + 1) / ANG * G + j;
+                cs[i / 2] = pk2(__shfl_sync(0xffffffffu, c[i % ANG], s0), __shfl_sync(0xffffffffu, c[(i + 1) % ANG], s1));
+                sn[i / 2] = pk2(__shfl_sync(0xffffffffu, s[i % ANG], s0), __shfl_sync(0xffffffffu, s[(i + 1) % ANG], s1));
+            }
+        }
+        h += HPW;
+        xp += HPW * (long long)sd.x.sh;
+        op += HPW * (long long)sd.o.sh;
+        if (BWD) ep += HPW * (long long)sd.dy.sh;
+        fresh = h >= h1;                                            // the same in all lanes
+        if (fresh) {
+            token = p.tokens - token > stride ? token + stride : p.tokens;
+            if (token < p.tokens) start();
+        }
+        if (token < p.tokens) fetch();
+
+        uint64_t ss = 0;                                            // two zeros
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = pfma2(x.v[i], x.v[i], ss);
+        if constexpr (!BWD) {
+            const float rstd = rsqrtf(group_sum<G>(lo2(ss) + hi2(ss)) * p.inv_dh + p.eps);
+            const uint64_t r2 = pk2(rstd, rstd);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x.v[i] = pmul2(pmul2(x.v[i], r2), gain.v[i]);
+            rotate<INTER, false>(l, x, cs, sn);
+        } else {
+            rotate<INTER, true>(l, e, cs, sn);
+            uint64_t wx = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) wx = pfma2(pmul2(e.v[i], gain.v[i]), x.v[i], wx);
+            const float rstd = rsqrtf(group_sum<G>(lo2(ss) + hi2(ss)) * p.inv_dh + p.eps);
+            const float t = -group_sum<G>(lo2(wx) + hi2(wx)) * rstd * p.inv_dh;   // -mean(w xhat)
+            const uint64_t r2 = pk2(rstd, rstd), t2 = pk2(t, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint64_t xh = pmul2(x.v[i], r2);
+                acc.v[i] = pfma2(e.v[i], xh, acc.v[i]);
+                x.v[i] = pmul2(pfma2(xh, t2, pmul2(e.v[i], gain.v[i])), r2);
+            }
+        }
+        if (on && l.has_a) o[0] = tc::p_to_h8(x.v);
+        if (on && l.has_b) o[ab] = tc::p_to_h8(x.v + 4);
     }
     if constexpr (BWD) {
         // lanes of the same slot, then the warps, in a fixed order
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
+            float a = lo2(acc.v[i]), b = hi2(acc.v[i]);
 #pragma unroll
             for (int o = G; o < 32; o <<= 1) {
-                da[i] += __shfl_xor_sync(0xffffffffu, da[i], o);
-                db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+                a += __shfl_xor_sync(0xffffffffu, a, o);
+                b += __shfl_xor_sync(0xffffffffu, b, o);
             }
-        }
-        if (g == 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (l.has_a) acc_s[warp][l.a + i] = da[i];
-                if (l.has_b) acc_s[warp][l.b + i] = db[i];
+            const int c = i < 4 ? 8 * l.a + 2 * i : 8 * l.b + 2 * (i - 4);
+            if (g == 0 && (i < 4 ? l.has_a : l.has_b)) {
+                acc_s[warp][c] = a;
+                acc_s[warp][c + 1] = b;
             }
         }
         __syncthreads();
@@ -218,28 +276,40 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const __grid_constant__ Pa
     }
 }
 
-// dgain[c] (+)= sum over the side's partial rows, one warp per channel.
+// dgain[c] (+)= sum over the side's partial rows: a block takes 32 channels, its warps every eighth row, and the
+// warps' sums are added in order.
 __global__ void __launch_bounds__(kThreads) qk_gain_kernel(float* dgq, float* dgk, const float* part, int dh, int rows0,
                                                            int rows, int accumulate) {
-    grid_dependency_sync();
-    const int ch = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    __shared__ float s[kWarps][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = blockIdx.x * 32 + lane;
     const int which = blockIdx.y;
     float* out = which ? dgk : dgq;
-    if (ch >= dh || !out) return;
+    grid_dependency_sync();
     float v = 0.0f;
-    for (int r = (which ? rows0 : 0) + lane; r < (which ? rows : rows0); r += 32) v += part[(size_t)r * dh + ch];
-    v = warp_sum(v);
-    if (lane == 0) out[ch] = accumulate ? out[ch] + v : v;
+    if (ch < dh) {
+        const int end = which ? rows : rows0;
+#pragma unroll 8
+        for (int r = (which ? rows0 : 0) + warp; r < end; r += kWarps) v += part[(size_t)r * dh + ch];
+    }
+    s[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && ch < dh && out) {
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) v += s[w][lane];
+        out[ch] = accumulate ? out[ch] + v : v;
+    }
 }
 
-template <bool BWD>
-int run(rbk_ctx* ctx, const Params& p, int grid, cudaStream_t st) {
+template <bool INTER, bool BWD>
+int run(const Params& p, int grid, cudaStream_t st) {
     const int slots = (p.dh + 15) / 16;
-    if (slots <= 1) RBK_CUDA(launch_pdl(qk_kernel<1, BWD>, dim3(grid), dim3(kThreads), 0, st, p));
-    else if (slots <= 2) RBK_CUDA(launch_pdl(qk_kernel<2, BWD>, dim3(grid), dim3(kThreads), 0, st, p));
-    else if (slots <= 4) RBK_CUDA(launch_pdl(qk_kernel<4, BWD>, dim3(grid), dim3(kThreads), 0, st, p));
-    else if (slots <= 8) RBK_CUDA(launch_pdl(qk_kernel<8, BWD>, dim3(grid), dim3(kThreads), 0, st, p));
-    else RBK_CUDA(launch_pdl(qk_kernel<16, BWD>, dim3(grid), dim3(kThreads), 0, st, p));
+    const dim3 gd(grid), bd(kThreads);
+    if (slots <= 1) RBK_CUDA(launch_pdl(qk_kernel<1, INTER, BWD>, gd, bd, 0, st, p));
+    else if (slots <= 2) RBK_CUDA(launch_pdl(qk_kernel<2, INTER, BWD>, gd, bd, 0, st, p));
+    else if (slots <= 4) RBK_CUDA(launch_pdl(qk_kernel<4, INTER, BWD>, gd, bd, 0, st, p));
+    else if (slots <= 8) RBK_CUDA(launch_pdl(qk_kernel<8, INTER, BWD>, gd, bd, 0, st, p));
+    else RBK_CUDA(launch_pdl(qk_kernel<16, INTER, BWD>, gd, bd, 0, st, p));
     RBK_LAUNCHED("qk_kernel");
     return RBK_OK;
 }
@@ -249,12 +319,15 @@ static int check_heads(const char* who, const char* what, const rbk_heads& t, co
     RBK_REQUIRE(aligned16(t.p), "%s: %s must be 16-byte aligned", who, what);
     RBK_REQUIRE(t.sb % 8 == 0 && t.ss % 8 == 0 && t.sh % 8 == 0, "%s: strides of %s must be multiples of 8 elements",
                 who, what);
+    const int64_t most = 8LL * 0x7fffffff;                           // strides are 32-bit counts of vectors
+    for (const int64_t s : {t.sb, t.ss, t.sh})
+        RBK_REQUIRE(s >= -most && s <= most, "%s: strides of %s must be below 2^34 elements", who, what);
     RBK_REQUIRE(!out || ((t.sb || a->B <= 1) && (t.ss || a->S <= 1) && (t.sh || H <= 1)),
                 "%s: %s is written and must not repeat elements (zero stride)", who, what);
     return RBK_OK;
 }
 
-static Heads heads(const rbk_heads& t) { return {(half*)t.p, t.sb, t.ss, t.sh}; }
+static Heads heads(const rbk_heads& t) { return {(uint4*)t.p, (int)(t.sb / 8), (int)(t.ss / 8), (int)(t.sh / 8)}; }
 
 template <bool BWD>
 int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
@@ -311,13 +384,13 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
         p.freq[i] = t >= 18446744073709551616.0L ? 0 : (unsigned long long)t;
         f *= ratio;
     }
-    // Enough warps to fill the machine first, then as many heads of a token per warp as there are, so that
-    // a token's angles are computed once.
-    const int hpw = [&] {
-        const int slots = (a->dh + 15) / 16;
-        return slots <= 1 ? 32 : slots <= 2 ? 16 : slots <= 4 ? 8 : slots <= 8 ? 4 : 2;
-    }();
-    const int max_blocks = 4 * ctx->num_sms < kMaxRows ? 4 * ctx->num_sms : kMaxRows;
+    // A warp takes all heads of a token where there are tokens for every warp, so that a token's angles are
+    // computed once; with fewer tokens its heads are shared out over up to kMaxParts warps.
+    const int slots = (a->dh + 15) / 16;
+    const int hpw = slots <= 1 ? 32 : slots <= 2 ? 16 : slots <= 4 ? 8 : slots <= 8 ? 4 : 2;
+    const int most = kPerSm<BWD> * ctx->num_sms;
+    const int max_blocks = std::min(most, kMaxRows - 2 * kMaxParts / kWarps);
+    const bool all = (long long)tokens * 2 >= (long long)max_blocks * kWarps;
     long long need[2];
     for (int i = 0; i < 2; ++i) {
         Side& s = p.side[i];
@@ -327,18 +400,17 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
         s.dy = heads(*dy[i]);
         s.gain = (const half*)(i ? a->gk : a->gq);
         const int steps = (H[i] + hpw - 1) / hpw;
-        const bool all = (long long)tokens * 2 >= (long long)max_blocks * kWarps;
-        s.heads_per_unit = all && steps ? steps * hpw : hpw;
-        s.units_per_token = all ? (steps ? 1 : 0) : steps;
-        need[i] = ((long long)tokens * s.units_per_token + kWarps - 1) / kWarps;
+        s.heads_per_part = hpw * (all ? steps : (steps + kMaxParts - 1) / kMaxParts);
+        s.parts = steps ? (H[i] + s.heads_per_part - 1) / s.heads_per_part : 1;
+        need[i] = steps ? ((long long)tokens * s.parts + kWarps - 1) / kWarps : 0;
     }
     cudaStream_t st = as_stream(stream);
     long long nb[2] = {need[0], need[1]};
     if (nb[0] + nb[1] > max_blocks) {                                // in proportion to the heads
-        nb[0] = need[0] ? (long long)max_blocks * a->Hq / (a->Hq + a->Hk) : 0;
-        nb[0] = need[0] && nb[0] < 1 ? 1 : nb[0];
+        nb[0] = (long long)max_blocks * a->Hq / ((long long)a->Hq + a->Hk);
         nb[1] = max_blocks - nb[0];
-        if (need[1] && nb[1] < 1) { nb[1] = 1; nb[0] = max_blocks - 1; }
+        for (int i = 0; i < 2; ++i)                                  // a warp for each part of a token
+            if (need[i]) nb[i] = std::max(nb[i], (long long)(p.side[i].parts + kWarps - 1) / kWarps);
     }
     p.blocks0 = (int)nb[0];
     const int grid = (int)(nb[0] + nb[1]);
@@ -350,9 +422,12 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
     }
     const double n = (double)tokens * (a->Hq + a->Hk) * a->dh;
     ProfScope prof(ctx, st, kCatOther, (BWD ? 6.0 : 4.0) * n);
-    if (grid) RBK_TRY(run<BWD>(ctx, p, grid, st));
+    if (grid) {
+        const int status = a->interleaved ? run<true, BWD>(p, grid, st) : run<false, BWD>(p, grid, st);
+        if (status != RBK_OK) return status;
+    }
     if (BWD && (a->dgq || a->dgk)) {
-        RBK_CUDA(launch_pdl(qk_gain_kernel, dim3((a->dh + kWarps - 1) / kWarps, 2), dim3(kThreads), 0, st, a->dgq, a->dgk,
+        RBK_CUDA(launch_pdl(qk_gain_kernel, dim3((a->dh + 31) / 32, 2), dim3(kThreads), 0, st, a->dgq, a->dgk,
                             (const float*)p.part, a->dh, p.blocks0, grid, a->accumulate));
         RBK_LAUNCHED("qk_gain_kernel");
     }

@@ -138,7 +138,7 @@ _SIGS = {
     "rbk_qk_norm_rope_bwd": (i32, [vp, C.POINTER(QkArgs), vp]),
     "rbk_gated_ffn_fwd": (i32, [vp, C.POINTER(FfnArgs), vp]),
     "rbk_gated_ffn_bwd": (i32, [vp, C.POINTER(FfnBwdArgs), vp]),
-    "rbk_clip_grad_norm": (i32, [vp, vp, i32, f32, vp, vp, vp, vp]),
+    "rbk_clip_grad_norm": (i32, [vp, C.c_char_p, i32, f32, vp, vp, vp, vp]),
     "rbk_model_create": (i32, [C.POINTER(vp), C.POINTER(Config), C.POINTER(ModelOpts)]),
     "rbk_model_destroy": (i32, [vp]),
     "rbk_model_buffer": (i32, [vp, i32, C.POINTER(vp), C.POINTER(i64)]),

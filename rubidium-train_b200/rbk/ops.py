@@ -8,6 +8,7 @@ device of the active context; there is no host or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 
 import torch
@@ -62,7 +63,7 @@ def ctx() -> Context:
 
 
 def _s():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def _p(t):
@@ -74,20 +75,16 @@ def _need(t, dtype, name):
         raise ValueError(f"{name}: expected a contiguous CUDA {dtype} tensor, got {t.dtype} on {t.device}")
 
 
-def _need_here(t, dtype, name, shape=None):
-    """A CUDA tensor of the current device, type and shape (any strides)."""
-    if t.dtype != dtype or not t.is_cuda:
-        raise ValueError(f"{name}: expected a CUDA {dtype} tensor, got {t.dtype} on {t.device}")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+def _here(t, dtype, name, shape, whole=True):
+    """A tensor of this type and shape (contiguous unless whole is False) on the current device; returns its address."""
+    if t.dtype is not dtype or t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"{name}: expected a {dtype} tensor on cuda:{torch.cuda.current_device()}, got {t.dtype} on "
+                         f"{t.device}")
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-
-
-def _whole(t, dtype, name, shape):
-    _need_here(t, dtype, name, shape)
-    if not t.is_contiguous():
+    if whole and not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous tensor, got strides {t.stride()}")
+    return t.data_ptr()
 
 
 # ----------------------------------------------------------------- LayerNorm --
@@ -206,28 +203,26 @@ def clip_grad_norm(grads, max_norm, scaler=None, out=None):
     grads: contiguous FP32 or half tensors.  scaler: a new_scaler() buffer (None: no loss scale).  out: a tensor for each
     of its gradient's type and size, or None in a place to count that gradient and not write it.  max_norm <= 0: only
     the norm is computed (and `out` is a copy)."""
-    dev, n = torch.cuda.current_device(), len(grads)
-    norm = torch.empty(1, dtype=torch.float32, device="cuda")
-    vals = []
+    dev, n = torch._C._cuda_getDevice(), len(grads)
+    f32, f16 = torch.float32, torch.float16
+    kinds = [(g.dtype, g.numel()) for g in grads]
     for i, g in enumerate(grads):
-        half = g.dtype == torch.float16
-        if not (half or g.dtype == torch.float32) or not g.is_cuda or g.get_device() != dev or not g.is_contiguous():
+        if (g.dtype is not f32 and g.dtype is not f16) or g.get_device() != dev or not g.is_contiguous():
             raise ValueError(f"grads[{i}]: expected a contiguous FP32 or half tensor on cuda:{dev}, got {g.dtype} on "
                              f"{g.device}")
-        vals += g.data_ptr(), g.data_ptr(), g.numel(), half
+    at = to = [g.data_ptr() for g in grads]
     if out is not None:
         if len(out) != n:
             raise ValueError(f"out: expected {n} tensors, got {len(out)}")
-        for i, (g, o) in enumerate(zip(grads, out)):
-            if o is not None and (o.dtype != g.dtype or o.numel() != g.numel() or o.get_device() != dev
-                                  or not o.is_contiguous()):
-                raise ValueError(f"out[{i}]: expected a contiguous {g.dtype} tensor of {g.numel()} elements on cuda:{dev}")
-            vals[4 * i + 1] = 0 if o is None else o.data_ptr()
-    if scaler is not None:
-        _whole(scaler, torch.int32, "scaler", (8,))
-    arr = (C.c_int64 * max(1, 4 * n))(*vals)
+        for i, (o, kind) in enumerate(zip(out, kinds)):
+            if o is not None and ((o.dtype, o.numel()) != kind or o.get_device() != dev or not o.is_contiguous()):
+                raise ValueError(f"out[{i}]: expected a contiguous {kind[0]} tensor of {kind[1]} elements on cuda:{dev}")
+        to = [0 if o is None else o.data_ptr() for o in out]
+    sc = None if scaler is None else _here(scaler, torch.int32, "scaler", (8,))
+    table = struct.pack(f"{4 * n}q", *[v for g, o, (dt, k) in zip(at, to, kinds) for v in (g, o, k, dt is f16)])
+    norm = torch.empty(1, dtype=f32, device="cuda")
     ws = torch.empty(RBK_CLIP_WS_BYTES, dtype=torch.uint8, device="cuda")
-    call("rbk_clip_grad_norm", ctx().handle, C.addressof(arr), n, max_norm, _p(scaler), _p(norm), _p(ws), _s())
+    call("rbk_clip_grad_norm", ctx().handle, table, n, max_norm, sc, norm.data_ptr(), ws.data_ptr(), _s())
     return norm
 
 
@@ -331,48 +326,41 @@ def attn_bwd(qkv, o, dout, lse, B, S, H, dh, scale=None, dbias=None):
 RBK_QK_BWD_WS_BYTES = 1024 * 256 * 4
 
 
-def _heads(t, name, shape=None):
-    _need_here(t, torch.float16, name, shape)
-    if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
+def _heads(t, name, shape):
+    p = _here(t, torch.float16, name, shape, whole=False)
+    st = t.stride()
+    if len(st) != 4 or (st[3] != 1 and shape[3] > 1):
         raise ValueError(f"{name}: expected [B, S, H, dh] heads with contiguous channels, got shape {tuple(t.shape)}, "
-                         f"strides {t.stride()}")
-    return Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+                         f"strides {st}")
+    return Heads(p, st[0], st[1], st[2])
 
 
 def _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out):
-    a = QkArgs()
-    a.B, a.S, a.Hq, a.dh = q.shape
-    a.q = _heads(q, "q")
-    if k is not None:
-        a.Hk = k.shape[2]
-        a.k = _heads(k, "k", (a.B, a.S, a.Hk, a.dh))
-    a.rot = a.dh if rot is None else rot
-    a.interleaved, a.eps, a.theta, a.pos0 = int(interleaved), eps, theta, pos0
+    shape = q.shape
+    hq = _heads(q, "q", shape)
+    B, S, Hq, dh = shape
+    rot = dh if rot is None else rot
+    freq = None
     if inv_freq is not None:
-        if len(inv_freq) != a.rot // 2:
-            raise ValueError(f"inv_freq: expected {a.rot // 2} values, got {len(inv_freq)}")
+        if len(inv_freq) != rot // 2:
+            raise ValueError(f"inv_freq: expected {rot // 2} values, got {len(inv_freq)}")
         freq = (C.c_double * max(1, len(inv_freq)))(*[float(x) for x in inv_freq])
-        a.inv_freq, a.kept = C.cast(freq, C.c_void_p), freq
-    if positions is not None:
-        _need_here(positions, torch.int32, "positions", (a.B, a.S))
-        if not positions.is_contiguous():
-            raise ValueError("positions: expected a contiguous tensor")
-        a.positions = positions.data_ptr()
-    for name, g in (("gq", gq), ("gk", gk)):
-        if g is not None:
-            _need_here(g, torch.float16, name, (a.dh,))
-            if not g.is_contiguous():
-                raise ValueError(f"{name}: expected a contiguous tensor")
-            setattr(a, name, g.data_ptr())
+    pos = None if positions is None else _here(positions, torch.int32, "positions", (B, S))
+    pq = None if gq is None else _here(gq, torch.float16, "gq", (dh,))
+    pk = None if gk is None else _here(gk, torch.float16, "gk", (dh,))
+    kshape = (B, S, 0, dh) if k is None else (B, S, k.shape[2], dh)
     if out is None:
         # queries and keys side by side, as the projection's rows hold them
-        both = torch.empty(a.B, a.S, a.Hq + a.Hk, a.dh, dtype=torch.float16, device=q.device)
-        out = both[:, :, :a.Hq], (both[:, :, a.Hq:] if k is not None else None)
-    oq, ok = out
-    a.oq = _heads(oq, "out[0]", q.shape)
+        both = torch.empty((B, S, Hq + kshape[2], dh), dtype=torch.float16, device=q.device)
+        out = (both, None) if k is None else both.split((Hq, kshape[2]), 2)
+    a = QkArgs(B, S, Hq, kshape[2], dh, rot, bool(interleaved), eps, theta, C.cast(freq, C.c_void_p) if freq else None,
+               pos, pos0, pq, pk, hq)
+    a.kept = freq
+    a.oq = _heads(out[0], "out[0]", shape)
     if k is not None:
-        a.ok = _heads(ok, "out[1]", k.shape)
-    return a, oq, ok
+        a.k = _heads(k, "k", kshape)
+        a.ok = _heads(out[1], "out[1]", kshape)
+    return a, out, kshape
 
 
 def qk_norm_rope_fwd(q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000.0, inv_freq=None, rot=None,
@@ -383,34 +371,32 @@ def qk_norm_rope_fwd(q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000
     [dh] gains.  positions: int32 [B, S], or None for pos0 + s.  inv_freq: rot / 2 host numbers, or None for
     theta^(-2 i / rot).  rot: leading channels that turn (default dh).  out: (yq, yk), e.g. the q and k blocks of
     the qkv rows that attn_fwd reads, or (q, k) themselves; by default one new tensor.  Returns (yq, yk)."""
-    a, yq, yk = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
+    a, out, _ = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
     call("rbk_qk_norm_rope_fwd", ctx().handle, C.byref(a), _s())
-    return yq, yk
+    return out[0], (None if k is None else out[1])
 
 
 def qk_norm_rope_bwd(dyq, dyk, q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000.0, inv_freq=None,
                      rot=None, interleaved=False, eps=1e-6, out=None, dgq=None, dgk=None):
     """Its backward (rbk_qk_norm_rope_bwd): q, k as the forward read them.  Returns (dq, dk, dgq, dgk); given
     FP32 [dh] dgq, dgk accumulate, else both are new.  out: (dq, dk), may be (dyq, dyk)."""
-    a, dq, dk = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
+    a, out, kshape = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
     a.dyq = _heads(dyq, "dyq", q.shape)
     if k is not None:
-        a.dyk = _heads(dyk, "dyk", k.shape)
-    if (dgq is None) != (dgk is None) and k is not None:
+        a.dyk = _heads(dyk, "dyk", kshape)
+    if k is not None and (dgq is None) != (dgk is None):
         raise ValueError("dgq and dgk: give both or neither")
-    a.accumulate = int(dgq is not None)
     if dgq is None:
-        both = torch.empty(2, a.dh, dtype=torch.float32, device=q.device)
-        dgq, dgk = both[0], (both[1] if k is not None else None)
-    for name, g in (("dgq", dgq), ("dgk", dgk)):
-        if g is not None:
-            _need(g, torch.float32, name)
-            _need_here(g, torch.float32, name, (a.dh,))
-            setattr(a, name, g.data_ptr())
+        dgq, dgk = torch.empty((2, a.dh), dtype=torch.float32, device=q.device).unbind(0)
+    else:
+        a.accumulate = 1
+    a.dgq = _here(dgq, torch.float32, "dgq", (a.dh,))
+    if k is not None:
+        a.dgk = _here(dgk, torch.float32, "dgk", (a.dh,))
     ws = torch.empty(RBK_QK_BWD_WS_BYTES, dtype=torch.uint8, device=q.device)
     a.ws = ws.data_ptr()
     call("rbk_qk_norm_rope_bwd", ctx().handle, C.byref(a), _s())
-    return dq, dk, dgq, dgk
+    return out[0], (None if k is None else out[1]), dgq, (None if k is None else dgk)
 
 
 # ------------------------------------------------------ gated feed-forward --
@@ -420,11 +406,12 @@ _ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU}
 
 
 def _rows(t, name, shape):
-    """A half [N, D] tensor with contiguous rows; returns its row stride."""
-    _need_here(t, torch.float16, name, shape)
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name}: expected contiguous rows, got strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    """A half [N, D] tensor with contiguous rows; returns its address and row stride."""
+    p = _here(t, torch.float16, name, shape, whole=False)
+    st = t.stride()
+    if st[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: expected contiguous rows, got strides {st}")
+    return p, (st[0] if shape[0] > 1 else shape[1])
 
 
 def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save=True, out=None):
@@ -433,30 +420,21 @@ def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save
     x [N, D], wgu [2F, D] (gate rows, then up rows), wd [D, F], biases [2F] and [D]: half.  act: "silu" or "gelu"
     (tanh form).  Returns (y, gu, h): gu [N, 2F] the two projections, for gated_ffn_bwd (None with save False),
     and h [N, F] the product.  out: y, may be residual."""
-    a = FfnArgs()
-    a.N, a.D = x.shape
-    a.F = wd.shape[1]
-    a.act = _ACTS[act]
-    a.ldx = _rows(x, "x", (a.N, a.D))
-    _whole(wgu, torch.float16, "wgu", (2 * a.F, a.D))
-    _whole(wd, torch.float16, "wd", (a.D, a.F))
-    y = torch.empty(a.N, a.D, dtype=torch.float16, device=x.device) if out is None else out
-    a.ldy = _rows(y, "out", (a.N, a.D))
-    a.x, a.wgu, a.wd, a.y = x.data_ptr(), wgu.data_ptr(), wd.data_ptr(), y.data_ptr()
-    if bgu is not None:
-        _whole(bgu, torch.float16, "bgu", (2 * a.F,))
-        a.bgu = bgu.data_ptr()
-    if bd is not None:
-        _whole(bd, torch.float16, "bd", (a.D,))
-        a.bd = bd.data_ptr()
-    if residual is not None:
-        a.ldr = _rows(residual, "residual", (a.N, a.D))
-        a.residual = residual.data_ptr()
-    h = torch.empty(a.N, a.F, dtype=torch.float16, device=x.device)
-    a.h = h.data_ptr()
-    gu = torch.empty(a.N, 2 * a.F, dtype=torch.float16, device=x.device) if save else None
-    if save:
-        a.gu = gu.data_ptr()
+    f16 = torch.float16
+    shape = x.shape
+    N, D = shape
+    F = wd.shape[1]
+    px, ldx = _rows(x, "x", shape)
+    pwgu, pwd = _here(wgu, f16, "wgu", (2 * F, D)), _here(wd, f16, "wd", (D, F))
+    pbgu = None if bgu is None else _here(bgu, f16, "bgu", (2 * F,))
+    pbd = None if bd is None else _here(bd, f16, "bd", (D,))
+    pres, ldr = (None, 0) if residual is None else _rows(residual, "residual", shape)
+    y = torch.empty(shape, dtype=f16, device=x.device) if out is None else out
+    py, ldy = _rows(y, "out", shape)
+    h = torch.empty((N, F), dtype=f16, device=x.device)
+    gu = torch.empty((N, 2 * F), dtype=f16, device=x.device) if save else None
+    a = FfnArgs(N, D, F, _ACTS[act], px, ldx, pwgu, pbgu, pwd, pbd, pres, ldr, py, ldy, gu.data_ptr() if save else None,
+                h.data_ptr())
     call("rbk_gated_ffn_fwd", ctx().handle, C.byref(a), _s())
     return y, gu, h
 
@@ -466,29 +444,22 @@ def gated_ffn_bwd(dy, x, gu, wgu, wd, act="silu", h=None, want_dx=True, dwgu=Non
     """Its backward (rbk_gated_ffn_bwd) from the saved gu.  h: the forward's, or None to have it computed again.
     dwgu [2F, D], dbgu [2F], dwd [D, F], dbd [D]: FP32, accumulate; those left out are not computed.  dgu: may be gu.
     Returns (dx or None, dgu, h)."""
-    a = FfnBwdArgs()
-    a.N, a.D = dy.shape
-    a.F = wd.shape[1]
-    a.act = _ACTS[act]
-    a.lddy, a.ldx = _rows(dy, "dy", (a.N, a.D)), _rows(x, "x", (a.N, a.D))
-    _whole(gu, torch.float16, "gu", (a.N, 2 * a.F))
-    _whole(wgu, torch.float16, "wgu", (2 * a.F, a.D))
-    _whole(wd, torch.float16, "wd", (a.D, a.F))
-    a.dy, a.x, a.gu, a.wgu, a.wd = (t.data_ptr() for t in (dy, x, gu, wgu, wd))
-    a.recompute_h = int(h is None)
-    h = torch.empty(a.N, a.F, dtype=torch.float16, device=dy.device) if h is None else h
-    _whole(h, torch.float16, "h", (a.N, a.F))
+    f16, f32 = torch.float16, torch.float32
+    shape = dy.shape
+    N, D = shape
+    F = wd.shape[1]
+    pdy, lddy = _rows(dy, "dy", shape)
+    px, ldx = _rows(x, "x", shape)
+    pgu = _here(gu, f16, "gu", (N, 2 * F))
+    pwgu, pwd = _here(wgu, f16, "wgu", (2 * F, D)), _here(wd, f16, "wd", (D, F))
+    recompute = h is None
+    h = torch.empty((N, F), dtype=f16, device=dy.device) if recompute else h
     dgu = torch.empty_like(gu) if dgu is None else dgu
-    _whole(dgu, torch.float16, "dgu", gu.shape)
-    a.h, a.dgu = h.data_ptr(), dgu.data_ptr()
-    dx = None
-    if want_dx:
-        dx = torch.empty(a.N, a.D, dtype=torch.float16, device=dy.device)
-        a.dx, a.lddx = dx.data_ptr(), a.D
-    for name, t, shape in (("dwgu", dwgu, (2 * a.F, a.D)), ("dbgu", dbgu, (2 * a.F,)), ("dwd", dwd, (a.D, a.F)),
-                           ("dbd", dbd, (a.D,))):
-        if t is not None:
-            _whole(t, torch.float32, name, shape)
-            setattr(a, name, t.data_ptr())
+    dx = torch.empty(shape, dtype=f16, device=dy.device) if want_dx else None
+    grads = [None if t is None else _here(t, f32, name, s)
+             for name, t, s in (("dwgu", dwgu, (2 * F, D)), ("dbgu", dbgu, (2 * F,)), ("dwd", dwd, (D, F)),
+                                ("dbd", dbd, (D,)))]
+    a = FfnBwdArgs(N, D, F, _ACTS[act], pdy, lddy, px, ldx, pgu, pwgu, pwd, _here(h, f16, "h", (N, F)), recompute,
+                   _here(dgu, f16, "dgu", (N, 2 * F)), dx.data_ptr() if want_dx else None, D, *grads)
     call("rbk_gated_ffn_bwd", ctx().handle, C.byref(a), _s())
     return dx, dgu, h

@@ -155,7 +155,7 @@ def clip(tensors, max_norm=1.0, norm=P, ws=P, count=None):
     from rbk import lib
     from rbk._lib import Grad
     arr = (Grad * max(1, len(tensors)))(*[Grad(*t) for t in tensors])
-    st = lib().rbk_clip_grad_norm(None, C.cast(arr, C.c_void_p), len(tensors) if count is None else count, max_norm,
+    st = lib().rbk_clip_grad_norm(None, C.cast(arr, C.c_char_p), len(tensors) if count is None else count, max_norm,
                                   None, norm, ws, None)
     return st, lib().rbk_last_error().decode()
 
