@@ -11,10 +11,13 @@
 // Memory bound: 4 bytes per element forward, 6 backward, each touched once.
 // Layout: a head is split over G lanes (the power of two >= dh / 16), a lane holding two
 // 16-byte chunks of it, chosen so that both members of every rotated pair are in the
-// same lane: no exchange is needed for the rotation.  A warp works on 32 / G heads of one
-// token at a time, so a token's angles are computed once for all of its heads, each by one
-// of the lanes that need it (they get it by shuffle).  The loads of a warp's next heads are in
-// flight while it works on its present ones, across tokens too.
+// same lane: no exchange is needed for the rotation.  A warp, or each half of one (T = 2,
+// where fewer lanes then idle: 12 heads of 64 are 3 full steps of 4 for two tokens and not one
+// full and one half step of 8), works on the heads of one token, so a token's angles are
+// computed once for all of its heads, each by one of the lanes that need it (they get it by
+// shuffle).  Each lane copies its vectors of the
+// warp's next steps, across tokens too, into slots of its own in shared memory with cp.async
+// and waits for its own copies only: no barrier, and no registers for what is in flight.
 #include <algorithm>
 #include <cmath>
 
@@ -50,7 +53,7 @@ struct Params {
 };
 
 // cos and sin of position p's angle for a frequency of `freq` 2^-64 turns per position.  The product wraps
-// modulo 2^64 = modulo a turn, exactly; its top 32 bits, rounded, are the angle to 2^-33 turns.
+// modulo 2^64 = modulo a turn, exactly; its top 32 bits, rounded, are the angle to 2^-32 turns.
 __device__ __forceinline__ void turn(int p, unsigned long long freq, float& c, float& s) {
     const unsigned long long t = (unsigned long long)(long long)p * freq + 0x80000000ull;
     sincospif((float)(int)(t >> 32) * 4.656612873077393e-10f, &s, &c);      // 2^-31: half turns
@@ -120,6 +123,15 @@ __device__ __forceinline__ void rotate(const Lane& l, Row& r, const uint64_t* cs
 }
 
 __device__ __forceinline__ uint4 load8(const uint4* p, bool on) { return on ? *p : make_uint4(0, 0, 0, 0); }
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint4* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t src) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+    return v;
+}
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
@@ -130,19 +142,29 @@ __device__ __forceinline__ float group_sum(float v) {
 // Blocks of an SM: 24 warps at 80 registers forward, 16 at 128 backward.
 template <bool BWD>
 constexpr int kPerSm = BWD ? 2 : 3;
+// Steps in flight, and what a warp's step takes of shared memory: 128 KB and 96 KB per SM.
+template <bool BWD>
+constexpr int kDepth = BWD ? 3 : 4;
+template <bool BWD>
+constexpr int kStep = 32 * 16 * (BWD ? 4 : 2);
+template <bool BWD>
+constexpr int kSmem = kWarps * kDepth<BWD> * kStep<BWD>;
+static_assert(kWarps * kMaxDh * 4 <= kSmem<true>, "the gain gradients' warp sums reuse it");
 
-template <int G, bool INTER, bool BWD>
+template <int G, int T, bool INTER, bool BWD>
 __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_constant__ Params p) {
-    constexpr int HPW = 32 / G;                                     // heads of a token per warp and step
-    constexpr int ANG = HPW >= 8 ? 1 : 8 / HPW;                     // angles that a lane computes of its slot's 8
-    __shared__ float acc_s[BWD ? kWarps : 1][BWD ? kMaxDh : 1];
+    constexpr int HPS = 32 / T / G;                                 // heads of a token per step
+    constexpr int ANG = HPS >= 8 ? 1 : 8 / HPS;                     // angles that a lane computes of its slot's 8
+    constexpr int DEPTH = kDepth<BWD>, STEP = kStep<BWD>;
+    extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int which = (int)blockIdx.x >= p.blocks0;
     const Side& sd = p.side[which];
     const int w = (which ? blockIdx.x - p.blocks0 : blockIdx.x) * kWarps + warp;
-    const int stride = max(1, (int)(which ? gridDim.x - p.blocks0 : p.blocks0) * kWarps / sd.parts);   // tokens of a round
-    const int g = lane / G, j = lane % G;
+    const int stride = T * max(1, (int)(which ? gridDim.x - p.blocks0 : p.blocks0) * kWarps / sd.parts);   // tokens of a round
+    const int g = lane % (32 / T) / G, j = lane % G, sub = lane / (32 / T);
     const Lane l = lane_of(p, j);
+    const uint32_t slot = tc::su32(smem) + warp * (DEPTH * STEP) + lane * 16;
     unsigned long long freq[ANG];
 #pragma unroll
     for (int i = 0; i < ANG; ++i) freq[i] = p.freq[8 * j + (g * ANG + i) % 8];
@@ -157,71 +179,82 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_
     }
     Row acc = {};                                                   // gain gradient
 
-    // The heads in flight: token (bi, si), this lane's head and pointers to its chunk a.
     const int part = w % sd.parts, h0 = part * sd.heads_per_part + g;
-    const int h1 = min(sd.H, (part + 1) * sd.heads_per_part) + g;   // of the group's heads: h - g < h1 - g
+    const int h1 = min(sd.H, (part + 1) * sd.heads_per_part) + g;   // a lane's heads: h0, h0 + HPS .. below h1
     const int ab = l.b - l.a;
-    int token = w / sd.parts < stride ? w / sd.parts : p.tokens, h = 0, pos = 0;
-    const uint4 *xp = nullptr, *ep = nullptr;
-    uint4* op = nullptr;
-    uint4 xa, xb, ea, eb;
-    auto at = [&](const Heads& t, int bi, int si) {
+    // the warp's token, or its first one: lanes with sub = 1 work on the next, if there is one
+    int token = T * (w / sd.parts) < stride ? T * (w / sd.parts) : p.tokens, h = h0;
+    auto next = [&](int tk) { return p.tokens - tk > stride ? tk + stride : p.tokens; };
+    auto at = [&](const Heads& t, int tk) {                         // this lane's chunk a of head h0
+        tk = min(tk + sub, p.tokens - 1);
+        const int bi = (int)((unsigned)tk / (unsigned)p.S), si = tk - bi * p.S;
         return t.p + ((long long)bi * t.sb + (long long)si * t.ss + (long long)h0 * t.sh + l.a);
     };
-    auto start = [&] {
-        const int bi = (int)((unsigned)token / (unsigned)p.S), si = token - bi * p.S;
-        pos = p.pos ? p.pos[token] : p.pos0 + si;
-        xp = at(sd.x, bi, si);
-        op = at(sd.o, bi, si);
-        if (BWD) ep = at(sd.dy, bi, si);
-        h = h0;
+    auto pos_of = [&](int tk) {
+        tk = min(tk + sub, p.tokens - 1);
+        return p.pos ? p.pos[tk] : p.pos0 + (int)((unsigned)tk % (unsigned)p.S);
     };
+    // whether this lane has head hd of token tk (+ sub)
+    auto has = [&](int tk, int hd) { return hd < sd.H && (T == 1 || tk + sub < p.tokens); };
+
+    // The copies run DEPTH - 1 steps ahead of the work: token ft, head fh.
+    int ft = token, fh = h0, fs = 0;
+    const uint4 *xp = nullptr, *ep = nullptr;
     auto fetch = [&] {
-        const bool on = h < sd.H;
-        xa = load8(xp, on && l.has_a);
-        xb = load8(xp + ab, on && l.has_b);
-        if (BWD) {
-            ea = load8(ep, on && l.has_a);
-            eb = load8(ep + ab, on && l.has_b);
+        if (ft < p.tokens) {
+            if (fh == h0) {
+                xp = at(sd.x, ft);
+                if (BWD) ep = at(sd.dy, ft);
+            }
+            const uint32_t d = slot + fs * STEP;
+            const bool on = has(ft, fh);
+            copy16(d, xp, on && l.has_a);
+            copy16(d + 512, xp + ab, on && l.has_b);
+            xp += HPS * (long long)sd.x.sh;
+            if (BWD) {
+                copy16(d + 1024, ep, on && l.has_a);
+                copy16(d + 1536, ep + ab, on && l.has_b);
+                ep += HPS * (long long)sd.dy.sh;
+            }
+            fh += HPS;
+            if (fh >= h1) {                                         // the same in all lanes
+                ft = next(ft);
+                fh = h0;
+            }
         }
+        fs = fs + 1 == DEPTH ? 0 : fs + 1;
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (token < p.tokens) {
-        start();
-        fetch();
-    }
-    bool fresh = true;
+#pragma unroll
+    for (int i = 0; i < DEPTH - 1; ++i) fetch();
+    uint4* op = nullptr;
+    int cur = 0, pos = token < p.tokens ? pos_of(token) : 0;
     uint64_t cs[4], sn[4];
     while (token < p.tokens) {
-        Row x, e;
-        tc::h8_to_p(xa, x.v);
-        tc::h8_to_p(xb, x.v + 4);
-        if (BWD) {
-            tc::h8_to_p(ea, e.v);
-            tc::h8_to_p(eb, e.v + 4);
-        }
-        const bool on = h < sd.H;
-        uint4* const o = op;
-        if (fresh) {                                                // a new token: its angles
+        if (h == h0) {                                              // a new token: its angles
+            op = at(sd.o, token);
             float c[ANG], s[ANG];
 #pragma unroll
             for (int i = 0; i < ANG; ++i) turn(pos, freq[i], c[i], s[i]);
+            pos = pos_of(next(token));
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                const int s0 = i / ANG * G + j, s1 = (i + 1) / ANG * G + j;
+                const int s0 = sub * (32 / T) + i / ANG * G + j, s1 = sub * (32 / T) + (i + 1) / ANG * G + j;
                 cs[i / 2] = pk2(__shfl_sync(0xffffffffu, c[i % ANG], s0), __shfl_sync(0xffffffffu, c[(i + 1) % ANG], s1));
                 sn[i / 2] = pk2(__shfl_sync(0xffffffffu, s[i % ANG], s0), __shfl_sync(0xffffffffu, s[(i + 1) % ANG], s1));
             }
         }
-        h += HPW;
-        xp += HPW * (long long)sd.x.sh;
-        op += HPW * (long long)sd.o.sh;
-        if (BWD) ep += HPW * (long long)sd.dy.sh;
-        fresh = h >= h1;                                            // the same in all lanes
-        if (fresh) {
-            token = p.tokens - token > stride ? token + stride : p.tokens;
-            if (token < p.tokens) start();
+        asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
+        const uint32_t d = slot + cur * STEP;
+        cur = cur + 1 == DEPTH ? 0 : cur + 1;
+        Row x, e;
+        tc::h8_to_p(lds16(d), x.v);
+        tc::h8_to_p(lds16(d + 512), x.v + 4);
+        if (BWD) {
+            tc::h8_to_p(lds16(d + 1024), e.v);
+            tc::h8_to_p(lds16(d + 1536), e.v + 4);
         }
-        if (token < p.tokens) fetch();
+        fetch();                                                    // into the slot of the step before
 
         uint64_t ss = 0;                                            // two zeros
 #pragma unroll
@@ -247,11 +280,21 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_
                 x.v[i] = pmul2(pfma2(xh, t2, pmul2(e.v[i], gain.v[i])), r2);
             }
         }
-        if (on && l.has_a) o[0] = tc::p_to_h8(x.v);
-        if (on && l.has_b) o[ab] = tc::p_to_h8(x.v + 4);
+        const bool on = has(token, h);
+        if (on && l.has_a) op[0] = tc::p_to_h8(x.v);
+        if (on && l.has_b) op[ab] = tc::p_to_h8(x.v + 4);
+        op += HPS * (long long)sd.o.sh;
+        h += HPS;
+        if (h >= h1) {                                              // the same in all lanes
+            token = next(token);
+            h = h0;
+        }
     }
     if constexpr (BWD) {
         // lanes of the same slot, then the warps, in a fixed order
+        float(*acc_s)[kMaxDh] = reinterpret_cast<float(*)[kMaxDh]>(smem);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();                                            // the slots are free
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float a = lo2(acc.v[i]), b = hi2(acc.v[i]);
@@ -261,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_
                 b += __shfl_xor_sync(0xffffffffu, b, o);
             }
             const int c = i < 4 ? 8 * l.a + 2 * i : 8 * l.b + 2 * (i - 4);
-            if (g == 0 && (i < 4 ? l.has_a : l.has_b)) {
+            if (lane < G && (i < 4 ? l.has_a : l.has_b)) {
                 acc_s[warp][c] = a;
                 acc_s[warp][c + 1] = b;
             }
@@ -301,15 +344,16 @@ __global__ void __launch_bounds__(kThreads) qk_gain_kernel(float* dgq, float* dg
     }
 }
 
-template <bool INTER, bool BWD>
-int run(const Params& p, int grid, cudaStream_t st) {
-    const int slots = (p.dh + 15) / 16;
+template <int T, bool INTER, bool BWD>
+int launch(const Params& p, int lanes, int grid, cudaStream_t st) {
     const dim3 gd(grid), bd(kThreads);
-    if (slots <= 1) RBK_CUDA(launch_pdl(qk_kernel<1, INTER, BWD>, gd, bd, 0, st, p));
-    else if (slots <= 2) RBK_CUDA(launch_pdl(qk_kernel<2, INTER, BWD>, gd, bd, 0, st, p));
-    else if (slots <= 4) RBK_CUDA(launch_pdl(qk_kernel<4, INTER, BWD>, gd, bd, 0, st, p));
-    else if (slots <= 8) RBK_CUDA(launch_pdl(qk_kernel<8, INTER, BWD>, gd, bd, 0, st, p));
-    else RBK_CUDA(launch_pdl(qk_kernel<16, INTER, BWD>, gd, bd, 0, st, p));
+    switch (lanes) {
+        case 1: RBK_CUDA(launch_pdl(qk_kernel<1, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
+        case 2: RBK_CUDA(launch_pdl(qk_kernel<2, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
+        case 4: RBK_CUDA(launch_pdl(qk_kernel<4, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
+        case 8: RBK_CUDA(launch_pdl(qk_kernel<8, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
+        default: RBK_CUDA(launch_pdl(qk_kernel<16, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
+    }
     RBK_LAUNCHED("qk_kernel");
     return RBK_OK;
 }
@@ -379,18 +423,23 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
         p.freq[i] = 0;
         if (i >= a->rot / 2) continue;
         long double t = (a->inv_freq ? (long double)a->inv_freq[i] : f) / tau;
-        t -= floorl(t);                                              // positions are whole: turns drop out
-        t = roundl(t * 18446744073709551616.0L);
+        if (t < 0.0L || t >= 1.0L) t -= floorl(t);                   // positions are whole: turns drop out
+        t *= 18446744073709551616.0L;
         p.freq[i] = t >= 18446744073709551616.0L ? 0 : (unsigned long long)t;
         f *= ratio;
     }
+    // A head's lanes, and the heads of a step.  Two tokens at a time where that leaves fewer lane steps.
+    const int slots = (a->dh + 15) / 16;
+    const int lanes = slots <= 1 ? 1 : slots <= 2 ? 2 : slots <= 4 ? 4 : slots <= 8 ? 8 : 16;
+    const auto steps_of = [](int heads, int per) { return (heads + per - 1) / per; };
+    const int one = 32 / lanes, two = one / 2;
+    const int T = steps_of(H[0], two) + steps_of(H[1], two) < 2 * (steps_of(H[0], one) + steps_of(H[1], one)) ? 2 : 1;
+    const int hps = T == 2 ? two : one;
     // A warp takes all heads of a token where there are tokens for every warp, so that a token's angles are
     // computed once; with fewer tokens its heads are shared out over up to kMaxParts warps.
-    const int slots = (a->dh + 15) / 16;
-    const int hpw = slots <= 1 ? 32 : slots <= 2 ? 16 : slots <= 4 ? 8 : slots <= 8 ? 4 : 2;
     const int most = kPerSm<BWD> * ctx->num_sms;
     const int max_blocks = std::min(most, kMaxRows - 2 * kMaxParts / kWarps);
-    const bool all = (long long)tokens * 2 >= (long long)max_blocks * kWarps;
+    const bool all = (long long)tokens * 2 >= (long long)max_blocks * kWarps * T;
     long long need[2];
     for (int i = 0; i < 2; ++i) {
         Side& s = p.side[i];
@@ -399,10 +448,10 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
         s.o = heads(*o[i]);
         s.dy = heads(*dy[i]);
         s.gain = (const half*)(i ? a->gk : a->gq);
-        const int steps = (H[i] + hpw - 1) / hpw;
-        s.heads_per_part = hpw * (all ? steps : (steps + kMaxParts - 1) / kMaxParts);
-        s.parts = steps ? (H[i] + s.heads_per_part - 1) / s.heads_per_part : 1;
-        need[i] = steps ? ((long long)tokens * s.parts + kWarps - 1) / kWarps : 0;
+        const int steps = steps_of(H[i], hps);
+        s.heads_per_part = hps * (all ? steps : steps_of(steps, kMaxParts));
+        s.parts = steps ? steps_of(H[i], s.heads_per_part) : 1;
+        need[i] = steps ? (((long long)tokens + T - 1) / T * s.parts + kWarps - 1) / kWarps : 0;
     }
     cudaStream_t st = as_stream(stream);
     long long nb[2] = {need[0], need[1]};
@@ -423,7 +472,10 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
     const double n = (double)tokens * (a->Hq + a->Hk) * a->dh;
     ProfScope prof(ctx, st, kCatOther, (BWD ? 6.0 : 4.0) * n);
     if (grid) {
-        const int status = a->interleaved ? run<true, BWD>(p, grid, st) : run<false, BWD>(p, grid, st);
+        const int status = a->interleaved ? (T == 2 ? launch<2, true, BWD>(p, lanes, grid, st)
+                                                    : launch<1, true, BWD>(p, lanes, grid, st))
+                                          : (T == 2 ? launch<2, false, BWD>(p, lanes, grid, st)
+                                                    : launch<1, false, BWD>(p, lanes, grid, st));
         if (status != RBK_OK) return status;
     }
     if (BWD && (a->dgq || a->dgk)) {

@@ -8,6 +8,7 @@ device of the active context; there is no host or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import struct
 import threading
 
@@ -77,14 +78,12 @@ def _need(t, dtype, name):
 
 def _here(t, dtype, name, shape, whole=True):
     """A tensor of this type and shape (contiguous unless whole is False) on the current device; returns its address."""
-    if t.dtype is not dtype or t.get_device() != torch._C._cuda_getDevice():
-        raise ValueError(f"{name}: expected a {dtype} tensor on cuda:{torch.cuda.current_device()}, got {t.dtype} on "
-                         f"{t.device}")
-    if t.shape != shape:
-        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if whole and not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor, got strides {t.stride()}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.shape == shape and t.get_device() == torch._C._cuda_getDevice() and (
+            not whole or t.is_contiguous()):
+        return t.data_ptr()
+    raise ValueError(f"{name}: expected a{' contiguous' if whole else ''} {dtype} tensor of shape {tuple(shape)} on "
+                     f"cuda:{torch.cuda.current_device()}, got {t.dtype}, shape {tuple(t.shape)}, strides {t.stride()} on "
+                     f"{t.device}")
 
 
 # ----------------------------------------------------------------- LayerNorm --
@@ -194,6 +193,7 @@ def adam_tail(p32, g, m, v, p16, scaler_buf, lr, b1=0.9, b2=0.999, eps=1e-8, wd=
 
 
 RBK_CLIP_WS_BYTES = 16 << 10
+_dtype = operator.attrgetter("dtype")
 
 
 def clip_grad_norm(grads, max_norm, scaler=None, out=None):
@@ -205,21 +205,21 @@ def clip_grad_norm(grads, max_norm, scaler=None, out=None):
     the norm is computed (and `out` is a copy)."""
     dev, n = torch._C._cuda_getDevice(), len(grads)
     f32, f16 = torch.float32, torch.float16
-    kinds = [(g.dtype, g.numel()) for g in grads]
-    for i, g in enumerate(grads):
-        if (g.dtype is not f32 and g.dtype is not f16) or g.get_device() != dev or not g.is_contiguous():
-            raise ValueError(f"grads[{i}]: expected a contiguous FP32 or half tensor on cuda:{dev}, got {g.dtype} on "
-                             f"{g.device}")
-    at = to = [g.data_ptr() for g in grads]
+    T = torch.Tensor
+    kinds = list(map(_dtype, grads))
+    sizes = list(map(T.numel, grads))
+    if (set(kinds) - {f32, f16} or set(map(T.get_device, grads)) - {dev} or not all(map(T.is_contiguous, grads))):
+        raise ValueError(f"grads: expected contiguous FP32 or half tensors on cuda:{dev}, got "
+                         f"{sorted({(str(g.dtype), str(g.device), g.is_contiguous()) for g in grads})}")
+    at = to = list(map(T.data_ptr, grads))
     if out is not None:
-        if len(out) != n:
-            raise ValueError(f"out: expected {n} tensors, got {len(out)}")
-        for i, (o, kind) in enumerate(zip(out, kinds)):
-            if o is not None and ((o.dtype, o.numel()) != kind or o.get_device() != dev or not o.is_contiguous()):
-                raise ValueError(f"out[{i}]: expected a contiguous {kind[0]} tensor of {kind[1]} elements on cuda:{dev}")
+        some = [o for o in out if o is not None]
+        if len(out) != n or set(map(T.get_device, some)) - {dev} or not all(map(T.is_contiguous, some)) or any(
+                o is not None and (o.dtype is not k or o.numel() != s) for o, k, s in zip(out, kinds, sizes)):
+            raise ValueError(f"out: expected {n} contiguous tensors (or None) of the gradients' types and sizes on cuda:{dev}")
         to = [0 if o is None else o.data_ptr() for o in out]
     sc = None if scaler is None else _here(scaler, torch.int32, "scaler", (8,))
-    table = struct.pack(f"{4 * n}q", *[v for g, o, (dt, k) in zip(at, to, kinds) for v in (g, o, k, dt is f16)])
+    table = struct.pack(f"{4 * n}q", *[v for row in zip(at, to, sizes, [k is f16 for k in kinds]) for v in row])
     norm = torch.empty(1, dtype=f32, device="cuda")
     ws = torch.empty(RBK_CLIP_WS_BYTES, dtype=torch.uint8, device="cuda")
     call("rbk_clip_grad_norm", ctx().handle, table, n, max_norm, sc, norm.data_ptr(), ws.data_ptr(), _s())
@@ -349,18 +349,25 @@ def _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, e
     pq = None if gq is None else _here(gq, torch.float16, "gq", (dh,))
     pk = None if gk is None else _here(gk, torch.float16, "gk", (dh,))
     kshape = (B, S, 0, dh) if k is None else (B, S, k.shape[2], dh)
-    if out is None:
-        # queries and keys side by side, as the projection's rows hold them
-        both = torch.empty((B, S, Hq + kshape[2], dh), dtype=torch.float16, device=q.device)
-        out = (both, None) if k is None else both.split((Hq, kshape[2]), 2)
     a = QkArgs(B, S, Hq, kshape[2], dh, rot, bool(interleaved), eps, theta, C.cast(freq, C.c_void_p) if freq else None,
                pos, pos0, pq, pk, hq)
     a.kept = freq
-    a.oq = _heads(out[0], "out[0]", shape)
     if k is not None:
         a.k = _heads(k, "k", kshape)
-        a.ok = _heads(out[1], "out[1]", kshape)
-    return a, out, kshape
+    if out is not None:
+        a.oq = _heads(out[0], "out[0]", shape)
+        if k is not None:
+            a.ok = _heads(out[1], "out[1]", kshape)
+        return a, out[0], (None if k is None else out[1]), kshape
+    # queries and keys side by side, as the projection's rows hold them
+    row = (Hq + kshape[2]) * dh
+    both = torch.empty((B, S, Hq + kshape[2], dh), dtype=torch.float16, device=q.device)
+    at = both.data_ptr()
+    a.oq = Heads(at, S * row, row, dh)
+    if k is None:
+        return a, both, None, kshape
+    a.ok = Heads(at + 2 * Hq * dh, S * row, row, dh)
+    return a, both.narrow(2, 0, Hq), both.narrow(2, Hq, kshape[2]), kshape
 
 
 def qk_norm_rope_fwd(q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000.0, inv_freq=None, rot=None,
@@ -371,23 +378,24 @@ def qk_norm_rope_fwd(q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000
     [dh] gains.  positions: int32 [B, S], or None for pos0 + s.  inv_freq: rot / 2 host numbers, or None for
     theta^(-2 i / rot).  rot: leading channels that turn (default dh).  out: (yq, yk), e.g. the q and k blocks of
     the qkv rows that attn_fwd reads, or (q, k) themselves; by default one new tensor.  Returns (yq, yk)."""
-    a, out, _ = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
+    a, yq, yk, _ = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
     call("rbk_qk_norm_rope_fwd", ctx().handle, C.byref(a), _s())
-    return out[0], (None if k is None else out[1])
+    return yq, yk
 
 
 def qk_norm_rope_bwd(dyq, dyk, q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000.0, inv_freq=None,
                      rot=None, interleaved=False, eps=1e-6, out=None, dgq=None, dgk=None):
     """Its backward (rbk_qk_norm_rope_bwd): q, k as the forward read them.  Returns (dq, dk, dgq, dgk); given
     FP32 [dh] dgq, dgk accumulate, else both are new.  out: (dq, dk), may be (dyq, dyk)."""
-    a, out, kshape = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
+    a, dq, dk, kshape = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
     a.dyq = _heads(dyq, "dyq", q.shape)
     if k is not None:
         a.dyk = _heads(dyk, "dyk", kshape)
     if k is not None and (dgq is None) != (dgk is None):
         raise ValueError("dgq and dgk: give both or neither")
     if dgq is None:
-        dgq, dgk = torch.empty((2, a.dh), dtype=torch.float32, device=q.device).unbind(0)
+        dgq = torch.empty(a.dh, dtype=torch.float32, device=q.device)
+        dgk = None if k is None else torch.empty_like(dgq)
     else:
         a.accumulate = 1
     a.dgq = _here(dgq, torch.float32, "dgq", (a.dh,))
@@ -396,7 +404,7 @@ def qk_norm_rope_bwd(dyq, dyk, q, k, gq=None, gk=None, positions=None, pos0=0, t
     ws = torch.empty(RBK_QK_BWD_WS_BYTES, dtype=torch.uint8, device=q.device)
     a.ws = ws.data_ptr()
     call("rbk_qk_norm_rope_bwd", ctx().handle, C.byref(a), _s())
-    return out[0], (None if k is None else out[1]), dgq, (None if k is None else dgk)
+    return dq, dk, dgq, (None if k is None else dgk)
 
 
 # ------------------------------------------------------ gated feed-forward --
