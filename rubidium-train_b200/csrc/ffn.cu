@@ -6,22 +6,38 @@
 // Many rows: tensor bound (6 N D F FLOP each way).  The CTA-pair GEMM of gemm.cu with epilogues of its own
 // makes h (gate and up tiles share one accumulator) and dgu; the other products are plain GEMMs.
 // Few rows: the weights, 6 D F bytes, are read once and that is the cost.  The kernels below stream them.
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace rbk {
 namespace ffn {
 
 // ---------------------------------------------------------------- few rows ----
-// out[n, r] = sum_k w[r, k] x[n, k] for up to 8 NT rows n: a CTA takes 16 rows r of the weights (GLU: 16 of
-// the gate and the same 16 of the up projection), its 8 warps take every eighth 64-wide block of k, and the
-// warps' sums are added in warp order through shared memory.  mma.sync m16n8k16 with the weights as the
-// 16-row operand: the tensor pipe is idle next to the memory, what matters is that a lane's fragment is a
-// whole 16-byte load.  The k order within a block is permuted for that, alike on both sides: lane 4 g + t
-// holds k = 8 t .. 8 t + 7 (and 32 + 8 t ..) of row g, and MMA m of the two that use it takes its elements
-// 4 m .. 4 m + 3.
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kRows = 16;                                // weight rows of a CTA
+// out[n, r] = sum_k w[r, k] x[n, k] for up to 8 NT rows n.  A tile is 16 MT weight rows (GLU: of each 16, eight
+// of the gate and the same eight of the up projection, so that a lane ends up with both of its elements); a CTA
+// goes through its tiles, its warps share k out in rounds of 64, and their sums are added in warp order through
+// shared memory.  mma.sync m16n8k16 with the weights as the 16-row operand: the tensor pipe is idle next to the
+// memory, what matters is that a lane's fragment is a whole 16-byte vector.  The k order within a half round is
+// permuted for that, alike on both sides: lane 4 g + t holds k = 8 t .. 8 t + 7 of row g, and MMA m of the two
+// that use them takes elements 4 m .. 4 m + 3.
+// A lane copies its vectors of the next DEPTH - 1 rounds, across tiles, into slots of its own with cp.async and
+// waits for its own copies only: the weights stream without registers or barriers.
 constexpr int kMaxTokens = 32;
+
+// WIDE: at most one tile per SM, so a CTA has all of its shared memory for what is in flight; else two or three
+// CTAs share an SM.
+template <int NT, bool WIDE>
+struct Few {
+    static constexpr int MT = NT == 4 && !WIDE ? 2 : 1;
+    static constexpr int WARPS = WIDE ? 8 : 4, THREADS = 32 * WARPS;
+    static constexpr int DEPTH = WIDE ? (NT == 1 ? 8 : NT == 2 ? 6 : 4) : (NT == 1 ? 6 : NT == 2 ? 4 : 3);
+    static constexpr int VECS = 4 * MT + 2 * NT;         // 16-byte vectors of a lane and round
+    static constexpr int ROUND = VECS * 512;
+    static constexpr int RING = WARPS * DEPTH * ROUND;
+    static constexpr int SUMS = WARPS * MT * 16 * (8 * NT + 1) * 4;
+    static constexpr int SMEM = RING + SUMS;
+    static constexpr int PER_SM = WIDE ? 1 : NT == 4 ? 2 : 3;
+    static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory of an SM");
+};
 
 __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -30,12 +46,13 @@ __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, ui
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 ldg_stream(const half* p, bool on) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (on)
-        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                     : "l"(p));
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const half* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t src) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
     return v;
 }
 
@@ -51,88 +68,178 @@ struct Params {
     long long ldo;
     half* gu;                      // gated: [N, 2R] or NULL
     int act;
+    int early;                     // the weights may be read before the kernel before this one has ended
 };
 
-template <int NT, bool GLU>
-__global__ void __launch_bounds__(kThreads) few_rows_kernel(const Params p) {
-    constexpr int MATS = GLU ? 2 : 1;
-    __shared__ float sums[kWarps][MATS][kRows][8 * NT + 1];
+template <int NT, bool WIDE, bool GLU>
+__global__ void __launch_bounds__(Few<NT, WIDE>::THREADS) few_rows_kernel(const Params p) {
+    using C = Few<NT, WIDE>;
+    constexpr int MT = C::MT, DEPTH = C::DEPTH;
+    constexpr int OUT = GLU ? 8 * MT : 16 * MT;          // output columns of a tile
+    extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int r0 = blockIdx.x * kRows;
-    grid_dependency_sync();
-    // rows past the end read the last row; what they give is not stored
-    const half* w0 = p.w + (size_t)min(r0 + g, p.R - 1) * p.K;
-    const half* w1 = p.w + (size_t)min(r0 + g + 8, p.R - 1) * p.K;
-    const size_t up = (size_t)p.R * p.K;
-    float acc[MATS][NT][4] = {};
-    for (int kb = warp * 64; kb < p.K; kb += kWarps * 64) {
+    const uint32_t ring = tc::su32(smem) + warp * (DEPTH * C::ROUND) + lane * 16;
+    auto sums = reinterpret_cast<float(*)[MT][16][8 * NT + 1]>(smem + C::RING);
+    const int tiles = (p.R + OUT - 1) / OUT;
+    const int k0 = 64 * warp + 8 * t;                    // this lane's first k
+
+    // the copies: tile ft, k fk, rows' pointers, x's pointer
+    int ft = blockIdx.x, fk = k0;
+    const half *wp[MT][2], *xp = nullptr;
+    uint32_t fd = ring;
+    auto rows = [&] {                                    // of tile ft; past the end, the last row: not stored
+        if (ft >= tiles) return;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            const int k = kb + 32 * hf + 8 * t;
-            const bool on = k < p.K;
-            uint4 a[MATS][2], b[NT];
+        for (int m = 0; m < MT; ++m) {
+            const int r = ft * OUT + (GLU ? 8 : 16) * m + g;
+            wp[m][0] = p.w + (size_t)min(r, p.R - 1) * p.K + k0;
+            wp[m][1] = p.w + (GLU ? (size_t)p.R + min(r, p.R - 1) : (size_t)min(r + 8, p.R - 1)) * p.K + k0;
+        }
+    };
+    auto fetch_w = [&](uint32_t d) {
+        if (ft >= tiles) return;
+        const bool on0 = fk < p.K, on1 = fk + 32 < p.K;
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) {
-                a[m][0] = ldg_stream(w0 + m * up + k, on);
-                a[m][1] = ldg_stream(w1 + m * up + k, on);
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                copy16(d + (4 * m + 2 * h) * 512, wp[m][h], on0);
+                copy16(d + (4 * m + 2 * h + 1) * 512, wp[m][h] + 32, on1);
+                wp[m][h] += 64 * C::WARPS;
             }
+    };
+    auto fetch_x = [&](uint32_t d) {
+        if (ft < tiles) {
+            const bool on0 = fk < p.K, on1 = fk + 32 < p.K;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int n = 8 * j + g;
-                b[j] = on && n < p.N ? *reinterpret_cast<const uint4*>(p.x + n * p.ldx + k) : make_uint4(0, 0, 0, 0);
+                const bool row = 8 * j + g < p.N;
+                copy16(d + (4 * MT + 2 * j) * 512, xp + 8 * j * p.ldx, row && on0);
+                copy16(d + (4 * MT + 2 * j + 1) * 512, xp + 8 * j * p.ldx + 32, row && on1);
             }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto advance = [&] {                                 // to the round after; every warp has the same number
+        fk += 64 * C::WARPS;
+        xp += 64 * C::WARPS;
+        fd = fd + C::ROUND == ring + DEPTH * C::ROUND ? ring : fd + C::ROUND;
+        if (fk - k0 >= p.K) {
+            ft += gridDim.x;
+            fk = k0;
+            xp = p.x + (size_t)g * p.ldx + k0;
+            rows();
+        }
+    };
+    xp = p.x + (size_t)g * p.ldx + k0;
+    rows();
+    if (p.early) {
+        // the weights of the first rounds, then x behind them in the same slots
+        const half* x1 = xp;
 #pragma unroll
-            for (int m = 0; m < MATS; ++m)
+        for (int i = 0; i < DEPTH - 1; ++i) { fetch_w(fd); advance(); }
+        grid_dependency_sync();
+        ft = blockIdx.x; fk = k0; xp = x1; fd = ring;
+        rows();
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    mma_16816(acc[m][j], a[m][0].x, a[m][1].x, a[m][0].y, a[m][1].y, b[j].x, b[j].y);
-                    mma_16816(acc[m][j], a[m][0].z, a[m][1].z, a[m][0].w, a[m][1].w, b[j].z, b[j].w);
+        for (int i = 0; i < DEPTH - 1; ++i) {
+            fetch_x(fd);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) { wp[m][0] += 64 * C::WARPS; wp[m][1] += 64 * C::WARPS; }
+            advance();
+        }
+    } else {
+        grid_dependency_sync();
+#pragma unroll
+        for (int i = 0; i < DEPTH - 1; ++i) { fetch_w(fd); fetch_x(fd); advance(); }
+    }
+
+    uint32_t d = ring;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        float acc[MT][NT][4] = {};
+        for (int k = 0; k < p.K; k += 64 * C::WARPS) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
+            uint4 a[MT][4], b[NT][2];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[m][i] = lds16(d + (4 * m + i) * 512);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) b[j][i] = lds16(d + (4 * MT + 2 * j + i) * 512);
+            d = d + C::ROUND == ring + DEPTH * C::ROUND ? ring : d + C::ROUND;
+            fetch_w(fd);                                 // into the slot of the round before
+            fetch_x(fd);
+            advance();
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        mma_16816(acc[m][j], a[m][i].x, a[m][2 + i].x, a[m][i].y, a[m][2 + i].y, b[j][i].x, b[j][i].y);
+                        mma_16816(acc[m][j], a[m][i].z, a[m][2 + i].z, a[m][i].w, a[m][2 + i].w, b[j][i].z, b[j][i].w);
+                    }
+        }
+        if (tile != blockIdx.x) __syncthreads();         // the sums of the tile before have been read
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sums[warp][m][g + 8 * (e >> 1)][8 * j + 2 * t + (e & 1)] = acc[m][j][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < OUT * p.N; i += C::THREADS) {
+            const int c = i % OUT, n = i / OUT, col = tile * OUT + c;
+            if (col >= p.R) continue;
+            const int m = c / (GLU ? 8 : 16), r = c % (GLU ? 8 : 16);
+            float v = 0.0f, u = 0.0f;
+#pragma unroll
+            for (int w = 0; w < C::WARPS; ++w) {
+                v += sums[w][m][r][n];
+                if (GLU) u += sums[w][m][r + 8][n];
+            }
+            if (p.bias) v += __half2float(p.bias[col]);
+            if constexpr (GLU) {
+                if (p.bias) u += __half2float(p.bias[p.R + col]);
+                if (p.gu) {
+                    p.gu[(size_t)n * 2 * p.R + col] = __float2half_rn(v);
+                    p.gu[(size_t)n * 2 * p.R + p.R + col] = __float2half_rn(u);
                 }
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < MATS; ++m)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            sums[warp][m][g][8 * j + 2 * t] = acc[m][j][0];
-            sums[warp][m][g][8 * j + 2 * t + 1] = acc[m][j][1];
-            sums[warp][m][g + 8][8 * j + 2 * t] = acc[m][j][2];
-            sums[warp][m][g + 8][8 * j + 2 * t + 1] = acc[m][j][3];
-        }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kRows * 8 * NT; i += kThreads) {
-        const int r = i % kRows, n = i / kRows, row = r0 + r;
-        if (n >= p.N || row >= p.R) continue;
-        float v[MATS];
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-            v[m] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) v[m] += sums[w][m][r][n];
-            if (p.bias) v[m] += __half2float(p.bias[m * p.R + row]);
-        }
-        if constexpr (GLU) {
-            if (p.gu) {
-                p.gu[(size_t)n * 2 * p.R + row] = __float2half_rn(v[0]);
-                p.gu[(size_t)n * 2 * p.R + p.R + row] = __float2half_rn(v[1]);
+                v = glu_act(v, p.act) * u;
+            } else if (p.residual) {
+                v += __half2float(p.residual[n * p.ldr + col]);
             }
-            v[0] = glu_act(v[0], p.act) * v[1];
-        } else if (p.residual) {
-            v[0] += __half2float(p.residual[n * p.ldr + row]);
+            p.out[n * p.ldo + col] = __float2half_rn(v);
         }
-        p.out[n * p.ldo + row] = __float2half_rn(v[0]);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <int NT, bool WIDE, bool GLU>
+int launch_few(rbk_ctx* ctx, const Params& p, cudaStream_t st) {
+    using C = Few<NT, WIDE>;
+    static int configured_device = -1;   // attribute is per device; one device per process
+    if (configured_device != ctx->device) {
+        RBK_CUDA(cudaFuncSetAttribute(few_rows_kernel<NT, WIDE, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        configured_device = ctx->device;
+    }
+    // the same number of tiles, or one fewer, for every CTA
+    const int out = (GLU ? 8 : 16) * C::MT, tiles = (p.R + out - 1) / out, slots = C::PER_SM * ctx->num_sms;
+    const int each = (tiles + slots - 1) / slots;
+    RBK_CUDA(launch_pdl(few_rows_kernel<NT, WIDE, GLU>, dim3((tiles + each - 1) / each), dim3(C::THREADS), C::SMEM, st, p));
+    RBK_LAUNCHED("few_rows_kernel");
+    return RBK_OK;
 }
 
 template <bool GLU>
 int few_rows(rbk_ctx* ctx, const Params& p, cudaStream_t st) {
-    const dim3 grid((p.R + kRows - 1) / kRows), block(kThreads);
     ProfScope prof(ctx, st, kCatGemm, (GLU ? 4.0 : 2.0) * p.N * (double)p.R * p.K, 0);
-    if (p.N <= 8) RBK_CUDA(launch_pdl(few_rows_kernel<1, GLU>, grid, block, 0, st, p));
-    else if (p.N <= 16) RBK_CUDA(launch_pdl(few_rows_kernel<2, GLU>, grid, block, 0, st, p));
-    else RBK_CUDA(launch_pdl(few_rows_kernel<4, GLU>, grid, block, 0, st, p));
-    RBK_LAUNCHED("few_rows_kernel");
-    return RBK_OK;
+    const bool wide = (p.R + (GLU ? 7 : 15)) / (GLU ? 8 : 16) <= ctx->num_sms;
+    if (p.N <= 8) return wide ? launch_few<1, true, GLU>(ctx, p, st) : launch_few<1, false, GLU>(ctx, p, st);
+    if (p.N <= 16) return wide ? launch_few<2, true, GLU>(ctx, p, st) : launch_few<2, false, GLU>(ctx, p, st);
+    return wide ? launch_few<4, true, GLU>(ctx, p, st) : launch_few<4, false, GLU>(ctx, p, st);
 }
 
 static int check_sizes(const char* who, int N, int D, int F, int act) {
@@ -193,6 +300,9 @@ int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
         d.bias = (const half*)a->bd;
         d.residual = (const half*)a->residual; d.ldr = a->ldr;
         d.out = (half*)a->y; d.ldo = a->ldy;
+        // The kernel before is the one above, which began only when everything before it had ended and writes no
+        // weights: wd is as it will be, h is not.
+        d.early = 1;
         return ffn::few_rows<false>(ctx, d, st);
     }
     RBK_TRY(glu_fwd_tiles(ctx, a->h, a->gu, a->x, a->ldx, a->wgu, a->bgu, a->N, a->D, a->F, a->act, st));

@@ -8,6 +8,7 @@ device of the active context; there is no host or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes as C
+import itertools
 import operator
 import struct
 import threading
@@ -213,13 +214,13 @@ def clip_grad_norm(grads, max_norm, scaler=None, out=None):
                          f"{sorted({(str(g.dtype), str(g.device), g.is_contiguous()) for g in grads})}")
     at = to = list(map(T.data_ptr, grads))
     if out is not None:
-        some = [o for o in out if o is not None]
-        if len(out) != n or set(map(T.get_device, some)) - {dev} or not all(map(T.is_contiguous, some)) or any(
-                o is not None and (o.dtype is not k or o.numel() != s) for o, k, s in zip(out, kinds, sizes)):
+        some = [g if o is None else o for g, o in zip(grads, out)]
+        if (len(out) != n or list(map(_dtype, some)) != kinds or list(map(T.numel, some)) != sizes
+                or set(map(T.get_device, some)) - {dev} or not all(map(T.is_contiguous, some))):
             raise ValueError(f"out: expected {n} contiguous tensors (or None) of the gradients' types and sizes on cuda:{dev}")
         to = [0 if o is None else o.data_ptr() for o in out]
     sc = None if scaler is None else _here(scaler, torch.int32, "scaler", (8,))
-    table = struct.pack(f"{4 * n}q", *[v for row in zip(at, to, sizes, [k is f16 for k in kinds]) for v in row])
+    table = struct.pack(f"{4 * n}q", *itertools.chain.from_iterable(zip(at, to, sizes, [k is f16 for k in kinds])))
     norm = torch.empty(1, dtype=f32, device="cuda")
     ws = torch.empty(RBK_CLIP_WS_BYTES, dtype=torch.uint8, device="cuda")
     call("rbk_clip_grad_norm", ctx().handle, table, n, max_norm, sc, norm.data_ptr(), ws.data_ptr(), _s())
