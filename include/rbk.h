@@ -354,6 +354,7 @@ typedef struct rbk_ffn_args {
     void* y; int ldy;        /* [N, D]                                           */
     void* gu;                /* [N, 2F]: gate | up for the backward, or NULL     */
     void* h;                 /* [N, F]: scratch, or kept for the backward        */
+    void* ws; int64_t ws_bytes;      /* see rbk_gated_ffn_ws_bytes               */
 } rbk_ffn_args;
 int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* args, void* stream);
 
@@ -375,8 +376,14 @@ typedef struct rbk_ffn_bwd_args {
     void* dgu;                   /* [N, 2F], may be gu                           */
     void* dx; int lddx;
     float *dwgu, *dbgu, *dwd, *dbd;
+    void* ws; int64_t ws_bytes;      /* see rbk_gated_ffn_ws_bytes               */
 } rbk_ffn_bwd_args;
 int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* args, void* stream);
+/* Device memory that the two calls need as `ws` (often 0): where N and D give too few
+ * output tiles for the machine, the down projection (backward: dx) shares its inner
+ * extent out and adds FP32 planes in a fixed order.  ws NULL: the ctx scratch (see
+ * rbk_qk_args.ws). */
+int rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int64_t* fwd, int64_t* bwd);
 
 /* ------------------------------------------------------------------------
  * LoRA adapters, kernel level (the model level runs the same GEMMs inside

@@ -123,6 +123,12 @@ int glu_fwd_tiles(rbk_ctx* ctx, void* h, void* gu, const void* x, int ldx, const
 int glu_bwd_tiles(rbk_ctx* ctx, void* dgu, void* h, const void* dy, int lddy, const void* wd, const void* gu, int N, int D,
                   int F, int act, cudaStream_t st);
 
+// rbk_gemm with RBK_EPI_STORE_F16 and alpha = 1 (gemm.cu), with K shared out over several CTA pairs per tile
+// where the tiles alone leave most of the machine idle: gemm_store_splits FP32 planes [M, N] in ws, which a
+// second launch adds in order.  One split is rbk_gemm itself, and needs no ws.
+int gemm_store_splits(rbk_ctx* ctx, int M, int N, int K);
+int gemm_store(rbk_ctx* ctx, const rbk_gemm_desc* d, float* ws, cudaStream_t st);
+
 // Ticket slots (see rbk_ctx::tickets).
 enum TicketSlot {
     kTicketSum = 0,

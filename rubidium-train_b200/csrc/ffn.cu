@@ -258,12 +258,35 @@ static int check_ptr(const char* who, const char* what, const void* p, bool opti
     return RBK_OK;
 }
 
+// The FP32 planes of the down projection (backward: of dx), if the call splits it.
+static int64_t plane_bytes(rbk_ctx* ctx, int M, int N, int K) {
+    const int s = gemm_store_splits(ctx, M, N, K);
+    return s > 1 ? (int64_t)s * M * N * 4 : 0;
+}
+static int planes(rbk_ctx* ctx, const char* who, void* ws, int64_t ws_bytes, int64_t need, void** out) {
+    *out = ws;
+    if (!need) return RBK_OK;
+    if (!ws) return ctx_scratch(ctx, need, out);
+    RBK_REQUIRE(ws_bytes >= need, "%s: ws has %lld bytes, %lld are needed", who, (long long)ws_bytes, (long long)need);
+    return RBK_OK;
+}
+
 }  // namespace ffn
 }  // namespace rbk
 
 using namespace rbk;
 
 extern "C" {
+
+int rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int64_t* fwd, int64_t* bwd) {
+    const char* who = "rbk_gated_ffn_ws_bytes";
+    RBK_REQUIRE(fwd && bwd, "%s: null argument", who);
+    RBK_TRY(ffn::check_sizes(who, N, D, F, RBK_ACT_SILU));
+    RBK_REQUIRE(ctx, "%s: ctx is NULL", who);
+    *fwd = N <= ffn::kMaxTokens ? 0 : ffn::plane_bytes(ctx, N, D, F);
+    *bwd = N ? ffn::plane_bytes(ctx, N, D, 2 * F) : 0;
+    return RBK_OK;
+}
 
 int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
     const char* who = "rbk_gated_ffn_fwd";
@@ -279,6 +302,7 @@ int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
         RBK_TRY(ffn::check_ptr(who, "y", a->y, false, a->ldy, a->D));
         RBK_TRY(ffn::check_ptr(who, "gu", a->gu, true));
         RBK_TRY(ffn::check_ptr(who, "h", a->h, false));
+        RBK_TRY(ffn::check_ptr(who, "ws", a->ws, true));
     }
     RBK_TRY(check_device(ctx, who));
     if (!a->N) return RBK_OK;
@@ -305,6 +329,8 @@ int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
         d.early = 1;
         return ffn::few_rows<false>(ctx, d, st);
     }
+    void* ws;
+    RBK_TRY(ffn::planes(ctx, who, a->ws, a->ws_bytes, ffn::plane_bytes(ctx, a->N, a->D, a->F), &ws));
     RBK_TRY(glu_fwd_tiles(ctx, a->h, a->gu, a->x, a->ldx, a->wgu, a->bgu, a->N, a->D, a->F, a->act, st));
     rbk_gemm_desc d = {};
     d.M = a->N; d.N = a->D; d.K = a->F;
@@ -315,7 +341,7 @@ int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
     d.bias = a->bd;
     d.aux = a->residual; d.ld_aux = a->residual ? a->ldr : 0;
     d.alpha = 1.0f;
-    return rbk_gemm(ctx, &d, stream);
+    return gemm_store(ctx, &d, (float*)ws, st);
 }
 
 int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* a, void* stream) {
@@ -335,11 +361,15 @@ int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* a, void* stream) {
         RBK_TRY(ffn::check_ptr(who, "h", a->h, !a->recompute_h && !a->dwd));
         RBK_TRY(ffn::check_ptr(who, "dgu", a->dgu, false));
         RBK_TRY(ffn::check_ptr(who, "dx", a->dx, true, a->lddx, a->D));
+        RBK_TRY(ffn::check_ptr(who, "ws", a->ws, true));
     }
     RBK_TRY(check_device(ctx, who));
     if (!a->N) return RBK_OK;
+    cudaStream_t st = as_stream(stream);
+    void* ws = nullptr;
+    if (a->dx) RBK_TRY(ffn::planes(ctx, who, a->ws, a->ws_bytes, ffn::plane_bytes(ctx, a->N, a->D, 2 * a->F), &ws));
     RBK_TRY(glu_bwd_tiles(ctx, a->dgu, a->recompute_h ? a->h : nullptr, a->dy, a->lddy, a->wd, a->gu, a->N, a->D, a->F,
-                          a->act, as_stream(stream)));
+                          a->act, st));
     if (a->dx) {
         rbk_gemm_desc d = {};
         d.M = a->N; d.N = a->D; d.K = 2 * a->F;
@@ -348,7 +378,7 @@ int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* a, void* stream) {
         d.C = a->dx; d.ldc = a->lddx;
         d.epilogue = RBK_EPI_STORE_F16;
         d.alpha = 1.0f;
-        RBK_TRY(rbk_gemm(ctx, &d, stream));
+        RBK_TRY(gemm_store(ctx, &d, (float*)ws, st));
     }
     rbk_gemm_desc d = {};
     d.K = a->N;

@@ -24,6 +24,7 @@
 // Every mbarrier wait is bounded (globaltimer); on expiry the kernel records
 // RBK_ERR_TIMEOUT, drains, frees TMEM and returns.
 // No cluster multicast is used anywhere.
+#include <algorithm>
 #include <type_traits>
 
 #include "tc.cuh"
@@ -146,6 +147,7 @@ struct Params {
     // in split order.  Otherwise (several splits, atomic mode) every unit reduce-adds into C.
     float* part;        // [splits - 1][M][ldp], or nullptr (atomic mode)
     float* part_rows;   // [splits - 1][M] row-sum partials (dbias_rows)
+    int plane0;         // the split whose plane is the first: 1 as above, or 0: every split stores a plane
     int ldp;            // row pitch of a plane (N rounded up to 4)
     int c_zero;         // ACC_F32 into a C known to hold zeros: the owner stores without reading C
     // gated feed-forward epilogues: N is F; bias / aux are the gate's, bias2 / aux2 the up projection's
@@ -159,6 +161,7 @@ struct Params {
 // holds zeros stores its values (C + acc = acc) instead of reading C first.
 enum AccMode { kAccAtomic = 0, kAccOwner = 1, kAccPlane = 2, kAccStore = 3 };
 __device__ __forceinline__ int acc_mode(const Params& p, int split) {
+    if (p.part && p.plane0 == 0) return kAccPlane;
     if (split == 0 && (p.splits == 1 || p.part)) return p.c_zero ? kAccStore : kAccOwner;
     return p.part ? kAccPlane : kAccAtomic;
 }
@@ -397,6 +400,50 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(float* __restrict__ 
             for (int sp = 0; sp < splits; ++sp) a += part_rows[(size_t)sp * M + m];
             dbias[m] = a;
         }
+    }
+}
+
+// out[m, n] = sum over the planes, in split order, + bias[n] + aux[m, n], rounded to half: 8 columns a thread.
+__global__ void __launch_bounds__(256) splitk_store_kernel(half* __restrict__ out, int ldo, const float* __restrict__ part,
+                                                           int M, int N, int ldp, int splits,
+                                                           const half* __restrict__ bias, const half* aux, int ld_aux) {
+    grid_dependency_sync();
+    const int q8 = N >> 3;
+    const size_t total = (size_t)M * q8, plane = (size_t)M * ldp, stride = (size_t)gridDim.x * blockDim.x;
+    for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < total; i += stride) {
+        const int m = (int)(i / q8), c = (int)(i - (size_t)m * q8) * 8;
+        const float* src = part + (size_t)m * ldp + c;
+        float v[8] = {};
+        for (int s0 = 0; s0 < splits; s0 += 4) {               // four planes' loads in flight
+            float4 b[4][2];
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    b[s][k] = s0 + s < splits ? __ldcs(reinterpret_cast<const float4*>(src + (s0 + s) * plane + 4 * k))
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    v[4 * k] += b[s][k].x;
+                    v[4 * k + 1] += b[s][k].y;
+                    v[4 * k + 2] += b[s][k].z;
+                    v[4 * k + 3] += b[s][k].w;
+                }
+        }
+        float t[8];
+        if (bias) {
+            h8_to_f(*reinterpret_cast<const uint4*>(bias + c), t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += t[e];
+        }
+        if (aux) {
+            h8_to_f(*reinterpret_cast<const uint4*>(aux + (size_t)m * ld_aux + c), t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += t[e];
+        }
+        *reinterpret_cast<uint4*>(out + (size_t)m * ldo + c) = f_to_h8(v);
     }
 }
 
@@ -840,7 +887,7 @@ __device__ __forceinline__ void epilogue_chunk_f32_tma(const Params& p, int m0, 
         __syncwarp();
         if (lane == 0) {
             const uint32_t ts = st_s + hh * 2048;
-            if (EPI == RBK_EPI_ACC_F32 && mode == kAccPlane) tma_store_3d(tmP, ts, n + 16 * hh, m0, split - 1);
+            if (EPI == RBK_EPI_ACC_F32 && mode == kAccPlane) tma_store_3d(tmP, ts, n + 16 * hh, m0, split - p.plane0);
             else if (EPI == RBK_EPI_ACC_F32 && mode == kAccAtomic) tma_reduce_add_2d(tmC, ts, n + 16 * hh, m0);
             else tma_store_2d(tmC, ts, n + 16 * hh, m0);
             bulk_commit();
@@ -1294,7 +1341,7 @@ int launch_pair(rbk_ctx* ctx, const rbk_gemm_desc* d, Params& p, cudaStream_t st
     } else {
         RBK_TRY(make_tmap(&tc_, d->C, d->N, d->M, d->ldc, 16, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
                           CU_TENSOR_MAP_SWIZZLE_64B));
-        if (p.part) RBK_TRY(make_tmap_3d(&tp, p.part, d->N, d->M, p.splits - 1, p.ldp, 16, 32));
+        if (p.part) RBK_TRY(make_tmap_3d(&tp, p.part, d->N, d->M, p.splits - p.plane0, p.ldp, 16, 32));
     }
     if (!d->a_major) RBK_TRY(make_tmap(&ta, d->A, d->K, d->M, d->lda, 64, 128));
     else RBK_TRY(make_tmap(&ta, d->A, d->M, d->K, d->lda, 64, 64));
@@ -1409,6 +1456,48 @@ int glu_fwd_tiles(rbk_ctx* ctx, void* h, void* gu, const void* x, int ldx, const
     return launch_glu<kEpiGlu>(ctx, ta, tb, tg, tu, th, p, st);
 }
 
+int gemm_store_splits(rbk_ctx* ctx, int M, int N, int K) {
+    using namespace gemm;
+    const int units = ((M + 2 * BM - 1) / (2 * BM)) * ((N + 255) / 256), kb = (K + BK - 1) / BK;
+    const int s = std::min(ctx->num_sms / 2 / units, kb / 8);
+    if (s < 2) return 1;
+    const int per = (kb + s - 1) / s;
+    return (kb + per - 1) / per;
+}
+
+int gemm_store(rbk_ctx* ctx, const rbk_gemm_desc* d, float* ws, cudaStream_t st) {
+    using namespace gemm;
+    const int splits = gemm_store_splits(ctx, d->M, d->N, d->K);
+    if (splits < 2) return rbk_gemm(ctx, d, st);
+    rbk_gemm_desc e = *d;
+    e.C = ws;
+    e.ldc = d->N;
+    Params p = {};
+    p.M = d->M; p.N = d->N; p.K = d->K;
+    p.m_blocks = (d->M + 2 * BM - 1) / (2 * BM);
+    p.n_blocks = (d->N + 255) / 256;
+    p.k_blocks = (d->K + BK - 1) / BK;
+    p.splits = splits;
+    p.kb_per_split = (p.k_blocks + splits - 1) / splits;
+    p.units = p.m_blocks * p.n_blocks * splits;
+    p.a_mn = d->a_major; p.b_mn = d->b_major;
+    p.C = ws; p.ldc = p.ldp = d->N;
+    p.alpha = 1.0f;
+    p.err = ctx->tickets + kGemmError;
+    p.part = ws;
+    {
+        ProfScope prof(ctx, st, kCatGemm, 2.0 * d->M * (double)d->N * d->K, d->b_major ? 1 : 0);
+        RBK_TRY((launch_pair<RBK_EPI_ACC_F32, false>(ctx, &e, p, st)));
+    }
+    ProfScope prof(ctx, st, kCatOther, (4.0 * splits + 2.0) * d->M * d->N);
+    const size_t want = ((size_t)d->M * (d->N / 8) + 255) / 256;
+    const int blocks = (int)std::min(want, (size_t)ctx->num_sms * 8);
+    RBK_CUDA(launch_pdl(splitk_store_kernel, dim3(blocks), dim3(256), 0, st, (half*)d->C, d->ldc, (const float*)ws, d->M,
+                        d->N, p.ldp, splits, (const half*)d->bias, (const half*)d->aux, d->ld_aux ? d->ld_aux : d->ldc));
+    RBK_LAUNCHED("splitk_store_kernel");
+    return RBK_OK;
+}
+
 int glu_bwd_tiles(rbk_ctx* ctx, void* dgu, void* h, const void* dy, int lddy, const void* wd, const void* gu, int N, int D,
                   int F, int act, cudaStream_t st) {
     using namespace gemm;
@@ -1519,6 +1608,7 @@ int rbk_gemm(rbk_ctx* ctx, const rbk_gemm_desc* d, void* stream) {
     p.err = ctx->tickets + kGemmError;
     p.part = nullptr;
     p.part_rows = nullptr;
+    p.plane0 = 1;
     p.bias2 = p.aux2 = nullptr;
     p.act = p.store_gu = p.store_h = 0;
     p.ldp = (d->N + 3) & ~3;

@@ -64,14 +64,16 @@ class QkArgs(C.Structure):
 class FfnArgs(C.Structure):
     """rbk_ffn_args (include/rbk.h)."""
     _fields_ = [("N", i32), ("D", i32), ("F", i32), ("act", i32), ("x", vp), ("ldx", i32), ("wgu", vp), ("bgu", vp),
-                ("wd", vp), ("bd", vp), ("residual", vp), ("ldr", i32), ("y", vp), ("ldy", i32), ("gu", vp), ("h", vp)]
+                ("wd", vp), ("bd", vp), ("residual", vp), ("ldr", i32), ("y", vp), ("ldy", i32), ("gu", vp), ("h", vp),
+                ("ws", vp), ("ws_bytes", i64)]
 
 
 class FfnBwdArgs(C.Structure):
     """rbk_ffn_bwd_args (include/rbk.h)."""
     _fields_ = [("N", i32), ("D", i32), ("F", i32), ("act", i32), ("dy", vp), ("lddy", i32), ("x", vp), ("ldx", i32),
                 ("gu", vp), ("wgu", vp), ("wd", vp), ("h", vp), ("recompute_h", i32), ("dgu", vp), ("dx", vp),
-                ("lddx", i32), ("dwgu", vp), ("dbgu", vp), ("dwd", vp), ("dbd", vp)]
+                ("lddx", i32), ("dwgu", vp), ("dbgu", vp), ("dwd", vp), ("dbd", vp), ("ws", vp),
+                ("ws_bytes", i64)]
 
 
 class Grad(C.Structure):
@@ -138,6 +140,7 @@ _SIGS = {
     "rbk_qk_norm_rope_bwd": (i32, [vp, C.POINTER(QkArgs), vp]),
     "rbk_gated_ffn_fwd": (i32, [vp, C.POINTER(FfnArgs), vp]),
     "rbk_gated_ffn_bwd": (i32, [vp, C.POINTER(FfnBwdArgs), vp]),
+    "rbk_gated_ffn_ws_bytes": (i32, [vp, i32, i32, i32, C.POINTER(i64), C.POINTER(i64)]),
     "rbk_clip_grad_norm": (i32, [vp, C.c_char_p, i32, f32, vp, vp, vp, vp]),
     "rbk_model_create": (i32, [C.POINTER(vp), C.POINTER(Config), C.POINTER(ModelOpts)]),
     "rbk_model_destroy": (i32, [vp]),

@@ -423,6 +423,17 @@ def _rows(t, name, shape):
     return p, (st[0] if shape[0] > 1 else shape[1])
 
 
+def _ffn_ws(a, N, D, F, back, device):
+    """The workspace that the call needs, if any, from torch's allocator (a captured graph keeps its own)."""
+    fwd, bwd = C.c_int64(), C.c_int64()
+    call("rbk_gated_ffn_ws_bytes", ctx().handle, N, D, F, C.byref(fwd), C.byref(bwd))
+    n = bwd.value if back else fwd.value
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    if n:
+        a.ws, a.ws_bytes = ws.data_ptr(), n
+    return ws
+
+
 def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save=True, out=None):
     """y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd + residual (rbk_gated_ffn_fwd).
 
@@ -444,6 +455,7 @@ def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save
     gu = torch.empty((N, 2 * F), dtype=f16, device=x.device) if save else None
     a = FfnArgs(N, D, F, _ACTS[act], px, ldx, pwgu, pbgu, pwd, pbd, pres, ldr, py, ldy, gu.data_ptr() if save else None,
                 h.data_ptr())
+    ws = _ffn_ws(a, N, D, F, False, x.device) if N > 32 else None   # noqa: F841 (held until the launch)
     call("rbk_gated_ffn_fwd", ctx().handle, C.byref(a), _s())
     return y, gu, h
 
@@ -470,5 +482,6 @@ def gated_ffn_bwd(dy, x, gu, wgu, wd, act="silu", h=None, want_dx=True, dwgu=Non
                                 ("dbd", dbd, (D,)))]
     a = FfnBwdArgs(N, D, F, _ACTS[act], pdy, lddy, px, ldx, pgu, pwgu, pwd, _here(h, f16, "h", (N, F)), recompute,
                    _here(dgu, f16, "dgu", (N, 2 * F)), dx.data_ptr() if want_dx else None, D, *grads)
+    ws = _ffn_ws(a, N, D, F, True, dy.device) if want_dx else None   # noqa: F841 (held until the launch)
     call("rbk_gated_ffn_bwd", ctx().handle, C.byref(a), _s())
     return dx, dgu, h
