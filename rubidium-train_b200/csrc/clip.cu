@@ -8,8 +8,10 @@
 // The tensors' addresses travel as kernel parameters, so the call copies nothing to the device and can be
 // captured into a graph.
 //
-// A tensor is cut into chunks of 32 KB whose borders lie on 16-byte boundaries of g: whatever g's alignment, all
-// its vectors but the first and the last are whole.
+// A tensor is cut into chunks of 16 KB whose borders lie on 16-byte boundaries of g: whatever g's alignment, all
+// its vectors but the first and the last are whole.  A block has a run of neighbouring chunks, so it looks its
+// tensor up once (the table is in constant memory, a search is a chain of dependent reads); the second kernel
+// goes through the same run backwards, to find in L2 what the first read last.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -20,8 +22,9 @@ namespace rbk {
 namespace clip {
 
 constexpr int kThreads = 256;
-constexpr int kChunkBytes = 32 << 10;
+constexpr int kChunkBytes = 16 << 10;
 constexpr int kVec = kChunkBytes / 16 / kThreads;        // 16-byte vectors of a chunk per thread
+constexpr int kPerSm = 6;                                // blocks
 constexpr int kMaxBlocks = RBK_CLIP_WS_BYTES / 8;        // FP64 sums, of all launches of a call
 
 struct Tensor {
@@ -50,6 +53,13 @@ __device__ __forceinline__ int tensor_of(const Table<CAP>& tab, int c) {
     return lo;
 }
 
+// Chunks [a, b) of block `block` of `blocks`: as many as the others, or one more.
+__device__ __forceinline__ void run_of(int chunks, int block, int blocks, int& a, int& b) {
+    const int each = chunks / blocks, more = chunks % blocks;
+    a = block * each + min(block, more);
+    b = a + each + (block < more);
+}
+
 // Sum of squares of one 16-byte vector.  FP32 squares go to FP64 one by one: a square may be beyond FP32's
 // range.  FP16 squares are exact in FP32 (22 bits) and eight of them stay far below its largest value.
 __device__ __forceinline__ double squares(const uint4& v, int half) {
@@ -65,22 +75,37 @@ __device__ __forceinline__ double squares(const uint4& v, int half) {
     return fma(a, a, b * b) + fma(c, c, d * d);
 }
 
-// Vector i (16 bytes) of the aligned span that holds the tensor; elements outside it read as zero.
-// `skip` = elements between that span's start and g.
-__device__ __forceinline__ uint4 load_vec(const Tensor& t, long long i, int skip) {
-    const int ve = t.half ? 8 : 4;
-    const long long e = i * ve - skip;
-    if (e >= 0 && e + ve <= t.n) return *reinterpret_cast<const uint4*>(t.g + e * (t.half ? 2 : 4));
-    uint4 v = make_uint4(0, 0, 0, 0);
-    for (int j = 0; j < ve; ++j) {
-        if (e + j < 0 || e + j >= t.n) continue;
-        if (t.half) reinterpret_cast<unsigned short*>(&v)[j] = reinterpret_cast<const unsigned short*>(t.g)[e + j];
-        else reinterpret_cast<uint32_t*>(&v)[j] = reinterpret_cast<const uint32_t*>(t.g)[e + j];
-    }
-    return v;
+// One chunk of a tensor as this thread's kVec vectors, kThreads apart: `e` is the element at which its first one
+// starts (negative where the aligned span begins before g).
+struct Chunk {
+    long long e;
+    bool whole;                                          // every vector of the chunk, of all threads
+};
+__device__ __forceinline__ Chunk chunk_of(const Tensor& t, int c) {
+    const int ve = t.half ? 8 : 4, skip = (int)(reinterpret_cast<uintptr_t>(t.g) & 15u) / (t.half ? 2 : 4);
+    const long long e0 = (long long)(c - t.first) * (kChunkBytes / 16) * ve - skip;
+    return {e0 + (long long)threadIdx.x * ve, e0 >= 0 && e0 + (kChunkBytes / 16) * ve <= t.n};
 }
-__device__ __forceinline__ int skip_of(const Tensor& t) {
-    return (int)(reinterpret_cast<uintptr_t>(t.g) & 15u) / (t.half ? 2 : 4);
+__device__ __forceinline__ void load_chunk(uint4* v, const Tensor& t, const Chunk& k) {
+    const int ve = t.half ? 8 : 4;
+    if (k.whole) {
+        const uint4* p = reinterpret_cast<const uint4*>(t.g + k.e * (t.half ? 2 : 4));
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = p[i * kThreads];
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {                     // the ends of a tensor, element by element: zeros outside
+        const long long e = k.e + (long long)i * kThreads * ve;
+        uint32_t w[4] = {};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j >= ve || e + j < 0 || e + j >= t.n) continue;
+            if (t.half) w[j / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(t.g)[e + j] << (16 * (j & 1));
+            else w[j & 3] = reinterpret_cast<const uint32_t*>(t.g)[e + j];
+        }
+        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -105,46 +130,58 @@ template <int CAP>
 __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Table<CAP> tab, double* part) {
     grid_dependency_sync();
     double acc = 0.0;
-    for (int c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-        const Tensor& t = tab.t[tensor_of(tab, c)];
-        const int skip = skip_of(t);
-        const long long v0 = (long long)(c - t.first) * (kChunkBytes / 16) + threadIdx.x;
+    int c, end;
+    run_of(tab.chunks, blockIdx.x, gridDim.x, c, end);
+    for (int k = tensor_of(tab, c); c < end; ++c) {
+        while (k + 1 < tab.count && tab.t[k + 1].first <= c) ++k;
+        const Tensor& t = tab.t[k];
         uint4 v[kVec];
+        load_chunk(v, t, chunk_of(t, c));
+        if (t.half) {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = load_vec(t, v0 + i * kThreads, skip);
+            for (int i = 0; i < kVec; ++i) acc += squares(v[i], 1);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) acc += squares(v[i], t.half);
+            for (int i = 0; i < kVec; ++i) acc += squares(v[i], 0);
+        }
     }
     acc = block_sum(acc);
     if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
 
-// One 16-byte vector times coef, to out (whose alignment is its own).
-__device__ __forceinline__ void store_vec(const Tensor& t, long long i, int skip, uint4 v, float coef) {
-    const int ve = t.half ? 8 : 4;
-    const long long e = i * ve - skip;
-    if (e + ve <= 0 || e >= t.n) return;
-    if (t.half) {
+__device__ __forceinline__ uint4 scaled(uint4 v, int half, float coef) {
+    if (half) {
         float f[8];
         h8_to_f(v, f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] *= coef;
-        v = f_to_h8(f);
-    } else {
-        v.x = __float_as_uint(__uint_as_float(v.x) * coef);
-        v.y = __float_as_uint(__uint_as_float(v.y) * coef);
-        v.z = __float_as_uint(__uint_as_float(v.z) * coef);
-        v.w = __float_as_uint(__uint_as_float(v.w) * coef);
+        return f_to_h8(f);
     }
-    char* o = t.out + e * (t.half ? 2 : 4);
-    if (e >= 0 && e + ve <= t.n && (reinterpret_cast<uintptr_t>(o) & 15u) == 0) {
-        *reinterpret_cast<uint4*>(o) = v;
+    v.x = __float_as_uint(__uint_as_float(v.x) * coef);
+    v.y = __float_as_uint(__uint_as_float(v.y) * coef);
+    v.z = __float_as_uint(__uint_as_float(v.z) * coef);
+    v.w = __float_as_uint(__uint_as_float(v.w) * coef);
+    return v;
+}
+// A chunk to out, whose alignment is its own.
+__device__ __forceinline__ void store_chunk(const Tensor& t, const Chunk& k, const uint4* v) {
+    const int ve = t.half ? 8 : 4;
+    char* o = t.out + k.e * (t.half ? 2 : 4);
+    if (k.whole && (reinterpret_cast<uintptr_t>(t.out + (k.e - (long long)threadIdx.x * ve) * (t.half ? 2 : 4)) & 15u) == 0) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) reinterpret_cast<uint4*>(o)[i * kThreads] = v[i];
         return;
     }
-    for (int j = 0; j < ve; ++j) {
-        if (e + j < 0 || e + j >= t.n) continue;
-        if (t.half) reinterpret_cast<unsigned short*>(o)[j] = reinterpret_cast<const unsigned short*>(&v)[j];
-        else reinterpret_cast<uint32_t*>(o)[j] = reinterpret_cast<const uint32_t*>(&v)[j];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+        const long long e = k.e + (long long)i * kThreads * ve;
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j >= ve || e + j < 0 || e + j >= t.n) continue;
+            if (t.half) reinterpret_cast<unsigned short*>(t.out)[e + j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+            else reinterpret_cast<uint32_t*>(t.out)[e + j] = w[j & 3];
+        }
     }
 }
 
@@ -166,16 +203,18 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
     }
     __syncthreads();
     const float coef = coef_s;
-    for (int c = tab.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-        const Tensor& t = tab.t[tensor_of(tab, c)];
+    int begin, c;
+    run_of(tab.chunks, blockIdx.x, gridDim.x, begin, c);
+    for (int k = tensor_of(tab, --c); c >= begin; --c) {
+        while (tab.t[k].first > c) --k;
+        const Tensor& t = tab.t[k];
         if (!t.out || (t.out == t.g && coef == 1.0f)) continue;
-        const int skip = skip_of(t);
-        const long long v0 = (long long)(c - t.first) * (kChunkBytes / 16) + threadIdx.x;
+        const Chunk ch = chunk_of(t, c);
         uint4 v[kVec];
+        load_chunk(v, t, ch);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = load_vec(t, v0 + i * kThreads, skip);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) store_vec(t, v0 + i * kThreads, skip, v[i], coef);
+        for (int i = 0; i < kVec; ++i) v[i] = scaled(v[i], t.half, coef);
+        store_chunk(t, ch, v);
     }
 }
 
@@ -258,7 +297,7 @@ static int run(rbk_ctx* ctx, const rbk_grad* t, int count, float max_norm, const
     Table<CAP> tab;
     // each launch of the first kernel has its own stretch of the sums
     const int launches = std::max(1, (count + CAP - 1) / CAP);
-    const int per = std::max(1, std::min(4 * ctx->num_sms, kMaxBlocks / launches));
+    const int per = std::max(1, std::min(kPerSm * ctx->num_sms, kMaxBlocks / launches));
     RBK_REQUIRE(launches * per <= kMaxBlocks, "rbk_clip_grad_norm: more than %d tensors", kMaxBlocks * CAP);
     int parts = 0;
     for (int at = 0; at < count;) {
@@ -272,7 +311,7 @@ static int run(rbk_ctx* ctx, const rbk_grad* t, int count, float max_norm, const
     int at = 0;
     do {
         fill(tab, t, count, &at);
-        const int grid = std::max(1, std::min(4 * ctx->num_sms, tab.chunks));
+        const int grid = std::max(1, std::min(kPerSm * ctx->num_sms, tab.chunks));
         RBK_CUDA(launch_pdl(scale_kernel<CAP>, dim3(grid), dim3(kThreads), 0, st, tab, (const double*)part, parts,
                             max_norm, scaler, norm));
         RBK_LAUNCHED("scale_kernel");
