@@ -226,23 +226,25 @@ __device__ __forceinline__ float gelu_grad_f(float x) {
     return 0.5f * (1.0f + t) + 0.5f * x * (1.0f - t * t) * c * (1.0f + 3.0f * a * x * x);
 }
 
-// The gate activations z sigma(r(z)): SiLU with r = z, the tanh form of GELU with
-// r = 2 sqrt(2 / pi) (z + 0.044715 z^3), since (1 + tanh(r / 2)) / 2 = sigma(r).
-// The exponential and the quotient are the fast ones, right to about 2^-21: what
-// they feed is rounded to FP16 (2^-11).
-__device__ __forceinline__ float glu_sigma(float z, int act) {
-    const float c = 1.5957691216057308f, a = 0.044715f;
-    const float r = act == RBK_ACT_GELU ? c * z * (1.0f + a * z * z) : z;
-    return __fdividef(1.0f, 1.0f + __expf(-r));
+// 2^x and 1 / x by the hardware units (2 and 1 ulp; subnormals read and give 0).
+__device__ __forceinline__ float ex2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
-__device__ __forceinline__ float glu_act(float z, int act) { return z * glu_sigma(z, act); }
-// a = act(z), da = act'(z) = s + z s (1 - s) r'(z)
-__device__ __forceinline__ void glu_act_grad(float z, int act, float& a, float& da) {
-    const float c = 1.5957691216057308f, a3 = 3.0f * 0.044715f;
-    const float s = glu_sigma(z, act);
-    a = z * s;
-    const float dr = act == RBK_ACT_GELU ? c * (1.0f + a3 * z * z) : 1.0f;
-    da = s + a * (1.0f - s) * dr;
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The gate activations z sigma(r(z)): SiLU with r = z, the tanh form of GELU with
+// r = 2 sqrt(2 / pi) (z + 0.044715 z^3), since (1 + tanh(r / 2)) / 2 = sigma(r);
+// sigma(r) = 1 / (1 + 2^(-r log2 e)), right to 2^-20 where it is not negligible in
+// FP16, to which what it makes is rounded.
+constexpr float kGluLog2e = 1.4426950408889634f, kGluC = 1.5957691216057308f, kGluA = 0.044715f;
+__device__ __forceinline__ float glu_act(float z, int act) {
+    const float r = act == RBK_ACT_GELU ? kGluC * z * (1.0f + kGluA * z * z) : z;
+    return z * rcp_fast(1.0f + ex2_fast(-kGluLog2e * r));
 }
 
 }  // namespace rbk

@@ -751,8 +751,30 @@ __device__ __forceinline__ void add_bias32(float* v, const half* bias, int n, in
     }
 }
 
+// sigma(r(z)) of two gates at once (glu_act's formula on packed pairs), and act'(z) = s + a (1 - s) r'(z), a = z s.
+template <int ACT>
+__device__ __forceinline__ uint64_t glu_sigma2(uint64_t z, uint64_t zz) {
+    uint64_t t;                                            // -r log2 e
+    if constexpr (ACT == RBK_ACT_GELU)
+        t = pmul2(z, pfma2(zz, pair_of(-kGluLog2e * kGluC * kGluA), pair_of(-kGluLog2e * kGluC)));
+    else
+        t = pmul2(z, pair_of(-kGluLog2e));
+    const uint64_t d = padd2(pk2(ex2_fast(lo2(t)), ex2_fast(hi2(t))), pair_of(1.0f));
+    return pk2(rcp_fast(lo2(d)), rcp_fast(hi2(d)));
+}
+template <int ACT>
+__device__ __forceinline__ void glu_grad2(uint64_t z, uint64_t& a, uint64_t& da) {
+    const uint64_t zz = ACT == RBK_ACT_GELU ? pmul2(z, z) : 0;
+    const uint64_t s = glu_sigma2<ACT>(z, zz);
+    a = pmul2(z, s);
+    uint64_t e = pmul2(a, psub2(pair_of(1.0f), s));
+    if constexpr (ACT == RBK_ACT_GELU) e = pmul2(e, pfma2(zz, pair_of(3.0f * kGluC * kGluA), pair_of(kGluC)));
+    da = padd2(s, e);
+}
+
 // Gated feed-forward, one 32 x 32 chunk: g, u the gate's and the up projection's accumulators.  The warp's
 // three tiles take gate, up and h.
+template <int ACT>
 __device__ __forceinline__ void glu_chunk(const Params& p, int m0, int n, const uint32_t* rg, const uint32_t* ru,
                                           uint8_t* st, uint32_t st_s, int lane, const CUtensorMap* tmG,
                                           const CUtensorMap* tmU, const CUtensorMap* tmH) {
@@ -774,7 +796,12 @@ __device__ __forceinline__ void glu_chunk(const Params& p, int m0, int n, const 
         row_to_sw(st + 2048, lane, u);
     }
 #pragma unroll
-    for (int j = 0; j < 32; ++j) g[j] = glu_act(g[j], p.act) * u[j];
+    for (int j = 0; j < 32; j += 2) {
+        const uint64_t z = pk2(g[j], g[j + 1]), zz = ACT == RBK_ACT_GELU ? pmul2(z, z) : 0;
+        const uint64_t v = pmul2(pmul2(z, glu_sigma2<ACT>(z, zz)), pk2(u[j], u[j + 1]));
+        g[j] = lo2(v);
+        g[j + 1] = hi2(v);
+    }
     row_to_sw(st + 4096, lane, g);
     fence_proxy_async();
     __syncwarp();
@@ -789,6 +816,7 @@ __device__ __forceinline__ void glu_chunk(const Params& p, int m0, int n, const 
 }
 
 // Its backward: r the accumulators of dh, pg / pu this chunk's saved gate and up values (prefetch_h).
+template <int ACT>
 __device__ __forceinline__ void glu_bwd_chunk(const Params& p, int m0, int n, const uint32_t* r, uint8_t* st,
                                               uint32_t st_s, int lane, const uint4* pg, const uint4* pu,
                                               const CUtensorMap* tmG, const CUtensorMap* tmU,
@@ -804,21 +832,21 @@ __device__ __forceinline__ void glu_bwd_chunk(const Params& p, int m0, int n, co
     for (int k = 0; k < 4; ++k) {
         uint4* sg = reinterpret_cast<uint4*>(st + swoff(lane, k));
         uint4* su = reinterpret_cast<uint4*>(st + 2048 + swoff(lane, k));
-        float g[8], u[8], h[8];
-        h8_to_f(*sg, g);
-        h8_to_f(*su, u);
+        uint64_t g[4], u[4], h[4];
+        h8_to_p(*sg, g);
+        h8_to_p(*su, u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float d = __uint_as_float(r[8 * k + j]);
-            float a, da;
-            glu_act_grad(g[j], p.act, a, da);
-            h[j] = a * u[j];
-            g[j] = d * u[j] * da;
-            u[j] = d * a;
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t d = pk2(__uint_as_float(r[8 * k + 2 * j]), __uint_as_float(r[8 * k + 2 * j + 1]));
+            uint64_t a, da;
+            glu_grad2<ACT>(g[j], a, da);
+            h[j] = pmul2(a, u[j]);
+            g[j] = pmul2(pmul2(d, u[j]), da);
+            u[j] = pmul2(d, a);
         }
-        *sg = f_to_h8(g);
-        *su = f_to_h8(u);
-        if (p.store_h) *reinterpret_cast<uint4*>(st + 4096 + swoff(lane, k)) = f_to_h8(h);
+        *sg = p_to_h8(g);
+        *su = p_to_h8(u);
+        if (p.store_h) *reinterpret_cast<uint4*>(st + 4096 + swoff(lane, k)) = p_to_h8(h);
     }
     fence_proxy_async();
     __syncwarp();
@@ -1254,12 +1282,20 @@ __global__ void __launch_bounds__(PairEpi<EPI, ROW>::THREADS, 1)
                         prefetch_h(pu, p.aux2, lda, m0, nb * BN + (c + 1) * 32, p, lane);
                     }
                     tmem_wait_ld();
-                    glu_bwd_chunk(p, m0, nb * BN + c * 32, r, my_stage, my_stage_s, lane, cur, curu, &tmC, &tmX, &tmP);
+                    const int n = nb * BN + c * 32;
+                    if (p.act == RBK_ACT_GELU)
+                        glu_bwd_chunk<RBK_ACT_GELU>(p, m0, n, r, my_stage, my_stage_s, lane, cur, curu, &tmC, &tmX, &tmP);
+                    else
+                        glu_bwd_chunk<RBK_ACT_SILU>(p, m0, n, r, my_stage, my_stage_s, lane, cur, curu, &tmC, &tmX, &tmP);
                     continue;
                 }
                 tmem_wait_ld();
                 if constexpr (EPI == kEpiGlu) {
-                    glu_chunk(p, m0, nb * TILE_N + c * 32, r, ru, my_stage, my_stage_s, lane, &tmC, &tmX, &tmP);
+                    const int n = nb * TILE_N + c * 32;
+                    if (p.act == RBK_ACT_GELU)
+                        glu_chunk<RBK_ACT_GELU>(p, m0, n, r, ru, my_stage, my_stage_s, lane, &tmC, &tmX, &tmP);
+                    else
+                        glu_chunk<RBK_ACT_SILU>(p, m0, n, r, ru, my_stage, my_stage_s, lane, &tmC, &tmX, &tmP);
                 } else if constexpr (kTma) {
                     epilogue_chunk_tma<EPI>(p, m0, nb * BN + c * 32, r, my_stage, my_stage_s, lane, cur, &tmC, &tmX, sc);
                 } else {
