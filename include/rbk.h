@@ -379,11 +379,11 @@ typedef struct rbk_ffn_bwd_args {
     void* ws; int64_t ws_bytes;      /* see rbk_gated_ffn_ws_bytes               */
 } rbk_ffn_bwd_args;
 int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* args, void* stream);
-/* Device memory that the two calls need as `ws` (often 0): where N and D give too few
- * output tiles for the machine, the down projection (backward: dx) shares its inner
- * extent out and adds FP32 planes in a fixed order.  ws NULL: the ctx scratch (see
- * rbk_qk_args.ws). */
-int rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int64_t* fwd, int64_t* bwd);
+/* Bytes of device memory that the forward (backward != 0: the backward with dx) needs as
+ * `ws`, often 0, or a negative status: where N and D give too few output tiles for the
+ * machine, the down projection (backward: dx) shares its inner extent out and adds FP32
+ * planes in a fixed order.  ws NULL: the ctx scratch (see rbk_qk_args.ws). */
+int64_t rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int backward);
 
 /* ------------------------------------------------------------------------
  * LoRA adapters, kernel level (the model level runs the same GEMMs inside

@@ -163,25 +163,65 @@ __device__ __forceinline__ uint4 scaled(uint4 v, int half, float coef) {
     v.w = __float_as_uint(__uint_as_float(v.w) * coef);
     return v;
 }
-// A chunk to out, whose alignment is its own.
-__device__ __forceinline__ void store_chunk(const Tensor& t, const Chunk& k, const uint4* v) {
-    const int ve = t.half ? 8 : 4;
-    char* o = t.out + k.e * (t.half ? 2 : 4);
-    if (k.whole && (reinterpret_cast<uintptr_t>(t.out + (k.e - (long long)threadIdx.x * ve) * (t.half ? 2 : 4)) & 15u) == 0) {
+// Elements [a, b) of a vector to dst.
+__device__ __forceinline__ void store_part(char* dst, const uint4& v, int half, int a, int b) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (j < a || j >= b) continue;
+        if (half) reinterpret_cast<unsigned short*>(dst)[j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+        else if (j < 4) reinterpret_cast<uint32_t*>(dst)[j] = w[j];
+    }
+}
+// The 16 bytes that start s bytes (a multiple of 2, the same in all threads) into v followed by next.
+__device__ __forceinline__ uint4 funnel(const uint4& v, const uint4& next, int s) {
+    uint32_t a[8] = {v.x, v.y, v.z, v.w, next.x, next.y, next.z, next.w};
+    if (s & 4)
+#pragma unroll
+        for (int k = 0; k < 7; ++k) a[k] = a[k + 1];
+    if (s & 8)
+#pragma unroll
+        for (int k = 0; k < 6; ++k) a[k] = a[k + 2];
+    if (s & 2)
+#pragma unroll
+        for (int k = 0; k < 5; ++k) a[k] = __funnelshift_r(a[k], a[k + 1], 16);
+    return make_uint4(a[0], a[1], a[2], a[3]);
+}
+// A chunk to out, scaled.  out's alignment is its own: where its 16-byte vectors lie s bytes off g's, each is put
+// together from two neighbouring vectors of g, the second from the next lane (lane 31 reads it again).
+__device__ __forceinline__ void store_chunk(const Tensor& t, const Chunk& k, const uint4* v, float coef) {
+    const int ve = t.half ? 8 : 4, es = t.half ? 2 : 4;
+    char* o = t.out + k.e * es;
+    if (!k.whole) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {                 // the ends of a tensor
+            const long long e = k.e + (long long)i * kThreads * ve;
+            if (e + ve > 0 && e < t.n)
+                store_part(o + (long long)i * kThreads * 16, v[i], t.half, (int)max(0LL, -e), (int)min((long long)ve, t.n - e));
+        }
+        return;
+    }
+    const int s = (int)(-reinterpret_cast<uintptr_t>(o) & 15u);
+    if (s == 0) {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) reinterpret_cast<uint4*>(o)[i * kThreads] = v[i];
         return;
     }
+    if (threadIdx.x == 0) store_part(o, v[0], t.half, 0, s / es);
+    const uint4* g = reinterpret_cast<const uint4*>(t.g + k.e * es);
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-        const long long e = k.e + (long long)i * kThreads * ve;
-        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (j >= ve || e + j < 0 || e + j >= t.n) continue;
-            if (t.half) reinterpret_cast<unsigned short*>(t.out)[e + j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
-            else reinterpret_cast<uint32_t*>(t.out)[e + j] = w[j & 3];
+        uint4 next;
+        next.x = __shfl_down_sync(0xffffffffu, v[i].x, 1);
+        next.y = __shfl_down_sync(0xffffffffu, v[i].y, 1);
+        next.z = __shfl_down_sync(0xffffffffu, v[i].z, 1);
+        next.w = __shfl_down_sync(0xffffffffu, v[i].w, 1);
+        if (i == kVec - 1 && threadIdx.x == kThreads - 1) {
+            store_part(o + (long long)i * kThreads * 16, v[i], t.half, s / es, ve);
+            continue;
         }
+        if ((threadIdx.x & 31) == 31) next = scaled(g[i * kThreads + 1], t.half, coef);
+        *reinterpret_cast<uint4*>(o + s + (long long)i * kThreads * 16) = funnel(v[i], next, s);
     }
 }
 
@@ -214,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
         load_chunk(v, t, ch);
 #pragma unroll
         for (int i = 0; i < kVec; ++i) v[i] = scaled(v[i], t.half, coef);
-        store_chunk(t, ch, v);
+        store_chunk(t, ch, v, coef);
     }
 }
 

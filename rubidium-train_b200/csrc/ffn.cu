@@ -278,14 +278,12 @@ using namespace rbk;
 
 extern "C" {
 
-int rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int64_t* fwd, int64_t* bwd) {
+int64_t rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int backward) {
     const char* who = "rbk_gated_ffn_ws_bytes";
-    RBK_REQUIRE(fwd && bwd, "%s: null argument", who);
     RBK_TRY(ffn::check_sizes(who, N, D, F, RBK_ACT_SILU));
     RBK_REQUIRE(ctx, "%s: ctx is NULL", who);
-    *fwd = N <= ffn::kMaxTokens ? 0 : ffn::plane_bytes(ctx, N, D, F);
-    *bwd = N ? ffn::plane_bytes(ctx, N, D, 2 * F) : 0;
-    return RBK_OK;
+    if (N == 0 || (!backward && N <= ffn::kMaxTokens)) return 0;
+    return ffn::plane_bytes(ctx, N, D, backward ? 2 * F : F);
 }
 
 int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 PKG_ROOT = os.path.dirname(_HERE)
@@ -76,6 +77,13 @@ class FfnBwdArgs(C.Structure):
                 ("ws_bytes", i64)]
 
 
+# The same structs packed from a flat tuple of their fields (pointers as integers, 0 for NULL): a sixth of the
+# time of filling the ctypes struct, which counts where a call takes a few microseconds.
+QK_PACK = struct.Struct("7i f d 2Q i 2Q 24q 2Q i Q")
+FFN_PACK = struct.Struct("4i Q i 5Q i Q i 3Q q")
+FFN_BWD_PACK = struct.Struct("4i Q i Q i 4Q i 2Q i 5Q q")
+
+
 class Grad(C.Structure):
     """rbk_grad (include/rbk.h)."""
     _fields_ = [("g", vp), ("out", vp), ("n", i64), ("half", i64)]
@@ -136,12 +144,12 @@ _SIGS = {
     "rbk_gemm_wgrad": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, vp]),
     "rbk_attn_fwd": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, f32, vp]),
     "rbk_attn_bwd": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, vp]),
-    "rbk_qk_norm_rope_fwd": (i32, [vp, C.POINTER(QkArgs), vp]),
-    "rbk_qk_norm_rope_bwd": (i32, [vp, C.POINTER(QkArgs), vp]),
-    "rbk_gated_ffn_fwd": (i32, [vp, C.POINTER(FfnArgs), vp]),
-    "rbk_gated_ffn_bwd": (i32, [vp, C.POINTER(FfnBwdArgs), vp]),
-    "rbk_gated_ffn_ws_bytes": (i32, [vp, i32, i32, i32, C.POINTER(i64), C.POINTER(i64)]),
-    "rbk_clip_grad_norm": (i32, [vp, C.c_char_p, i32, f32, vp, vp, vp, vp]),
+    "rbk_qk_norm_rope_fwd": (i32, [vp, vp, vp]),
+    "rbk_qk_norm_rope_bwd": (i32, [vp, vp, vp]),
+    "rbk_gated_ffn_fwd": (i32, [vp, vp, vp]),
+    "rbk_gated_ffn_bwd": (i32, [vp, vp, vp]),
+    "rbk_gated_ffn_ws_bytes": (i64, [vp, i32, i32, i32, i32]),
+    "rbk_clip_grad_norm": (i32, [vp, vp, i32, f32, vp, vp, vp, vp]),
     "rbk_model_create": (i32, [C.POINTER(vp), C.POINTER(Config), C.POINTER(ModelOpts)]),
     "rbk_model_destroy": (i32, [vp]),
     "rbk_model_buffer": (i32, [vp, i32, C.POINTER(vp), C.POINTER(i64)]),

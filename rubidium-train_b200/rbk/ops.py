@@ -15,7 +15,7 @@ import threading
 
 import torch
 
-from ._lib import FfnArgs, FfnBwdArgs, GemmDesc, Heads, QkArgs, Scaler, TailArgs, call, lib
+from ._lib import FFN_BWD_PACK, FFN_PACK, QK_PACK, GemmDesc, RbkError, Scaler, TailArgs, call, lib
 
 EPI_STORE_F16, EPI_BIAS_GELU, EPI_GELU_BWD, EPI_ACC_F32, EPI_STORE_F32 = range(5)
 LN_REFERENCE_FORMULA = 1
@@ -327,16 +327,22 @@ def attn_bwd(qkv, o, dout, lse, B, S, H, dh, scale=None, dbias=None):
 RBK_QK_BWD_WS_BYTES = 1024 * 256 * 4
 
 
+_F16, _F32 = torch.float16, torch.float32
+_NO_HEADS = (0, 0, 0, 0)
+
+
 def _heads(t, name, shape):
-    p = _here(t, torch.float16, name, shape, whole=False)
+    """Address and strides of half heads [B, S, H, dh] with contiguous channels (an rbk_heads)."""
+    p = _here(t, _F16, name, shape, False)
     st = t.stride()
     if len(st) != 4 or (st[3] != 1 and shape[3] > 1):
         raise ValueError(f"{name}: expected [B, S, H, dh] heads with contiguous channels, got shape {tuple(t.shape)}, "
                          f"strides {st}")
-    return Heads(p, st[0], st[1], st[2])
+    return p, st[0], st[1], st[2]
 
 
-def _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out):
+def _qk_call(name, q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out, back=None):
+    """Checks the tensors, allocates what is not given and calls rbk_qk_norm_rope_*; returns the two outputs."""
     shape = q.shape
     hq = _heads(q, "q", shape)
     B, S, Hq, dh = shape
@@ -346,29 +352,40 @@ def _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, e
         if len(inv_freq) != rot // 2:
             raise ValueError(f"inv_freq: expected {rot // 2} values, got {len(inv_freq)}")
         freq = (C.c_double * max(1, len(inv_freq)))(*[float(x) for x in inv_freq])
-    pos = None if positions is None else _here(positions, torch.int32, "positions", (B, S))
-    pq = None if gq is None else _here(gq, torch.float16, "gq", (dh,))
-    pk = None if gk is None else _here(gk, torch.float16, "gk", (dh,))
-    kshape = (B, S, 0, dh) if k is None else (B, S, k.shape[2], dh)
-    a = QkArgs(B, S, Hq, kshape[2], dh, rot, bool(interleaved), eps, theta, C.cast(freq, C.c_void_p) if freq else None,
-               pos, pos0, pq, pk, hq)
-    a.kept = freq
-    if k is not None:
-        a.k = _heads(k, "k", kshape)
-    if out is not None:
-        a.oq = _heads(out[0], "out[0]", shape)
-        if k is not None:
-            a.ok = _heads(out[1], "out[1]", kshape)
-        return a, out[0], (None if k is None else out[1]), kshape
-    # queries and keys side by side, as the projection's rows hold them
-    row = (Hq + kshape[2]) * dh
-    both = torch.empty((B, S, Hq + kshape[2], dh), dtype=torch.float16, device=q.device)
-    at = both.data_ptr()
-    a.oq = Heads(at, S * row, row, dh)
+    pos = 0 if positions is None else _here(positions, torch.int32, "positions", (B, S))
+    pq = 0 if gq is None else _here(gq, _F16, "gq", (dh,))
+    pk = 0 if gk is None else _here(gk, _F16, "gk", (dh,))
     if k is None:
-        return a, both, None, kshape
-    a.ok = Heads(at + 2 * Hq * dh, S * row, row, dh)
-    return a, both.narrow(2, 0, Hq), both.narrow(2, Hq, kshape[2]), kshape
+        Hk, kshape, hk, ok = 0, None, _NO_HEADS, _NO_HEADS
+    else:
+        Hk = k.shape[2]
+        kshape = (B, S, Hk, dh)
+        hk = _heads(k, "k", kshape)
+    if out is None:
+        # queries and keys side by side, as the projection's rows hold them
+        both = torch.empty((B, S, Hq + Hk, dh), dtype=_F16, device=q.device)
+        at, row = both.data_ptr(), (Hq + Hk) * dh
+        oq = (at, S * row, row, dh)
+        out = both, None
+        if k is not None:
+            ok = (at + 2 * Hq * dh, S * row, row, dh)
+            stride = (S * row, row, dh, 1)
+            out = both.as_strided(shape, stride), both.as_strided(kshape, stride, Hq * dh)
+    else:
+        out = out[0], (None if k is None else out[1])
+        oq = _heads(out[0], "out[0]", shape)
+        if k is not None:
+            ok = _heads(out[1], "out[1]", kshape)
+    if back is None:
+        tail = _NO_HEADS + _NO_HEADS + (0, 0, 0, 0)
+    else:
+        dyq, dyk, dgq, dgk, add, ws = back
+        tail = (_heads(dyq, "dyq", shape) + (_NO_HEADS if k is None else _heads(dyk, "dyk", kshape))
+                + (dgq, dgk, add, ws.data_ptr()))
+    call(name, ctx().handle, QK_PACK.pack(B, S, Hq, Hk, dh, rot, bool(interleaved), eps, theta,
+                                          C.addressof(freq) if freq else 0, pos, pos0, pq, pk, *hq, *hk, *oq, *ok,
+                                          *tail), _s())
+    return out
 
 
 def qk_norm_rope_fwd(q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000.0, inv_freq=None, rot=None,
@@ -379,32 +396,26 @@ def qk_norm_rope_fwd(q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000
     [dh] gains.  positions: int32 [B, S], or None for pos0 + s.  inv_freq: rot / 2 host numbers, or None for
     theta^(-2 i / rot).  rot: leading channels that turn (default dh).  out: (yq, yk), e.g. the q and k blocks of
     the qkv rows that attn_fwd reads, or (q, k) themselves; by default one new tensor.  Returns (yq, yk)."""
-    a, yq, yk, _ = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
-    call("rbk_qk_norm_rope_fwd", ctx().handle, C.byref(a), _s())
-    return yq, yk
+    return _qk_call("rbk_qk_norm_rope_fwd", q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
 
 
 def qk_norm_rope_bwd(dyq, dyk, q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000.0, inv_freq=None,
                      rot=None, interleaved=False, eps=1e-6, out=None, dgq=None, dgk=None):
     """Its backward (rbk_qk_norm_rope_bwd): q, k as the forward read them.  Returns (dq, dk, dgq, dgk); given
     FP32 [dh] dgq, dgk accumulate, else both are new.  out: (dq, dk), may be (dyq, dyk)."""
-    a, dq, dk, kshape = _qk_args(q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
-    a.dyq = _heads(dyq, "dyq", q.shape)
-    if k is not None:
-        a.dyk = _heads(dyk, "dyk", kshape)
-    if k is not None and (dgq is None) != (dgk is None):
+    dh, add = q.shape[-1], dgq is not None
+    if add != (dgk is not None) and k is not None:
         raise ValueError("dgq and dgk: give both or neither")
-    if dgq is None:
-        dgq = torch.empty(a.dh, dtype=torch.float32, device=q.device)
-        dgk = None if k is None else torch.empty_like(dgq)
+    if add:
+        _here(dgq, _F32, "dgq", (dh,))
+        if k is not None:
+            _here(dgk, _F32, "dgk", (dh,))
     else:
-        a.accumulate = 1
-    a.dgq = _here(dgq, torch.float32, "dgq", (a.dh,))
-    if k is not None:
-        a.dgk = _here(dgk, torch.float32, "dgk", (a.dh,))
+        dgq = torch.empty(dh, dtype=_F32, device=q.device)
+        dgk = None if k is None else torch.empty_like(dgq)
     ws = torch.empty(RBK_QK_BWD_WS_BYTES, dtype=torch.uint8, device=q.device)
-    a.ws = ws.data_ptr()
-    call("rbk_qk_norm_rope_bwd", ctx().handle, C.byref(a), _s())
+    dq, dk = _qk_call("rbk_qk_norm_rope_bwd", q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out,
+                      (dyq, dyk, dgq.data_ptr(), 0 if k is None else dgk.data_ptr(), add, ws))
     return dq, dk, dgq, (None if k is None else dgk)
 
 
@@ -416,22 +427,22 @@ _ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU}
 
 def _rows(t, name, shape):
     """A half [N, D] tensor with contiguous rows; returns its address and row stride."""
-    p = _here(t, torch.float16, name, shape, whole=False)
+    p = _here(t, _F16, name, shape, False)
     st = t.stride()
     if st[1] != 1 and shape[1] > 1:
         raise ValueError(f"{name}: expected contiguous rows, got strides {st}")
     return p, (st[0] if shape[0] > 1 else shape[1])
 
 
-def _ffn_ws(a, N, D, F, back, device):
+def _ffn_ws(handle, N, D, F, back, device):
     """The workspace that the call needs, if any, from torch's allocator (a captured graph keeps its own)."""
-    fwd, bwd = C.c_int64(), C.c_int64()
-    call("rbk_gated_ffn_ws_bytes", ctx().handle, N, D, F, C.byref(fwd), C.byref(bwd))
-    n = bwd.value if back else fwd.value
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    if n:
-        a.ws, a.ws_bytes = ws.data_ptr(), n
-    return ws
+    n = lib().rbk_gated_ffn_ws_bytes(handle, N, D, F, back)
+    if n < 0:
+        raise RbkError(n, "rbk_gated_ffn_ws_bytes", lib().rbk_last_error().decode(errors="replace"))
+    if n == 0:
+        return None, 0, 0
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), n
 
 
 def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save=True, out=None):
@@ -440,23 +451,29 @@ def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save
     x [N, D], wgu [2F, D] (gate rows, then up rows), wd [D, F], biases [2F] and [D]: half.  act: "silu" or "gelu"
     (tanh form).  Returns (y, gu, h): gu [N, 2F] the two projections, for gated_ffn_bwd (None with save False),
     and h [N, F] the product.  out: y, may be residual."""
-    f16 = torch.float16
-    shape = x.shape
+    shape, dev = x.shape, x.device
     N, D = shape
     F = wd.shape[1]
     px, ldx = _rows(x, "x", shape)
-    pwgu, pwd = _here(wgu, f16, "wgu", (2 * F, D)), _here(wd, f16, "wd", (D, F))
-    pbgu = None if bgu is None else _here(bgu, f16, "bgu", (2 * F,))
-    pbd = None if bd is None else _here(bd, f16, "bd", (D,))
-    pres, ldr = (None, 0) if residual is None else _rows(residual, "residual", shape)
-    y = torch.empty(shape, dtype=f16, device=x.device) if out is None else out
-    py, ldy = _rows(y, "out", shape)
-    h = torch.empty((N, F), dtype=f16, device=x.device)
-    gu = torch.empty((N, 2 * F), dtype=f16, device=x.device) if save else None
-    a = FfnArgs(N, D, F, _ACTS[act], px, ldx, pwgu, pbgu, pwd, pbd, pres, ldr, py, ldy, gu.data_ptr() if save else None,
-                h.data_ptr())
-    ws = _ffn_ws(a, N, D, F, False, x.device) if N > 32 else None   # noqa: F841 (held until the launch)
-    call("rbk_gated_ffn_fwd", ctx().handle, C.byref(a), _s())
+    pwgu, pwd = _here(wgu, _F16, "wgu", (2 * F, D)), _here(wd, _F16, "wd", (D, F))
+    pbgu = 0 if bgu is None else _here(bgu, _F16, "bgu", (2 * F,))
+    pbd = 0 if bd is None else _here(bd, _F16, "bd", (D,))
+    pres, ldr = (0, 0) if residual is None else _rows(residual, "residual", shape)
+    if out is None:
+        y = torch.empty(shape, dtype=_F16, device=dev)
+        py, ldy = y.data_ptr(), D
+    else:
+        y = out
+        py, ldy = _rows(y, "out", shape)
+    h = torch.empty((N, F), dtype=_F16, device=dev)
+    gu, pgu = None, 0
+    if save:
+        gu = torch.empty((N, 2 * F), dtype=_F16, device=dev)
+        pgu = gu.data_ptr()
+    handle = ctx().handle
+    ws, pws, nws = _ffn_ws(handle, N, D, F, 0, dev)
+    call("rbk_gated_ffn_fwd", handle, FFN_PACK.pack(N, D, F, _ACTS[act], px, ldx, pwgu, pbgu, pwd, pbd, pres, ldr, py,
+                                                    ldy, pgu, h.data_ptr(), pws, nws), _s())
     return y, gu, h
 
 
@@ -465,23 +482,28 @@ def gated_ffn_bwd(dy, x, gu, wgu, wd, act="silu", h=None, want_dx=True, dwgu=Non
     """Its backward (rbk_gated_ffn_bwd) from the saved gu.  h: the forward's, or None to have it computed again.
     dwgu [2F, D], dbgu [2F], dwd [D, F], dbd [D]: FP32, accumulate; those left out are not computed.  dgu: may be gu.
     Returns (dx or None, dgu, h)."""
-    f16, f32 = torch.float16, torch.float32
-    shape = dy.shape
+    shape, dev = dy.shape, dy.device
     N, D = shape
     F = wd.shape[1]
     pdy, lddy = _rows(dy, "dy", shape)
     px, ldx = _rows(x, "x", shape)
-    pgu = _here(gu, f16, "gu", (N, 2 * F))
-    pwgu, pwd = _here(wgu, f16, "wgu", (2 * F, D)), _here(wd, f16, "wd", (D, F))
+    pgu = _here(gu, _F16, "gu", (N, 2 * F))
+    pwgu, pwd = _here(wgu, _F16, "wgu", (2 * F, D)), _here(wd, _F16, "wd", (D, F))
     recompute = h is None
-    h = torch.empty((N, F), dtype=f16, device=dy.device) if recompute else h
+    h = torch.empty((N, F), dtype=_F16, device=dev) if recompute else h
+    ph = _here(h, _F16, "h", (N, F))
     dgu = torch.empty_like(gu) if dgu is None else dgu
-    dx = torch.empty(shape, dtype=f16, device=dy.device) if want_dx else None
-    grads = [None if t is None else _here(t, f32, name, s)
-             for name, t, s in (("dwgu", dwgu, (2 * F, D)), ("dbgu", dbgu, (2 * F,)), ("dwd", dwd, (D, F)),
-                                ("dbd", dbd, (D,)))]
-    a = FfnBwdArgs(N, D, F, _ACTS[act], pdy, lddy, px, ldx, pgu, pwgu, pwd, _here(h, f16, "h", (N, F)), recompute,
-                   _here(dgu, f16, "dgu", (N, 2 * F)), dx.data_ptr() if want_dx else None, D, *grads)
-    ws = _ffn_ws(a, N, D, F, True, dy.device) if want_dx else None   # noqa: F841 (held until the launch)
-    call("rbk_gated_ffn_bwd", ctx().handle, C.byref(a), _s())
+    pdgu = _here(dgu, _F16, "dgu", (N, 2 * F))
+    handle = ctx().handle
+    dx, pdx, ws, pws, nws = None, 0, None, 0, 0
+    if want_dx:
+        dx = torch.empty(shape, dtype=_F16, device=dev)
+        pdx = dx.data_ptr()
+        ws, pws, nws = _ffn_ws(handle, N, D, F, 1, dev)
+    p1 = 0 if dwgu is None else _here(dwgu, _F32, "dwgu", (2 * F, D))
+    p2 = 0 if dbgu is None else _here(dbgu, _F32, "dbgu", (2 * F,))
+    p3 = 0 if dwd is None else _here(dwd, _F32, "dwd", (D, F))
+    p4 = 0 if dbd is None else _here(dbd, _F32, "dbd", (D,))
+    call("rbk_gated_ffn_bwd", handle, FFN_BWD_PACK.pack(N, D, F, _ACTS[act], pdy, lddy, px, ldx, pgu, pwgu, pwd, ph,
+                                                        recompute, pdgu, pdx, D, p1, p2, p3, p4, pws, nws), _s())
     return dx, dgu, h

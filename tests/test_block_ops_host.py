@@ -155,7 +155,7 @@ def clip(tensors, max_norm=1.0, norm=P, ws=P, count=None):
     from rbk import lib
     from rbk._lib import Grad
     arr = (Grad * max(1, len(tensors)))(*[Grad(*t) for t in tensors])
-    st = lib().rbk_clip_grad_norm(None, C.cast(arr, C.c_char_p), len(tensors) if count is None else count, max_norm,
+    st = lib().rbk_clip_grad_norm(None, C.cast(arr, C.c_void_p), len(tensors) if count is None else count, max_norm,
                                   None, norm, ws, None)
     return st, lib().rbk_last_error().decode()
 
@@ -185,6 +185,33 @@ def test_clip_accepts(tensors):
     """What is not refused for its tensors is refused for the missing context only."""
     st, msg = clip(tensors)
     assert st == -1 and "ctx is NULL" in msg
+
+
+def test_packed_args_are_the_structs():
+    """The packed forms that the ops pass have the structs' bytes."""
+    from rbk import _lib
+    for cls, pack in ((_lib.QkArgs, _lib.QK_PACK), (_lib.FfnArgs, _lib.FFN_PACK), (_lib.FfnBwdArgs, _lib.FFN_BWD_PACK)):
+        flat, n = [], 0
+
+        def fill(s):
+            nonlocal n
+            for f, ty in s._fields_:
+                if issubclass(ty, C.Structure):
+                    fill(getattr(s, f))
+                    continue
+                n += 1
+                setattr(s, f, n)
+                flat.append(n)
+
+        s = cls()
+        fill(s)
+        assert pack.pack(*flat) + bytes(C.sizeof(cls) - pack.size) == bytes(s)
+
+
+def test_ffn_ws_bytes_refusals():
+    from rbk import lib
+    for args in ((-1, 64, 128, 0), (4, 60, 128, 1), (4, 64, 0, 0), (64, 64, 128, 0)):
+        assert lib().rbk_gated_ffn_ws_bytes(None, *args) == -1
 
 
 def test_args_layouts_match_header(tmp_path):
