@@ -21,21 +21,26 @@ namespace ffn {
 // that use them takes elements 4 m .. 4 m + 3.
 // A lane copies its vectors of the next DEPTH - 1 rounds, across tiles, into slots of its own with cp.async and
 // waits for its own copies only: the weights stream without registers or barriers.
-constexpr int kMaxTokens = 32;
 
-// WIDE: at most one tile per SM, so a CTA has all of its shared memory for what is in flight; else two or three
-// CTAs share an SM.
+// Which calls they serve: up to 32 rows, and up to 64 of a block whose weights are few, where the tiles' fixed
+// cost is most of their time.  Measured at 33 to 64 rows, these kernels against the tiles: D 512, F 1024: 8 us
+// against 17; D 768, F 2048: 12 against 18; D 1024, F 2816: 20 against 21; D 2048, F 5632: 44 against 33.
+static bool few(int N, int D, int F) { return N <= 32 || (N <= 64 && (int64_t)D * F <= (3 << 20)); }
+
+// WIDE: at most one tile per SM, so a CTA has all of its shared memory for what is in flight; else up to three
+// CTAs share an SM, and a tile is 32 weight rows where x, which comes from L2 for each, is more than the weights
+// (16 rows n, D 1888, F 4312: 21.5 us with 16 weight rows, 16.6 with 32).
 template <int NT, bool WIDE>
 struct Few {
-    static constexpr int MT = NT == 4 && !WIDE ? 2 : 1;
+    static constexpr int MT = NT > 1 && !WIDE ? 2 : 1;
     static constexpr int WARPS = WIDE ? 8 : 4, THREADS = 32 * WARPS;
-    static constexpr int DEPTH = WIDE ? (NT == 1 ? 8 : NT == 2 ? 6 : 4) : (NT == 1 ? 6 : NT == 2 ? 4 : 3);
+    static constexpr int DEPTH = WIDE ? (NT == 1 ? 8 : NT == 2 ? 6 : NT == 4 ? 4 : 2) : (NT == 1 ? 6 : NT == 2 ? 4 : 3);
     static constexpr int VECS = 4 * MT + 2 * NT;         // 16-byte vectors of a lane and round
     static constexpr int ROUND = VECS * 512;
     static constexpr int RING = WARPS * DEPTH * ROUND;
     static constexpr int SUMS = WARPS * MT * 16 * (8 * NT + 1) * 4;
     static constexpr int SMEM = RING + SUMS;
-    static constexpr int PER_SM = WIDE ? 1 : NT == 4 ? 2 : 3;
+    static constexpr int PER_SM = WIDE || NT == 8 ? 1 : NT == 1 ? 3 : 2;
     static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory of an SM");
 };
 
@@ -239,7 +244,8 @@ int few_rows(rbk_ctx* ctx, const Params& p, cudaStream_t st) {
     const bool wide = (p.R + (GLU ? 7 : 15)) / (GLU ? 8 : 16) <= ctx->num_sms;
     if (p.N <= 8) return wide ? launch_few<1, true, GLU>(ctx, p, st) : launch_few<1, false, GLU>(ctx, p, st);
     if (p.N <= 16) return wide ? launch_few<2, true, GLU>(ctx, p, st) : launch_few<2, false, GLU>(ctx, p, st);
-    return wide ? launch_few<4, true, GLU>(ctx, p, st) : launch_few<4, false, GLU>(ctx, p, st);
+    if (p.N <= 32) return wide ? launch_few<4, true, GLU>(ctx, p, st) : launch_few<4, false, GLU>(ctx, p, st);
+    return wide ? launch_few<8, true, GLU>(ctx, p, st) : launch_few<8, false, GLU>(ctx, p, st);
 }
 
 static int check_sizes(const char* who, int N, int D, int F, int act) {
@@ -282,7 +288,7 @@ int64_t rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int backward) 
     const char* who = "rbk_gated_ffn_ws_bytes";
     RBK_TRY(ffn::check_sizes(who, N, D, F, RBK_ACT_SILU));
     RBK_REQUIRE(ctx, "%s: ctx is NULL", who);
-    if (N == 0 || (!backward && N <= ffn::kMaxTokens)) return 0;
+    if (N == 0 || (!backward && ffn::few(N, D, F))) return 0;
     return ffn::plane_bytes(ctx, N, D, backward ? 2 * F : F);
 }
 
@@ -305,7 +311,7 @@ int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
     RBK_TRY(check_device(ctx, who));
     if (!a->N) return RBK_OK;
     cudaStream_t st = as_stream(stream);
-    if (a->N <= ffn::kMaxTokens) {
+    if (ffn::few(a->N, a->D, a->F)) {
         ffn::Params p = {};
         p.N = a->N; p.R = a->F; p.K = a->D;
         p.w = (const half*)a->wgu;

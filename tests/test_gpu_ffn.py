@@ -32,7 +32,8 @@ def case(N, D, F, bias=False, res=False, seed=0):
 
 
 SIZES = [(1, 8, 8), (1, 64, 128), (2, 72, 24), (7, 520, 40), (8, 256, 264), (9, 64, 1000), (16, 136, 16), (17, 776, 520),
-         (31, 8, 2056), (32, 1024, 72), (33, 8, 8), (33, 64, 24), (64, 264, 136), (129, 72, 520), (257, 512, 1032),
+         (31, 8, 2056), (32, 1024, 72), (33, 8, 8), (33, 64, 24), (64, 264, 136), (23, 520, 2504), (10, 264, 2504),
+         (47, 776, 2504), (64, 2504, 1256), (50, 1256, 2512), (65, 64, 136), (129, 72, 520), (257, 512, 1032),
          (300, 776, 256), (1000, 136, 2056), (2500, 256, 640)]
 
 
