@@ -366,7 +366,8 @@ int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* args, void* stream);
  * dgu is rounded to half once; the weight gradients are FP32 and accumulate.
  * recompute_h: h is written by the first kernel from gu (it need not have been
  * kept); else the forward's h is read, and only by dWd.  dx, dwgu, dbgu, dwd and
- * dbd may be NULL (dbgu needs dwgu, dbd needs dwd); x is read for dwgu only. */
+ * dbd may be NULL (dbgu needs dwgu, dbd needs dwd); x is read for dwgu only.  dx
+ * may be dy or x: it is written last. */
 typedef struct rbk_ffn_bwd_args {
     int N, D, F;
     int act;
@@ -450,7 +451,8 @@ typedef struct rbk_heads {
  * The angle is taken modulo a turn in 64-bit fixed point, so it is as exact at
  * position 2^31 - 1 as at 1.
  *   dh a multiple of 8, 8 <= dh <= 256; rot a multiple of 16 (8 when
- *   interleaved), 0 <= rot <= dh; B, S >= 0; Hq, Hk >= 0 (Hk = 0: queries only).
+ *   interleaved), 0 <= rot <= dh; B, S >= 0; 0 <= Hq, Hk <= 2^20 (Hk = 0: queries
+ *   only); strides below 2^34.
  * No counterpart in the reference, whose positions are learned embeddings. */
 typedef struct rbk_qk_args {
     int B, S, Hq, Hk, dh;
@@ -462,10 +464,12 @@ typedef struct rbk_qk_args {
     int pos0;
     const void *gq, *gk;     /* half [dh] gains of queries and keys, or NULL     */
     rbk_heads q, k;          /* the heads before the normalisation               */
-    rbk_heads oq, ok;        /* forward: y (may be q, k themselves); backward: dx */
+    rbk_heads oq, ok;        /* forward: y (may be q, k themselves); backward: dx.
+                                Else they share no element with what is read     */
     /* backward only */
     rbk_heads dyq, dyk;      /* gradients of y (dx may be dy itself)             */
-    float *dgq, *dgk;        /* FP32 [dh] gradients of the gains, or NULL        */
+    float *dgq, *dgk;        /* FP32 [dh] gradients of the gains, or NULL; the same
+                                pointer twice (one gain for both): their sum     */
     int accumulate;          /* 1: dgq, dgk += ; 0: they are set                 */
     /* Scratch of the backward: RBK_QK_BWD_WS_BYTES of device memory, or NULL for
      * the ctx scratch.  A caller that captures the call into a CUDA graph passes

@@ -269,11 +269,9 @@ static int64_t plane_bytes(rbk_ctx* ctx, int M, int N, int K) {
     const int s = gemm_store_splits(ctx, M, N, K);
     return s > 1 ? (int64_t)s * M * N * 4 : 0;
 }
-static int planes(rbk_ctx* ctx, const char* who, void* ws, int64_t ws_bytes, int64_t need, void** out) {
-    *out = ws;
-    if (!need) return RBK_OK;
-    if (!ws) return ctx_scratch(ctx, need, out);
-    RBK_REQUIRE(ws_bytes >= need, "%s: ws has %lld bytes, %lld are needed", who, (long long)ws_bytes, (long long)need);
+static int check_ws(const char* who, const void* ws, int64_t ws_bytes, int64_t need) {
+    RBK_REQUIRE(!ws || ws_bytes >= need, "%s: ws has %lld bytes, %lld are needed", who, (long long)ws_bytes,
+                (long long)need);
     return RBK_OK;
 }
 
@@ -333,8 +331,10 @@ int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
         d.early = 1;
         return ffn::few_rows<false>(ctx, d, st);
     }
-    void* ws;
-    RBK_TRY(ffn::planes(ctx, who, a->ws, a->ws_bytes, ffn::plane_bytes(ctx, a->N, a->D, a->F), &ws));
+    void* ws = a->ws;
+    const int64_t need = ffn::plane_bytes(ctx, a->N, a->D, a->F);
+    RBK_TRY(ffn::check_ws(who, ws, a->ws_bytes, need));
+    if (!ws && need) RBK_TRY(ctx_scratch(ctx, need, &ws));
     RBK_TRY(glu_fwd_tiles(ctx, a->h, a->gu, a->x, a->ldx, a->wgu, a->bgu, a->N, a->D, a->F, a->act, st));
     rbk_gemm_desc d = {};
     d.M = a->N; d.N = a->D; d.K = a->F;
@@ -369,21 +369,12 @@ int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* a, void* stream) {
     }
     RBK_TRY(check_device(ctx, who));
     if (!a->N) return RBK_OK;
+    const int64_t need = a->dx ? ffn::plane_bytes(ctx, a->N, a->D, 2 * a->F) : 0;
+    RBK_TRY(ffn::check_ws(who, a->ws, a->ws_bytes, need));
     cudaStream_t st = as_stream(stream);
-    void* ws = nullptr;
-    if (a->dx) RBK_TRY(ffn::planes(ctx, who, a->ws, a->ws_bytes, ffn::plane_bytes(ctx, a->N, a->D, 2 * a->F), &ws));
     RBK_TRY(glu_bwd_tiles(ctx, a->dgu, a->recompute_h ? a->h : nullptr, a->dy, a->lddy, a->wd, a->gu, a->N, a->D, a->F,
                           a->act, st));
-    if (a->dx) {
-        rbk_gemm_desc d = {};
-        d.M = a->N; d.N = a->D; d.K = 2 * a->F;
-        d.A = a->dgu; d.lda = 2 * a->F;
-        d.B = a->wgu; d.ldb = a->D; d.b_major = 1;            // B(n, k = gate or up row) = Wgu[k, n]
-        d.C = a->dx; d.ldc = a->lddx;
-        d.epilogue = RBK_EPI_STORE_F16;
-        d.alpha = 1.0f;
-        RBK_TRY(gemm_store(ctx, &d, (float*)ws, st));
-    }
+    // the weight gradients before dx, which may then lie over dy or x
     rbk_gemm_desc d = {};
     d.K = a->N;
     d.a_major = d.b_major = 1;
@@ -405,7 +396,17 @@ int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* a, void* stream) {
         d.dbias_rows = a->dbd;
         RBK_TRY(rbk_gemm(ctx, &d, stream));
     }
-    return RBK_OK;
+    if (!a->dx) return RBK_OK;
+    void* ws = a->ws;
+    if (!ws && need) RBK_TRY(ctx_scratch(ctx, need, &ws));        // after the GEMMs above, which may move it
+    rbk_gemm_desc e = {};
+    e.M = a->N; e.N = a->D; e.K = 2 * a->F;
+    e.A = a->dgu; e.lda = 2 * a->F;
+    e.B = a->wgu; e.ldb = a->D; e.b_major = 1;                // B(n, k = gate or up row) = Wgu[k, n]
+    e.C = a->dx; e.ldc = a->lddx;
+    e.epilogue = RBK_EPI_STORE_F16;
+    e.alpha = 1.0f;
+    return gemm_store(ctx, &e, (float*)ws, st);
 }
 
 }  // extern "C"

@@ -378,6 +378,7 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
     const char* who = BWD ? "rbk_qk_norm_rope_bwd" : "rbk_qk_norm_rope_fwd";
     RBK_REQUIRE(a, "%s: args is NULL", who);
     RBK_REQUIRE(a->B >= 0 && a->S >= 0 && a->Hq >= 0 && a->Hk >= 0, "%s: negative size", who);
+    RBK_REQUIRE(a->Hq <= (1 << 20) && a->Hk <= (1 << 20), "%s: more than 2^20 heads", who);
     RBK_REQUIRE((long long)a->B * a->S <= 0x7fffffffLL, "%s: more than 2^31 - 1 tokens", who);
     RBK_REQUIRE(a->dh >= 8 && a->dh <= kMaxDh && a->dh % 8 == 0, "%s: dh must be a multiple of 8 in [8, %d], got %d",
                 who, kMaxDh, a->dh);
@@ -479,8 +480,11 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
         if (status != RBK_OK) return status;
     }
     if (BWD && (a->dgq || a->dgk)) {
-        RBK_CUDA(launch_pdl(qk_gain_kernel, dim3((a->dh + 31) / 32, 2), dim3(kThreads), 0, st, a->dgq, a->dgk,
-                            (const float*)p.part, a->dh, p.blocks0, grid, a->accumulate));
+        // one gradient for both: its first side's rows are all rows, and it has no second
+        const bool one_gain = a->dgq == a->dgk;
+        RBK_CUDA(launch_pdl(qk_gain_kernel, dim3((a->dh + 31) / 32, 2), dim3(kThreads), 0, st, a->dgq,
+                            one_gain ? nullptr : a->dgk, (const float*)p.part, a->dh, one_gain ? grid : p.blocks0, grid,
+                            a->accumulate));
         RBK_LAUNCHED("qk_gain_kernel");
     }
     return RBK_OK;

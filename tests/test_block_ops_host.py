@@ -35,6 +35,8 @@ def test_qk_refusals(name):
     from rbk._lib import Heads
     for kw, match in [
         (dict(B=-1), "negative"), (dict(Hk=-1), "negative"), (dict(B=65536, S=65536), "tokens"),
+        (dict(Hq=(1 << 20) + 1), "heads"), (dict(q=Heads(P, 1 << 35, 256, 64)), "2^34"),
+        (dict(oq=Heads(P, 1024, -(1 << 35), 64)), "2^34"),
         (dict(dh=0, rot=0), "dh"), (dict(dh=60, rot=0), "dh"), (dict(dh=264, rot=0), "dh"),
         (dict(rot=80), "rot"), (dict(rot=-16), "rot"), (dict(rot=24), "rot"), (dict(rot=4, interleaved=1), "rot"),
         (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(theta=0.0), "theta"),

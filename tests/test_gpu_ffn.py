@@ -82,6 +82,57 @@ def test_backward_accumulates_and_reads_the_kept_product(ops):
     within("dwd", dwd, want, (N + 2) * ref.E * (3.0 + c["dy"].double().abs().T @ h.double().abs()))
 
 
+@pytest.mark.parametrize("over", ["dy", "x"])
+@pytest.mark.parametrize("ws", [False, True])
+def test_dx_over_what_is_read_and_the_scratch_of_the_context(ops, over, ws):
+    """dx over dy or over x, with the call's own workspace and with the context's scratch, in the deterministic mode
+    whose weight gradients use that scratch too."""
+    import ctypes as C
+
+    from rbk._lib import FFN_BWD_PACK, call, lib
+    N, D, F = 600, 264, 1032
+    c = case(N, D, F, seed=6)
+    gu = (c["x"].float() @ c["wgu"].float().T).half()
+    want = {k: torch.zeros(s, device="cuda") for k, s in (("dwgu", (2 * F, D)), ("dwd", (D, F)))}
+    got = {k: torch.zeros_like(v) for k, v in want.items()}
+    fresh = ops.Context()                                  # no scratch yet: the first use allocates it
+    call("rbk_ctx_set_deterministic", fresh.handle, 1)
+    call("rbk_ctx_set_deterministic", ops.ctx().handle, 1)
+    dx, dgu, h = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], **want)
+    call("rbk_ctx_set_deterministic", ops.ctx().handle, 0)
+    t = c[over]
+    n = lib().rbk_gated_ffn_ws_bytes(fresh.handle, N, D, F, 1)
+    assert n > 0                                           # these sizes share K out
+    buf = torch.empty(n, dtype=torch.uint8, device="cuda")
+    h2, dgu2 = torch.empty_like(h), torch.empty_like(dgu)
+    args = FFN_BWD_PACK.pack(N, D, F, 0, c["dy"].data_ptr(), D, c["x"].data_ptr(), D, gu.data_ptr(), c["wgu"].data_ptr(),
+                             c["wd"].data_ptr(), h2.data_ptr(), 1, dgu2.data_ptr(), t.data_ptr(), D,
+                             got["dwgu"].data_ptr(), 0, got["dwd"].data_ptr(), 0, buf.data_ptr() if ws else 0,
+                             n if ws else 0)
+    call("rbk_gated_ffn_bwd", fresh.handle, args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert torch.equal(t, dx) and torch.equal(h2, h) and torch.equal(dgu2, dgu)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+def test_a_workspace_that_is_too_small_is_refused(ops):
+    from rbk._lib import FFN_BWD_PACK, FFN_PACK, lib
+    N, D, F = 100, 264, 2056
+    c = case(N, D, F, seed=7)
+    gu, dgu, dx = (torch.zeros(N, k, device="cuda").half() for k in (2 * F, 2 * F, D))
+    y, h, ws = torch.zeros_like(c["x"]), torch.zeros(N, F, device="cuda").half(), torch.zeros(256, device="cuda")
+    args = FFN_PACK.pack(N, D, F, 0, c["x"].data_ptr(), D, c["wgu"].data_ptr(), 0, c["wd"].data_ptr(), 0, 0, 0,
+                         y.data_ptr(), D, 0, h.data_ptr(), ws.data_ptr(), 256)
+    assert lib().rbk_gated_ffn_fwd(ops.ctx().handle, args, None) == -1
+    assert b"are needed" in lib().rbk_last_error()
+    args = FFN_BWD_PACK.pack(N, D, F, 0, c["dy"].data_ptr(), D, c["x"].data_ptr(), D, gu.data_ptr(), c["wgu"].data_ptr(),
+                             c["wd"].data_ptr(), h.data_ptr(), 1, dgu.data_ptr(), dx.data_ptr(), D, 0, 0, 0, 0,
+                             ws.data_ptr(), 256)
+    assert lib().rbk_gated_ffn_bwd(ops.ctx().handle, args, None) == -1
+    assert b"are needed" in lib().rbk_last_error()
+    assert not any(bool(t.any()) for t in (y, h, dgu, dx))     # nothing has run
+
+
 @pytest.mark.parametrize("N", [5, 100])
 def test_strides_and_what_lies_beside(ops, N):
     """Row strides of x, residual and y; y over the residual; neighbours of the rows stay as they were."""

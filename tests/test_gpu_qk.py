@@ -123,6 +123,18 @@ def test_no_gain_own_frequencies_and_accumulation(ops):
     assert torch.equal(a, dgq + nq) and torch.equal(b, dgk + nk)
 
 
+def test_one_gain_for_queries_and_keys(ops):
+    B, S, dh = 2, 90, 64
+    q, k, g, _, dyq, dyk, _ = case(B, S, 6, 2, dh, dh, False, "rows", "seq", 9)
+    _, _, a, b = ops.qk_norm_rope_bwd(dyq, dyk, q, k, g, g)
+    both = torch.full((dh,), 5.0, device="cuda")
+    ops.qk_norm_rope_bwd(dyq, dyk, q, k, g, g, dgq=both, dgk=both)
+    _, _, _, mq = ref.bwd(dyq, q, g, ref.angles(B, S, dh, 10000.0), dh, False, EPS)
+    _, _, _, mk = ref.bwd(dyk, k, g, ref.angles(B, S, dh, 10000.0), dh, False, EPS)
+    # the same terms in another order
+    assert bool(((both - 5.0 - (a + b)).abs() <= (64 + B * S * 8) * E * (mq + mk + 5.0)).all())
+
+
 def test_in_place_and_into_attention_rows(ops):
     """y over x gives the bits of y apart, and a qkv row's value block and its neighbours stay as they were."""
     B, S, H, dh = 2, 50, 6, 64
