@@ -5,6 +5,8 @@
 // Memory bound: the gradients are read for the norm, and where clipping bites (or out is not g) read again
 // and written.  Two launches, ordered by programmatic dependent launch: every block of the first leaves the
 // FP64 sum of its chunks, every block of the second adds those sums in the same order and scales its chunks.
+// 163 M FP32 gradients (652 MB), out of place: 331 us, 100 for the norm (6.5 TB/s) and 230 for the scaling
+// (5.7 TB/s); 48 tensors of 48 KB: 5.4 us.
 // The tensors' addresses travel as kernel parameters, so the call copies nothing to the device and can be
 // captured into a graph.
 //

@@ -4,7 +4,8 @@
 //   dh = dy Wd,  dgate = dh up act'(gate),  dup = dh act(gate),  dx = dgate Wg + dup Wu
 //
 // Many rows: tensor bound (6 N D F FLOP each way).  The CTA-pair GEMM of gemm.cu with epilogues of its own
-// makes h (gate and up tiles share one accumulator) and dgu; the other products are plain GEMMs.
+// makes h (gate and up tiles share one accumulator) and dgu; the other products are plain GEMMs.  8192 rows,
+// D 2048, F 5632: forward 430 to 490 us (the power limit moves it), backward without weight gradients 510 to 535.
 // Few rows: the weights, 6 D F bytes, are read once and that is the cost.  The kernels below stream them.
 #include "tc.cuh"
 
@@ -20,7 +21,10 @@ namespace ffn {
 // permuted for that, alike on both sides: lane 4 g + t holds k = 8 t .. 8 t + 7 of row g, and MMA m of the two
 // that use them takes elements 4 m .. 4 m + 3.
 // A lane copies its vectors of the next DEPTH - 1 rounds, across tiles, into slots of its own with cp.async and
-// waits for its own copies only: the weights stream without registers or barriers.
+// waits for its own copies only: the weights stream without registers or barriers.  Bound by HBM where the weights
+// are large (1 row, D 2048, F 5632: 15.1 us for both kernels, 69 MB, 4580 GB/s with two ramps; plain loads in
+// the loop took 22.4), by latency where they are not (D 768, F 2048: 5.0 us), and from 16 rows on also by x, which
+// every tile reads from L2 (32 rows: 26.7 us).
 
 // Which calls they serve: up to 32 rows, and up to 64 of a block whose weights are few, where the tiles' fixed
 // cost is most of their time.  Measured at 33 to 64 rows, these kernels against the tiles: D 512, F 1024: 8 us
