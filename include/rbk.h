@@ -457,7 +457,7 @@ typedef struct rbk_heads {
 typedef struct rbk_qk_args {
     int B, S, Hq, Hk, dh;
     int rot, interleaved;
-    float eps;               /* > 0                                              */
+    float eps;               /* > 0, not subnormal                               */
     double theta;            /* inv_freq[i] = theta^(-2 i / rot) when inv_freq is NULL */
     const double* inv_freq;  /* host [rot / 2], radians per position, or NULL    */
     const int* positions;    /* device [B * S], or NULL: token (b, s) has pos0 + s */

@@ -22,6 +22,7 @@
 // and waits for its own copies only: no barrier, and no registers for what is in flight (with
 // the next step's vectors in registers the same forward took 55.6 us, the backward 93.2).
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "tc.cuh"
@@ -47,6 +48,7 @@ struct Side {                                // the queries or the keys
 struct Params {
     Side side[2];
     int tokens, S, dh, rot, interleaved;
+    uint32_t s_mul, s_shift;                 // token / S = (umulhi(token, s_mul) + token) >> s_shift
     int blocks0;                             // blocks [0, blocks0) work on side 0, the others on side 1
     float eps, inv_dh;
     const int* pos;
@@ -56,10 +58,24 @@ struct Params {
 };
 
 // cos and sin of position p's angle for a frequency of `freq` 2^-64 turns per position.  The product wraps
-// modulo 2^64 = modulo a turn, exactly; its top 32 bits, rounded, are the angle to 2^-32 turns.
+// modulo 2^64 = modulo a turn, exactly; its top 32 bits, rounded, are the angle to 2^-32 turns.  Split into the
+// nearest quarter turn and a rest of at most an eighth, x = 2 pi rest <= pi / 4, whose sine and cosine are Taylor
+// sums (the first terms left out: x^11 / 11! < 2^-28, x^10 / 10! < 2^-25).
 __device__ __forceinline__ void turn(int p, unsigned long long freq, float& c, float& s) {
     const unsigned long long t = (unsigned long long)(long long)p * freq + 0x80000000ull;
-    sincospif((float)(int)(t >> 32) * 4.656612873077393e-10f, &s, &c);      // 2^-31: half turns
+    const uint32_t u = (uint32_t)(t >> 32), q = (u + 0x20000000u) >> 30;
+    const float x = (float)(int)(u - (q << 30)) * 1.4629180792671596e-9f;   // 2 pi 2^-32
+    const float z = x * x;
+    const float sx = fmaf(x * z, fmaf(z, fmaf(z, fmaf(z, 1.0f / 362880.0f, -1.0f / 5040.0f), 1.0f / 120.0f), -1.0f / 6.0f), x);
+    const float cx = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1.0f / 40320.0f, -1.0f / 720.0f), 1.0f / 24.0f), -0.5f), 1.0f);
+    const float a = q & 1 ? sx : cx, b = q & 1 ? cx : sx;
+    c = __uint_as_float(__float_as_uint(a) ^ ((q + 1) << 30 & 0x80000000u));   // minus in quarters 1 and 2
+    s = __uint_as_float(__float_as_uint(b) ^ (q << 30 & 0x80000000u));         // minus in quarters 2 and 3
+}
+__device__ __forceinline__ float rsqrt_fast(float x) {
+    float y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // What a lane holds of a head: chunks (8 channels, one vector each) a and b.
@@ -189,14 +205,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_
     // the warp's token, or its first one: lanes with sub = 1 work on the next, if there is one
     int token = T * (w / sd.parts) < stride ? T * (w / sd.parts) : p.tokens, h = h0;
     auto next = [&](int tk) { return p.tokens - tk > stride ? tk + stride : p.tokens; };
+    auto row_of = [&](int tk) { return (int)((__umulhi((uint32_t)tk, p.s_mul) + (uint32_t)tk) >> p.s_shift); };
     auto at = [&](const Heads& t, int tk) {                         // this lane's chunk a of head h0
         tk = min(tk + sub, p.tokens - 1);
-        const int bi = (int)((unsigned)tk / (unsigned)p.S), si = tk - bi * p.S;
+        const int bi = row_of(tk), si = tk - bi * p.S;
         return t.p + ((long long)bi * t.sb + (long long)si * t.ss + (long long)h0 * t.sh + l.a);
     };
     auto pos_of = [&](int tk) {
         tk = min(tk + sub, p.tokens - 1);
-        return p.pos ? p.pos[tk] : p.pos0 + (int)((unsigned)tk % (unsigned)p.S);
+        return p.pos ? p.pos[tk] : p.pos0 + tk - row_of(tk) * p.S;
     };
     // whether this lane has head hd of token tk (+ sub)
     auto has = [&](int tk, int hd) { return hd < sd.H && (T == 1 || tk + sub < p.tokens); };
@@ -264,24 +281,30 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = pfma2(x.v[i], x.v[i], ss);
         if constexpr (!BWD) {
-            const float rstd = rsqrtf(group_sum<G>(lo2(ss) + hi2(ss)) * p.inv_dh + p.eps);
+            const float rstd = rsqrt_fast(group_sum<G>(lo2(ss) + hi2(ss)) * p.inv_dh + p.eps);
             const uint64_t r2 = pk2(rstd, rstd);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x.v[i] = pmul2(pmul2(x.v[i], r2), gain.v[i]);
             rotate<INTER, false>(l, x, cs, sn);
         } else {
             rotate<INTER, true>(l, e, cs, sn);
+            // d in e: m = d x gives both sums, sum of w x = m gain and the gain gradient's d xhat = m rstd
+            Row m;
             uint64_t wx = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) wx = pfma2(pmul2(e.v[i], gain.v[i]), x.v[i], wx);
-            const float rstd = rsqrtf(group_sum<G>(lo2(ss) + hi2(ss)) * p.inv_dh + p.eps);
-            const float t = -group_sum<G>(lo2(wx) + hi2(wx)) * rstd * p.inv_dh;   // -mean(w xhat)
+            for (int i = 0; i < 8; ++i) {
+                m.v[i] = pmul2(e.v[i], x.v[i]);
+                wx = pfma2(m.v[i], gain.v[i], wx);
+                e.v[i] = pmul2(e.v[i], gain.v[i]);                   // w
+            }
+            const float rstd = rsqrt_fast(group_sum<G>(lo2(ss) + hi2(ss)) * p.inv_dh + p.eps);
+            // dx = rstd w - x rstd^2 mean(w xhat)
+            const float t = -group_sum<G>(lo2(wx) + hi2(wx)) * p.inv_dh * rstd * rstd * rstd;
             const uint64_t r2 = pk2(rstd, rstd), t2 = pk2(t, t);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint64_t xh = pmul2(x.v[i], r2);
-                acc.v[i] = pfma2(e.v[i], xh, acc.v[i]);
-                x.v[i] = pmul2(pfma2(xh, t2, pmul2(e.v[i], gain.v[i])), r2);
+                acc.v[i] = pfma2(m.v[i], r2, acc.v[i]);
+                x.v[i] = pfma2(x.v[i], t2, pmul2(e.v[i], r2));
             }
         }
         const bool on = has(token, h);
@@ -388,7 +411,7 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
                 who, kMaxDh, a->dh);
     RBK_REQUIRE(a->rot >= 0 && a->rot <= a->dh && a->rot % (a->interleaved ? 8 : 16) == 0,
                 "%s: rot must be a multiple of %d in [0, dh], got %d", who, a->interleaved ? 8 : 16, a->rot);
-    RBK_REQUIRE(a->eps > 0.0f && std::isfinite(a->eps), "%s: eps must be positive", who);
+    RBK_REQUIRE(a->eps >= FLT_MIN && std::isfinite(a->eps), "%s: eps must be positive and normal", who);
     RBK_REQUIRE(a->inv_freq || a->rot == 0 || (a->theta > 0.0 && std::isfinite(a->theta)),
                 "%s: theta must be positive", who);
     RBK_REQUIRE((!a->gq || aligned16(a->gq)) && (!a->gk || aligned16(a->gk)), "%s: gains must be 16-byte aligned", who);
@@ -412,6 +435,9 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
     Params p;
     p.tokens = tokens;
     p.S = a->S;
+    p.s_shift = 0;
+    while (a->S > 0 && (1u << p.s_shift) < (uint32_t)a->S) ++p.s_shift;
+    p.s_mul = a->S > 0 ? (uint32_t)((((1ull << p.s_shift) - (uint32_t)a->S) << 32) / (uint32_t)a->S + 1) : 0;
     p.dh = a->dh;
     p.rot = a->rot;
     p.interleaved = a->interleaved != 0;
