@@ -210,6 +210,17 @@ def test_packed_args_are_the_structs():
         assert pack.pack(*flat) + bytes(C.sizeof(cls) - pack.size) == bytes(s)
 
 
+def test_workspace_sizes_match_header():
+    import os
+    import re
+
+    from rbk import ops
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "rbk.h")).read()
+    for name in ("RBK_QK_BWD_WS_BYTES", "RBK_CLIP_WS_BYTES"):
+        expr = re.search(rf"#define {name} \((.*)\)", src).group(1)
+        assert eval(expr) == getattr(ops, name), name
+
+
 def test_ffn_ws_bytes_refusals():
     from rbk import lib
     for args in ((-1, 64, 128, 0), (4, 60, 128, 1), (4, 64, 0, 0), (64, 64, 128, 0)):
