@@ -21,6 +21,7 @@ EPI_STORE_F16, EPI_BIAS_GELU, EPI_GELU_BWD, EPI_ACC_F32, EPI_STORE_F32 = range(5
 LN_REFERENCE_FORMULA = 1
 
 _tls = threading.local()
+_dev = torch._C._cuda_getDevice                          # the current device's index
 
 
 class Context:
@@ -65,7 +66,7 @@ def ctx() -> Context:
 
 
 def _s():
-    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(_dev()))
 
 
 def _p(t):
@@ -77,14 +78,16 @@ def _need(t, dtype, name):
         raise ValueError(f"{name}: expected a contiguous CUDA {dtype} tensor, got {t.dtype} on {t.device}")
 
 
-def _here(t, dtype, name, shape, whole=True):
-    """A tensor of this type and shape (contiguous unless whole is False) on the current device; returns its address."""
-    if t.dtype is dtype and t.shape == shape and t.get_device() == torch._C._cuda_getDevice() and (
-            not whole or t.is_contiguous()):
+def _refuse(t, dtype, name, shape, what):
+    raise ValueError(f"{name}: expected {what} {dtype} tensor of shape {tuple(shape)} on cuda:{torch.cuda.current_device()}, "
+                     f"got {t.dtype}, shape {tuple(t.shape)}, strides {t.stride()} on {t.device}")
+
+
+def _here(t, dtype, name, shape):
+    """The address of a contiguous tensor of this type and shape on the current device."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == _dev() and t.is_contiguous():
         return t.data_ptr()
-    raise ValueError(f"{name}: expected a{' contiguous' if whole else ''} {dtype} tensor of shape {tuple(shape)} on "
-                     f"cuda:{torch.cuda.current_device()}, got {t.dtype}, shape {tuple(t.shape)}, strides {t.stride()} on "
-                     f"{t.device}")
+    _refuse(t, dtype, name, shape, "a contiguous")
 
 
 # ----------------------------------------------------------------- LayerNorm --
@@ -204,7 +207,7 @@ def clip_grad_norm(grads, max_norm, scaler=None, out=None):
     grads: contiguous FP32 or half tensors.  scaler: a new_scaler() buffer (None: no loss scale).  out: a tensor for each
     of its gradient's type and size, or None in a place to count that gradient and not write it.  max_norm <= 0: only
     the norm is computed (and `out` is a copy)."""
-    dev, n = torch._C._cuda_getDevice(), len(grads)
+    dev, n = _dev(), len(grads)
     f32, f16 = torch.float32, torch.float16
     T = torch.Tensor
     kinds = list(map(_dtype, grads))
@@ -333,12 +336,11 @@ _NO_HEADS = (0, 0, 0, 0)
 
 def _heads(t, name, shape):
     """Address and strides of half heads [B, S, H, dh] with contiguous channels (an rbk_heads)."""
-    p = _here(t, _F16, name, shape, False)
     st = t.stride()
-    if len(st) != 4 or (st[3] != 1 and shape[3] > 1):
-        raise ValueError(f"{name}: expected [B, S, H, dh] heads with contiguous channels, got shape {tuple(t.shape)}, "
-                         f"strides {st}")
-    return p, st[0], st[1], st[2]
+    if (t.dtype is _F16 and t.shape == shape and t.get_device() == _dev() and len(st) == 4
+            and (st[3] == 1 or shape[3] == 1)):
+        return t.data_ptr(), st[0], st[1], st[2]
+    _refuse(t, _F16, name, shape, "heads [B, S, H, dh] with contiguous channels, a")
 
 
 def _qk_call(name, q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out, back=None):
@@ -362,15 +364,11 @@ def _qk_call(name, q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interlea
         kshape = (B, S, Hk, dh)
         hk = _heads(k, "k", kshape)
     if out is None:
-        # queries and keys side by side, as the projection's rows hold them
-        both = torch.empty((B, S, Hq + Hk, dh), dtype=_F16, device=q.device)
-        at, row = both.data_ptr(), (Hq + Hk) * dh
-        oq = (at, S * row, row, dh)
-        out = both, None
-        if k is not None:
-            ok = (at + 2 * Hq * dh, S * row, row, dh)
-            stride = (S * row, row, dh, 1)
-            out = both.as_strided(shape, stride), both.as_strided(kshape, stride, Hq * dh)
+        oq = torch.empty(shape, dtype=_F16, device=q.device)
+        ok = None if k is None else torch.empty(kshape, dtype=_F16, device=q.device)
+        out = oq, ok
+        oq = oq.data_ptr(), S * Hq * dh, Hq * dh, dh
+        ok = _NO_HEADS if k is None else (ok.data_ptr(), S * Hk * dh, Hk * dh, dh)
     else:
         out = out[0], (None if k is None else out[1])
         oq = _heads(out[0], "out[0]", shape)
@@ -395,7 +393,7 @@ def qk_norm_rope_fwd(q, k, gq=None, gk=None, positions=None, pos0=0, theta=10000
     q [B, S, Hq, dh], k [B, S, Hk, dh] (or None): half, any strides with contiguous channels.  gq, gk: half
     [dh] gains.  positions: int32 [B, S], or None for pos0 + s.  inv_freq: rot / 2 host numbers, or None for
     theta^(-2 i / rot).  rot: leading channels that turn (default dh).  out: (yq, yk), e.g. the q and k blocks of
-    the qkv rows that attn_fwd reads, or (q, k) themselves; by default one new tensor.  Returns (yq, yk)."""
+    the qkv rows that attn_fwd reads, or (q, k) themselves; by default new tensors.  Returns (yq, yk)."""
     return _qk_call("rbk_qk_norm_rope_fwd", q, k, gq, gk, positions, pos0, theta, inv_freq, rot, interleaved, eps, out)
 
 
@@ -426,12 +424,11 @@ _ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU}
 
 
 def _rows(t, name, shape):
-    """A half [N, D] tensor with contiguous rows; returns its address and row stride."""
-    p = _here(t, _F16, name, shape, False)
+    """Address and row stride of a half [N, D] tensor with contiguous rows."""
     st = t.stride()
-    if st[1] != 1 and shape[1] > 1:
-        raise ValueError(f"{name}: expected contiguous rows, got strides {st}")
-    return p, (st[0] if shape[0] > 1 else shape[1])
+    if t.dtype is _F16 and t.shape == shape and t.get_device() == _dev() and (st[1] == 1 or shape[1] == 1):
+        return t.data_ptr(), (st[0] if shape[0] > 1 else shape[1])
+    _refuse(t, _F16, name, shape, "contiguous rows, a")
 
 
 def _ffn_ws(handle, N, D, F, back, device):
