@@ -9,9 +9,10 @@
 // backward needs no statistics from the forward.
 //
 // Memory bound: 4 bytes per element forward, 6 backward, each touched once.  16384 tokens, 16 + 16 heads of
-// 128: forward 45.7 us = 5880 GB/s, backward 66.2 us = 6080 GB/s (0.91 and 0.94 of a copy's rate); 16384
-// tokens, 12 + 12 heads of 64: backward 28.1 us = 5380 GB/s; 32 tokens forward: 2.8 us, a launch.
-// Layout: a head is split over G lanes (the power of two >= dh / 16), a lane holding two
+// 128: forward 45.7 us = 5880 GB/s, backward 65.4 us = 6160 GB/s (0.91 and 0.95 of a copy's rate); 16384
+// tokens, 12 + 12 heads of 64: backward 27.5 us = 5490 GB/s; 32 tokens forward: 2.8 us, a launch.  Few heads
+// and odd widths are bound by their instructions: 65740 tokens, 3 + 3 heads of 80, backward 54 us = 3500 GB/s.
+// Layout: a head is split over G lanes (dh / 16, or the next of 8, 10 and 16), a lane holding two
 // 16-byte chunks of it, chosen so that both members of every rotated pair are in the
 // same lane: no exchange is needed for the rotation.  A warp, or each half of one (T = 2,
 // where fewer lanes then idle: 12 heads of 64 are 3 full steps of 4 for two tokens and not one
@@ -78,26 +79,33 @@ __device__ __forceinline__ float rsqrt_fast(float x) {
     return y;
 }
 
-// What a lane holds of a head: chunks (8 channels, one vector each) a and b.
+// What a lane holds of a head: chunks (8 channels, one vector each) a and b, each neighbours of the next lane's.
 struct Lane {
     int a, b;
     bool has_a, has_b, rot_a, rot_b;
+    int fa, fb;                              // the frequencies of its first and its last four pairs start here
 };
 __device__ __forceinline__ Lane lane_of(const Params& p, int j) {
     Lane l;
     const int chunks = p.dh >> 3, rs = p.rot >> 4;
-    if (p.interleaved) {
-        l.a = 2 * j;
-        l.b = l.a + 1;
+    if (p.interleaved) {                     // pairs within a chunk
+        l.a = j;
+        l.b = j + ((chunks + 1) >> 1);
+        l.has_a = l.a < (chunks + 1) >> 1;
         l.rot_a = l.a < (p.rot >> 3);
         l.rot_b = l.b < (p.rot >> 3);
-    } else {
-        l.a = j < rs ? j : 2 * j;
-        l.b = j < rs ? j + rs : 2 * j + 1;
+        l.fa = 4 * l.a;
+        l.fb = 4 * l.b;
+    } else {                                 // rs chunks and their partners, then those that do not turn
+        const int half = (chunks - 2 * rs + 1) >> 1, t = j - rs;
+        l.a = j < rs ? j : 2 * rs + t;
+        l.b = j < rs ? j + rs : 2 * rs + half + t;
+        l.has_a = j < rs || t < half;
         l.rot_a = l.rot_b = j < rs;
+        l.fa = 8 * j;
+        l.fb = 8 * j + 4;
     }
-    l.has_a = l.a < chunks;
-    l.has_b = l.b < chunks;
+    l.has_b = l.has_a && l.b < chunks;
     return l;
 }
 
@@ -151,43 +159,67 @@ __device__ __forceinline__ uint4 lds16(uint32_t src) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
     return v;
 }
+// The sum over the G lanes of this lane's group.  G a power of two: a butterfly.  Else running sums over the next
+// 2, 4, .. lanes of the group, in a circle, put together to G: each lane adds in an order of its own.
 template <int G>
-__device__ __forceinline__ float group_sum(float v) {
+__device__ __forceinline__ float group_sum(float v, int j) {
+    if constexpr ((G & (G - 1)) == 0) {
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+        for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    } else {
+        const int lane = threadIdx.x & 31;
+        auto ahead = [&](float x, int o) { return __shfl_sync(0xffffffffu, x, j + o < G ? lane + o : lane + o - G); };
+        float sum = 0.0f;
+        int done = 0;                                               // lanes in sum
+#pragma unroll
+        for (int n = 1; n <= G; n <<= 1) {                          // v: the next n lanes
+            if (G & n) {
+                sum = done ? sum + ahead(v, done) : v;
+                done += n;
+            }
+            if (2 * n <= G) v += ahead(v, n);
+        }
+        return sum;
+    }
 }
 
-// Blocks of an SM: 24 warps at 80 registers forward (32 at 64 registers spill: 53.0 us against 45.7), 16 at 128
-// backward.
-template <bool BWD>
-constexpr int kPerSm = BWD ? 2 : 3;
-// Steps in flight, and what a warp's step takes of shared memory: 128 KB and 96 KB per SM.
-template <bool BWD>
-constexpr int kDepth = BWD ? 3 : 4;
-template <bool BWD>
-constexpr int kStep = 32 * 16 * (BWD ? 4 : 2);
-template <bool BWD>
-constexpr int kSmem = kWarps * kDepth<BWD> * kStep<BWD>;
-static_assert(kWarps * kMaxDh * 4 <= kSmem<true>, "the gain gradients' warp sums reuse it");
+// Blocks of an SM, steps in flight and a step's bytes of a warp.  16 warps at 128 registers with 5 steps under way
+// (backward: 2 of twice the bytes); heads of 128, forward, one token a warp: 24 warps at 78 registers with 3 under
+// way, which is 45.8 us against 50.6 for 16384 tokens of 16 + 16 heads.  The other forwards are bound by their
+// instructions and lose at 80 registers: one head of 256 on each side 80 us against 41, 12 + 4 heads of 200 56
+// against 38, 12 + 12 of 64 alike.
+constexpr int per_sm(int lanes, int T, bool bwd) { return !bwd && lanes == 8 && T == 1 ? 3 : 2; }
+template <int G, int T, bool BWD>
+struct Flight {
+    static constexpr int PER_SM = per_sm(G, T, BWD);
+    static constexpr int DEPTH = BWD ? 3 : PER_SM == 3 ? 4 : 6;
+    static constexpr int STEP = 32 * 16 * (BWD ? 4 : 2);
+    static constexpr int SMEM = kWarps * DEPTH * STEP;
+};
+static_assert(kWarps * 32 * 16 * 4 <= Flight<1, 1, true>::SMEM, "the gain gradients' sums, at most 16 per lane, reuse it");
 
 template <int G, int T, bool INTER, bool BWD>
-__global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, per_sm(G, T, BWD)) qk_kernel(const __grid_constant__ Params p) {
     constexpr int HPS = 32 / T / G;                                 // heads of a token per step
-    constexpr int ANG = HPS >= 8 ? 1 : 8 / HPS;                     // angles that a lane computes of its slot's 8
-    constexpr int DEPTH = kDepth<BWD>, STEP = kStep<BWD>;
+    constexpr int ANG = (8 + HPS - 1) / HPS;                        // angles that a lane computes of its slot's 8
+    constexpr bool POW2 = (G & (G - 1)) == 0;                       // else some lanes are in no group
+    constexpr int DEPTH = Flight<G, T, BWD>::DEPTH, STEP = Flight<G, T, BWD>::STEP;
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int which = (int)blockIdx.x >= p.blocks0;
     const Side& sd = p.side[which];
     const int w = (which ? blockIdx.x - p.blocks0 : blockIdx.x) * kWarps + warp;
     const int stride = T * max(1, (int)(which ? gridDim.x - p.blocks0 : p.blocks0) * kWarps / sd.parts);   // tokens of a round
-    const int g = lane % (32 / T) / G, j = lane % G, sub = lane / (32 / T);
+    const int g = lane % (32 / T) / G, j = lane % (32 / T) % G, sub = lane / (32 / T);
     const Lane l = lane_of(p, j);
     const uint32_t slot = tc::su32(smem) + warp * (DEPTH * STEP) + lane * 16;
     unsigned long long freq[ANG];
 #pragma unroll
-    for (int i = 0; i < ANG; ++i) freq[i] = p.freq[8 * j + (g * ANG + i) % 8];
+    for (int i = 0; i < ANG; ++i) {
+        const int k = min(g * ANG + i, 7);
+        freq[i] = p.freq[min(k < 4 ? l.fa + k : l.fb + k - 4, kMaxDh / 2 - 1)];
+    }
     grid_dependency_sync();
 
     Row gain;
@@ -216,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_
         return p.pos ? p.pos[tk] : p.pos0 + tk - row_of(tk) * p.S;
     };
     // whether this lane has head hd of token tk (+ sub)
-    auto has = [&](int tk, int hd) { return hd < sd.H && (T == 1 || tk + sub < p.tokens); };
+    auto has = [&](int tk, int hd) { return hd < sd.H && (T == 1 || tk + sub < p.tokens) && (POW2 || g < HPS); };
 
     // The copies run DEPTH - 1 steps ahead of the work: token ft, head fh.
     int ft = token, fh = h0, fs = 0;
@@ -281,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = pfma2(x.v[i], x.v[i], ss);
         if constexpr (!BWD) {
-            const float rstd = rsqrt_fast(group_sum<G>(lo2(ss) + hi2(ss)) * p.inv_dh + p.eps);
+            const float rstd = rsqrt_fast(group_sum<G>(lo2(ss) + hi2(ss), j) * p.inv_dh + p.eps);
             const uint64_t r2 = pk2(rstd, rstd);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x.v[i] = pmul2(pmul2(x.v[i], r2), gain.v[i]);
@@ -297,9 +329,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_
                 wx = pfma2(m.v[i], gain.v[i], wx);
                 e.v[i] = pmul2(e.v[i], gain.v[i]);                   // w
             }
-            const float rstd = rsqrt_fast(group_sum<G>(lo2(ss) + hi2(ss)) * p.inv_dh + p.eps);
+            const float rstd = rsqrt_fast(group_sum<G>(lo2(ss) + hi2(ss), j) * p.inv_dh + p.eps);
             // dx = rstd w - x rstd^2 mean(w xhat)
-            const float t = -group_sum<G>(lo2(wx) + hi2(wx)) * p.inv_dh * rstd * rstd * rstd;
+            const float t = -group_sum<G>(lo2(wx) + hi2(wx), j) * p.inv_dh * rstd * rstd * rstd;
             const uint64_t r2 = pk2(rstd, rstd), t2 = pk2(t, t);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -319,28 +351,33 @@ __global__ void __launch_bounds__(kThreads, kPerSm<BWD>) qk_kernel(const __grid_
     }
     if constexpr (BWD) {
         // lanes of the same slot, then the warps, in a fixed order
-        float(*acc_s)[kMaxDh] = reinterpret_cast<float(*)[kMaxDh]>(smem);
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();                                            // the slots are free
+        constexpr int ROWS = POW2 ? 1 : T * HPS;                    // of sums that a warp leaves
+        auto acc_s = reinterpret_cast<float(*)[16 * G]>(smem);      // [kWarps * ROWS]
+        const int row = POW2 ? warp : warp * ROWS + sub * HPS + g;
+        const bool keeps = POW2 ? lane < G : g < HPS;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float a = lo2(acc.v[i]), b = hi2(acc.v[i]);
+            if constexpr (POW2) {
 #pragma unroll
-            for (int o = G; o < 32; o <<= 1) {
-                a += __shfl_xor_sync(0xffffffffu, a, o);
-                b += __shfl_xor_sync(0xffffffffu, b, o);
+                for (int o = G; o < 32; o <<= 1) {
+                    a += __shfl_xor_sync(0xffffffffu, a, o);
+                    b += __shfl_xor_sync(0xffffffffu, b, o);
+                }
             }
             const int c = i < 4 ? 8 * l.a + 2 * i : 8 * l.b + 2 * (i - 4);
-            if (lane < G && (i < 4 ? l.has_a : l.has_b)) {
-                acc_s[warp][c] = a;
-                acc_s[warp][c + 1] = b;
+            if (keeps && (i < 4 ? l.has_a : l.has_b)) {
+                acc_s[row][c] = a;
+                acc_s[row][c + 1] = b;
             }
         }
         __syncthreads();
         for (int c = threadIdx.x; c < p.dh; c += kThreads) {
             float v = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) v += acc_s[w][c];
+#pragma unroll 8
+            for (int w = 0; w < kWarps * ROWS; ++w) v += acc_s[w][c];
             p.part[(size_t)blockIdx.x * p.dh + c] = v;
         }
     }
@@ -371,15 +408,22 @@ __global__ void __launch_bounds__(kThreads) qk_gain_kernel(float* dgq, float* dg
     }
 }
 
+template <int G, int T, bool INTER, bool BWD>
+cudaError_t launch_one(const Params& p, int grid, cudaStream_t st) {
+    return launch_pdl(qk_kernel<G, T, INTER, BWD>, dim3(grid), dim3(kThreads), Flight<G, T, BWD>::SMEM, st, p);
+}
 template <int T, bool INTER, bool BWD>
 int launch(const Params& p, int lanes, int grid, cudaStream_t st) {
-    const dim3 gd(grid), bd(kThreads);
     switch (lanes) {
-        case 1: RBK_CUDA(launch_pdl(qk_kernel<1, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
-        case 2: RBK_CUDA(launch_pdl(qk_kernel<2, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
-        case 4: RBK_CUDA(launch_pdl(qk_kernel<4, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
-        case 8: RBK_CUDA(launch_pdl(qk_kernel<8, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
-        default: RBK_CUDA(launch_pdl(qk_kernel<16, T, INTER, BWD>, gd, bd, kSmem<BWD>, st, p)); break;
+        case 1: RBK_CUDA((launch_one<1, T, INTER, BWD>(p, grid, st))); break;
+        case 2: RBK_CUDA((launch_one<2, T, INTER, BWD>(p, grid, st))); break;
+        case 3: RBK_CUDA((launch_one<3, T, INTER, BWD>(p, grid, st))); break;
+        case 4: RBK_CUDA((launch_one<4, T, INTER, BWD>(p, grid, st))); break;
+        case 5: RBK_CUDA((launch_one<5, T, INTER, BWD>(p, grid, st))); break;
+        case 6: RBK_CUDA((launch_one<6, T, INTER, BWD>(p, grid, st))); break;
+        case 8: RBK_CUDA((launch_one<8, T, INTER, BWD>(p, grid, st))); break;
+        case 10: RBK_CUDA((launch_one<10, T, INTER, BWD>(p, grid, st))); break;
+        default: RBK_CUDA((launch_one<16, T, INTER, BWD>(p, grid, st))); break;
     }
     RBK_LAUNCHED("qk_kernel");
     return RBK_OK;
@@ -461,14 +505,14 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
     }
     // A head's lanes, and the heads of a step.  Two tokens at a time where that leaves fewer lane steps.
     const int slots = (a->dh + 15) / 16;
-    const int lanes = slots <= 1 ? 1 : slots <= 2 ? 2 : slots <= 4 ? 4 : slots <= 8 ? 8 : 16;
+    const int lanes = slots <= 6 ? slots : slots <= 8 ? 8 : slots <= 10 ? 10 : 16;
     const auto steps_of = [](int heads, int per) { return (heads + per - 1) / per; };
-    const int one = 32 / lanes, two = one / 2;
+    const int one = 32 / lanes, two = 16 / lanes;
     const int T = steps_of(H[0], two) + steps_of(H[1], two) < 2 * (steps_of(H[0], one) + steps_of(H[1], one)) ? 2 : 1;
     const int hps = T == 2 ? two : one;
     // A warp takes all heads of a token where there are tokens for every warp, so that a token's angles are
     // computed once; with fewer tokens its heads are shared out over up to kMaxParts warps.
-    const int most = kPerSm<BWD> * ctx->num_sms;
+    const int most = per_sm(lanes, T, BWD) * ctx->num_sms;
     const int max_blocks = std::min(most, kMaxRows - 2 * kMaxParts / kWarps);
     const bool all = (long long)tokens * 2 >= (long long)max_blocks * kWarps * T;
     long long need[2];
@@ -486,8 +530,12 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
     }
     cudaStream_t st = as_stream(stream);
     long long nb[2] = {need[0], need[1]};
-    if (nb[0] + nb[1] > max_blocks) {                                // in proportion to the heads
-        nb[0] = (long long)max_blocks * a->Hq / ((long long)a->Hq + a->Hk);
+    if (nb[0] + nb[1] > max_blocks) {
+        // In proportion to the work: a token's steps, and half a step for its angles and addresses (by heads alone, 16
+        // query heads beside one key head, 16384 tokens of heads of 128: 54 us, and 31 so).
+        long long cost[2];
+        for (int i = 0; i < 2; ++i) cost[i] = need[i] ? 2 * steps_of(H[i], hps) + 1 : 0;
+        nb[0] = max_blocks * cost[0] / (cost[0] + cost[1]);
         nb[1] = max_blocks - nb[0];
         for (int i = 0; i < 2; ++i)                                  // a warp for each part of a token
             if (need[i]) nb[i] = std::max(nb[i], (long long)(p.side[i].parts + kWarps - 1) / kWarps);

@@ -66,6 +66,15 @@ CASES = [
     (3, 1500, 8, 4, 64, 64, False, "fused", "far"),
     (2, 2000, 5, 5, 128, 128, True, "rows", "seq"),
     (7, 31, 2, 0, 64, 64, False, "rows", "seq"),
+    (3, 401, 3, 3, 80, 80, False, "fused", "far"),
+    (2, 333, 7, 5, 40, 40, True, "planes", "far"),
+    (5, 97, 11, 2, 48, 48, False, "rows", "seq"),
+    (1, 700, 6, 6, 96, 64, False, "rows", "far"),
+    (2, 150, 5, 3, 88, 88, True, "fused", "edge"),
+    (3, 55, 4, 1, 136, 128, False, "planes", "far"),
+    (2, 123, 7, 7, 152, 152, True, "rows", "seq"),
+    (1, 64, 3, 2, 160, 160, False, "fused", "seq"),
+    (4, 37, 8, 8, 104, 96, False, "rows", "far"),
 ]
 
 
