@@ -457,7 +457,7 @@ def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save
     pbd = 0 if bd is None else _here(bd, _F16, "bd", (D,))
     pres, ldr = (0, 0) if residual is None else _rows(residual, "residual", shape)
     if out is None:
-        y = torch.empty(shape, dtype=_F16, device=dev)
+        y = torch.empty_like(x)                             # contiguous, whatever x's row stride
         py, ldy = y.data_ptr(), D
     else:
         y = out
@@ -487,14 +487,20 @@ def gated_ffn_bwd(dy, x, gu, wgu, wd, act="silu", h=None, want_dx=True, dwgu=Non
     pgu = _here(gu, _F16, "gu", (N, 2 * F))
     pwgu, pwd = _here(wgu, _F16, "wgu", (2 * F, D)), _here(wd, _F16, "wd", (D, F))
     recompute = h is None
-    h = torch.empty((N, F), dtype=_F16, device=dev) if recompute else h
-    ph = _here(h, _F16, "h", (N, F))
-    dgu = torch.empty_like(gu) if dgu is None else dgu
-    pdgu = _here(dgu, _F16, "dgu", (N, 2 * F))
+    if recompute:
+        h = torch.empty((N, F), dtype=_F16, device=dev)
+        ph = h.data_ptr()
+    else:
+        ph = _here(h, _F16, "h", (N, F))
+    if dgu is None:
+        dgu = torch.empty_like(gu)
+        pdgu = dgu.data_ptr()
+    else:
+        pdgu = _here(dgu, _F16, "dgu", (N, 2 * F))
     handle = ctx().handle
     dx, pdx, ws, pws, nws = None, 0, None, 0, 0
     if want_dx:
-        dx = torch.empty(shape, dtype=_F16, device=dev)
+        dx = torch.empty_like(dy)
         pdx = dx.data_ptr()
         ws, pws, nws = _ffn_ws(handle, N, D, F, 1, dev)
     p1 = 0 if dwgu is None else _here(dwgu, _F32, "dwgu", (2 * F, D))
