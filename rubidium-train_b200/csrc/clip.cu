@@ -5,15 +5,15 @@
 // Memory bound: the gradients are read for the norm, and where clipping bites (or out is not g) read again
 // and written.  Two launches, ordered by programmatic dependent launch: every block of the first leaves the
 // FP64 sum of its chunks, every block of the second adds those sums in the same order and scales its chunks.
-// 163 M FP32 gradients (652 MB), out of place: 331 us, 100 for the norm (6.5 TB/s) and 230 for the scaling
-// (5.7 TB/s); 48 tensors of 48 KB: 5.4 us.
+// 163 M FP32 gradients (652 MB), out of place: 323 us, of which 303 are its bytes at the rate of a copy; 48 tensors
+// of 48 KB: 5.2 us.
 // The tensors' addresses travel as kernel parameters, so the call copies nothing to the device and can be
 // captured into a graph.
 //
 // A tensor is cut into chunks of 16 KB whose borders lie on 16-byte boundaries of g: whatever g's alignment, all
-// its vectors but the first and the last are whole.  A block has a run of neighbouring chunks, so it looks its
-// tensor up once (the table is in constant memory, a search is a chain of dependent reads); the second kernel
-// goes through the same run backwards, to find in L2 what the first read last.
+// its vectors but the first and the last are whole.  The blocks take the chunks in turn, so that they stream through
+// the same stretch of memory together (each its own run of neighbours: 338 us against 323); a block searches the
+// table for its first chunk's tensor and walks on from there.  The second kernel goes backwards.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -53,13 +53,6 @@ __device__ __forceinline__ int tensor_of(const Table<CAP>& tab, int c) {
         else hi = mid - 1;
     }
     return lo;
-}
-
-// Chunks [a, b) of block `block` of `blocks`: as many as the others, or one more.
-__device__ __forceinline__ void run_of(int chunks, int block, int blocks, int& a, int& b) {
-    const int each = chunks / blocks, more = chunks % blocks;
-    a = block * each + min(block, more);
-    b = a + each + (block < more);
 }
 
 // Sum of squares of one 16-byte vector.  FP32 squares go to FP64 one by one: a square may be beyond FP32's
@@ -132,9 +125,8 @@ template <int CAP>
 __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Table<CAP> tab, double* part) {
     grid_dependency_sync();
     double acc = 0.0;
-    int c, end;
-    run_of(tab.chunks, blockIdx.x, gridDim.x, c, end);
-    for (int k = tensor_of(tab, c); c < end; ++c) {
+    int c = blockIdx.x;
+    for (int k = tensor_of(tab, c); c < tab.chunks; c += gridDim.x) {
         while (k + 1 < tab.count && tab.t[k + 1].first <= c) ++k;
         const Tensor& t = tab.t[k];
         uint4 v[kVec];
@@ -245,9 +237,8 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
     }
     __syncthreads();
     const float coef = coef_s;
-    int begin, c;
-    run_of(tab.chunks, blockIdx.x, gridDim.x, begin, c);
-    for (int k = tensor_of(tab, --c); c >= begin; --c) {
+    int c = tab.chunks - 1 - (int)blockIdx.x;
+    for (int k = c >= 0 ? tensor_of(tab, c) : 0; c >= 0; c -= gridDim.x) {
         while (tab.t[k].first > c) --k;
         const Tensor& t = tab.t[k];
         if (!t.out || (t.out == t.g && coef == 1.0f)) continue;
