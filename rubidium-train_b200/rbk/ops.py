@@ -468,7 +468,8 @@ def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save
         gu = torch.empty((N, 2 * F), dtype=_F16, device=dev)
         pgu = gu.data_ptr()
     handle = ctx().handle
-    ws, pws, nws = _ffn_ws(handle, N, D, F, 0, dev)
+    # few rows need none: the kernels that stream the weights split nothing
+    ws, pws, nws = (None, 0, 0) if N <= 32 else _ffn_ws(handle, N, D, F, 0, dev)
     call("rbk_gated_ffn_fwd", handle, FFN_PACK.pack(N, D, F, _ACTS[act], px, ldx, pwgu, pbgu, pwd, pbd, pres, ldr, py,
                                                     ldy, pgu, h.data_ptr(), pws, nws), _s())
     return y, gu, h

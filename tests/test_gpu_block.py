@@ -165,3 +165,44 @@ def test_block_rows_one_at_a_time(ops):
         assert torch.equal(yq[0, 0], qkv[:H]) and torch.equal(yk[0, 0], qkv[H:2 * H])
         y, _, _ = ops.gated_ffn_fwd(s["h2"][n:n + 1], w["wgu"], w["wd"], residual=s["x1"][n:n + 1], save=False)
         assert rel(y, s["y"][n:n + 1]) < 3 * 2.0 ** -11
+
+
+def test_threads_with_their_own_streams(ops):
+    """Four host threads, each with its own context and stream, run the operators at once: every one gets the bits of a
+    run by itself."""
+    import threading
+    w, x, _ = weights(3)
+    s = forward(ops, w, x)
+    q, k = s["qk"][:, :, :H], s["qk"][:, :, H:]
+    dyq, dyk = (torch.randn(B, S, H, DH, device="cuda").half() for _ in range(2))
+    grads = [torch.randn(n, device="cuda") for n in (100003, 7, 40000)]
+
+    def run():
+        out = [*ops.qk_norm_rope_fwd(q, k, w["gq"], w["gk"]), *ops.qk_norm_rope_bwd(dyq, dyk, q, k, w["gq"], w["gk"])]
+        for n in (3, N):
+            out += ops.gated_ffn_fwd(s["h2"][:n], w["wgu"], w["wd"], residual=s["x1"][:n])
+        out += ops.gated_ffn_bwd(x, s["h2"], s["gu"], w["wgu"], w["wd"])
+        clipped = [torch.empty_like(g) for g in grads]
+        return out + [ops.clip_grad_norm(grads, 1.0, out=clipped)] + clipped
+
+    want = run()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = run()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(i)
+        except Exception as e:                             # a thread's exception is not pytest's
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

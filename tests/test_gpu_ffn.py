@@ -154,6 +154,22 @@ def test_strides_and_what_lies_beside(ops, N):
     assert all(torch.equal(s, t) for s, t in zip(a, b))
 
 
+@pytest.mark.parametrize("N", [1, 31, 47, 65, 255, 257])
+def test_rows_behind_the_last_stay(ops, N):
+    """y, and through the C entry gu and h, in larger buffers: the rows from N on stay as they were."""
+    import ctypes as C
+
+    from rbk._lib import FFN_PACK, call
+    D, F = 136, 264
+    c = case(N, D, F, seed=8)
+    bufs = [torch.full((N + 300, k), 9.0, device="cuda").half() for k in (D, 2 * F, F)]
+    args = FFN_PACK.pack(N, D, F, 0, c["x"].data_ptr(), D, c["wgu"].data_ptr(), 0, c["wd"].data_ptr(), 0, 0, 0,
+                         bufs[0].data_ptr(), D, bufs[1].data_ptr(), bufs[2].data_ptr(), 0, 0)
+    call("rbk_gated_ffn_fwd", ops.ctx().handle, args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    for got, want in zip(bufs, ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"])):
+        assert torch.equal(got[:N], want) and bool((got[N:] == 9.0).all())
+
+
 @pytest.mark.parametrize("N", [6, 70])
 def test_a_row_that_is_not_finite_spoils_itself_only(ops, N):
     D, F = 64, 136
@@ -186,6 +202,13 @@ def test_extreme_gates(ops):
         d = 2.0 ** -6
         assert bool((dgu[:, :F // 2] == d * 0.5).all()) and bool((dgu[:, F // 2:F] == 0).all())
         assert bool((dgu[:, F:F + F // 2] == d * 60000).all()) and bool((dgu[:, F + F // 2:] == 0).all())
+
+
+def test_few_rows_need_no_workspace(ops):
+    from rbk._lib import lib
+    for N in (1, 8, 32):
+        for D, F in ((8, 8), (264, 8192), (2048, 5632), (8192, 8192)):
+            assert lib().rbk_gated_ffn_ws_bytes(ops.ctx().handle, N, D, F, 0) == 0
 
 
 def test_no_rows(ops):
