@@ -22,7 +22,7 @@ namespace ffn {
 // that use them takes elements 4 m .. 4 m + 3.
 // A lane copies its vectors of the next DEPTH - 1 rounds, across tiles, into slots of its own with cp.async and
 // waits for its own copies only: the weights stream without registers or barriers.  Bound by HBM where the weights
-// are large (1 row, D 2048, F 5632: 15.1 us for both kernels, 69 MB, 4580 GB/s with two ramps; plain loads in
+// are large (1 row, D 2048, F 5632: 14.6 us for both kernels, 69 MB, 4740 GB/s with two ramps; plain loads in
 // the loop took 22.4), by latency where they are not (D 768, F 2048: 5.0 us), and from 16 rows on also by x, which
 // every tile reads from L2 (32 rows: 26.7 us).
 
@@ -31,20 +31,21 @@ namespace ffn {
 // against 17; D 768, F 2048: 12 against 18; D 1024, F 2816: 20 against 21; D 2048, F 5632: 44 against 33.
 static bool few(int N, int D, int F) { return N <= 32 || (N <= 64 && (int64_t)D * F <= (3 << 20)); }
 
-// WIDE: at most one tile per SM, so a CTA has all of its shared memory for what is in flight; else up to three
-// CTAs share an SM, and a tile is 32 weight rows where x, which comes from L2 for each, is more than the weights
-// (16 rows n, D 1888, F 4312: 21.5 us with 16 weight rows, 16.6 with 32).
+// WIDE: at most one tile per SM, so a CTA has all of its shared memory for what is in flight; else two CTAs share
+// an SM (1 row, D 4096, F 11264: 48.1 us; three of four warps with deeper slots 52.8), and a tile is 32 weight
+// rows where x, which comes from L2 for each, is more than the weights (16 rows n, D 1888, F 4312: 21.5 us with 16
+// weight rows, 16.6 with 32).
 template <int NT, bool WIDE>
 struct Few {
     static constexpr int MT = NT > 1 && !WIDE ? 2 : 1;
-    static constexpr int WARPS = WIDE ? 8 : 4, THREADS = 32 * WARPS;
-    static constexpr int DEPTH = WIDE ? (NT == 1 ? 8 : NT == 2 ? 6 : NT == 4 ? 4 : 2) : (NT == 1 ? 6 : NT == 2 ? 4 : 3);
+    static constexpr int WARPS = WIDE || NT == 1 ? 8 : 4, THREADS = 32 * WARPS;
+    static constexpr int DEPTH = WIDE ? (NT == 1 ? 8 : NT == 2 ? 6 : NT == 4 ? 4 : 2) : NT == 2 ? 4 : 3;
     static constexpr int VECS = 4 * MT + 2 * NT;         // 16-byte vectors of a lane and round
     static constexpr int ROUND = VECS * 512;
     static constexpr int RING = WARPS * DEPTH * ROUND;
     static constexpr int SUMS = WARPS * MT * 16 * (8 * NT + 1) * 4;
     static constexpr int SMEM = RING + SUMS;
-    static constexpr int PER_SM = WIDE || NT == 8 ? 1 : NT == 1 ? 3 : 2;
+    static constexpr int PER_SM = WIDE || NT == 8 ? 1 : 2;
     static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory of an SM");
 };
 
