@@ -344,7 +344,7 @@ enum { RBK_ACT_SILU = 0, RBK_ACT_GELU = 1 /* the tanh form */ };
  * the weights is the cost, both are kernels that stream them.  h is rounded to half
  * once. */
 typedef struct rbk_ffn_args {
-    int N, D, F;             /* N >= 0 rows                                      */
+    int N, D, F;             /* N rows, 0 <= N <= 2^30; D, F <= 2^29             */
     int act;                 /* RBK_ACT_*                                        */
     const void* x; int ldx;  /* [N, D]                                           */
     const void* wgu;         /* [2F, D]: the rows of Wg, then those of Wu        */
@@ -452,7 +452,7 @@ typedef struct rbk_heads {
  * position 2^31 - 1 as at 1.
  *   dh a multiple of 8, 8 <= dh <= 256; rot a multiple of 16 (8 when
  *   interleaved), 0 <= rot <= dh; B, S >= 0; 0 <= Hq, Hk <= 2^20 (Hk = 0: queries
- *   only); strides below 2^34.
+ *   only); strides below 2^34; pos0 + S - 1 at most 2^31 - 1.
  * No counterpart in the reference, whose positions are learned embeddings. */
 typedef struct rbk_qk_args {
     int B, S, Hq, Hk, dh;

@@ -255,8 +255,9 @@ int few_rows(rbk_ctx* ctx, const Params& p, cudaStream_t st) {
 
 static int check_sizes(const char* who, int N, int D, int F, int act) {
     RBK_REQUIRE(N >= 0, "%s: negative N", who);
-    RBK_REQUIRE(D > 0 && F > 0 && D % 8 == 0 && F % 8 == 0 && F <= (1 << 29),
-                "%s: D and F must be positive multiples of 8 (D=%d F=%d)", who, D, F);
+    RBK_REQUIRE(N <= (1 << 30), "%s: more than 2^30 rows", who);         // rounded up to tiles they stay an int
+    RBK_REQUIRE(D > 0 && F > 0 && D % 8 == 0 && F % 8 == 0 && D <= (1 << 29) && F <= (1 << 29),
+                "%s: D and F must be positive multiples of 8, at most 2^29 (D=%d F=%d)", who, D, F);
     RBK_REQUIRE(act == RBK_ACT_SILU || act == RBK_ACT_GELU, "%s: act must be RBK_ACT_SILU or RBK_ACT_GELU", who);
     return RBK_OK;
 }

@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(G, T, BWD)) qk_kernel(const _
     };
     auto pos_of = [&](int tk) {
         tk = min(tk + sub, p.tokens - 1);
-        return p.pos ? p.pos[tk] : p.pos0 + tk - row_of(tk) * p.S;
+        return p.pos ? p.pos[tk] : p.pos0 + (tk - row_of(tk) * p.S);
     };
     // whether this lane has head hd of token tk (+ sub)
     auto has = [&](int tk, int hd) { return hd < sd.H && (T == 1 || tk + sub < p.tokens) && (POW2 || g < HPS); };
@@ -458,6 +458,7 @@ int entry(rbk_ctx* ctx, const rbk_qk_args* a, void* stream) {
     RBK_REQUIRE(a->eps >= FLT_MIN && std::isfinite(a->eps), "%s: eps must be positive and normal", who);
     RBK_REQUIRE(a->inv_freq || a->rot == 0 || (a->theta > 0.0 && std::isfinite(a->theta)),
                 "%s: theta must be positive", who);
+    RBK_REQUIRE(a->positions || a->pos0 <= 0x7fffffffLL - std::max(a->S - 1, 0), "%s: positions beyond 2^31 - 1", who);
     RBK_REQUIRE((!a->gq || aligned16(a->gq)) && (!a->gk || aligned16(a->gk)), "%s: gains must be 16-byte aligned", who);
     const int H[2] = {a->Hq, a->Hk};
     const rbk_heads* x[2] = {&a->q, &a->k};

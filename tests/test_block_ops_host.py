@@ -43,11 +43,14 @@ def test_qk_refusals(name):
         (dict(theta=float("inf")), "theta"), (dict(gq=P + 2), "gains"), (dict(gk=P + 8), "gains"),
         (dict(q=Heads(None, 1024, 256, 64)), "q is NULL"), (dict(k=Heads(P + 2, 1024, 256, 64)), "k must be 16-byte"),
         (dict(q=Heads(P, 1024, 252, 64)), "strides of q"), (dict(ok=Heads(P, 1024, 256, 63)), "strides of ok"),
+        (dict(pos0=2 ** 31 - 3), "2^31 - 1"),
         (dict(oq=Heads(P, 1024, 256, 0)), "zero stride"), (dict(oq=Heads(P, 0, 256, 64)), "zero stride"),
     ]:
         refused(name, qk(**kw), match)
     freq = (C.c_double * 32)(*([0.5] * 31 + [float("inf")]))
     refused(name, qk(inv_freq=C.cast(freq, C.c_void_p)), "inv_freq[31]")
+    refused(name, qk(pos0=2 ** 31 - 4), "ctx is NULL")       # positions up to 2^31 - 1
+    refused(name, qk(pos0=-2 ** 31), "ctx is NULL")
     refused(name, qk(), "ctx is NULL")                       # nothing else is wrong with these arguments
     refused(name, qk(Hk=0, k=Heads(), ok=Heads(), dyk=Heads()), "ctx is NULL")
 
@@ -94,6 +97,7 @@ def test_ffn_fwd_refusals():
     n = "rbk_gated_ffn_fwd"
     for kw, match in [
         (dict(N=-1), "negative"), (dict(D=0), "multiples of 8"), (dict(D=60), "multiples of 8"),
+        (dict(N=2 ** 30 + 1), "2^30 rows"), (dict(D=2 ** 29 + 8, ldx=2 ** 29 + 8), "2^29"), (dict(F=2 ** 29 + 8), "2^29"),
         (dict(F=-8), "multiples of 8"), (dict(F=12), "multiples of 8"), (dict(act=2), "act"), (dict(act=-1), "act"),
         (dict(x=None), "x is NULL"), (dict(wgu=None), "wgu is NULL"), (dict(wd=None), "wd is NULL"),
         (dict(y=None), "y is NULL"), (dict(h=None), "h is NULL"), (dict(x=P + 2), "x must be 16-byte"),

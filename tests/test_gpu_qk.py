@@ -132,6 +132,19 @@ def test_no_gain_own_frequencies_and_accumulation(ops):
     assert torch.equal(a, dgq + nq) and torch.equal(b, dgk + nk)
 
 
+def test_the_last_positions(ops):
+    """Batched rows that end at position 2^31 - 1, counted from pos0, give the bits of the same positions listed."""
+    B, S, H, dh = 33, 3, 2, 64
+    q, k, gq, gk, dyq, dyk, _ = case(B, S, H, H, dh, dh, False, "rows", "seq", 4)
+    pos0 = 2 ** 31 - S
+    positions = (pos0 + torch.arange(S)).to(torch.int32).cuda().expand(B, S).contiguous()
+    for a, b in zip(ops.qk_norm_rope_fwd(q, k, gq, gk, pos0=pos0),
+                    ops.qk_norm_rope_fwd(q, k, gq, gk, positions=positions)):
+        assert torch.equal(a, b)
+    with pytest.raises(Exception, match="positions beyond"):
+        ops.qk_norm_rope_fwd(q, k, gq, gk, pos0=pos0 + 1)
+
+
 def test_one_gain_for_queries_and_keys(ops):
     B, S, dh = 2, 90, 64
     q, k, g, _, dyq, dyk, _ = case(B, S, 6, 2, dh, dh, False, "rows", "seq", 9)
