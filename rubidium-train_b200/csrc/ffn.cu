@@ -271,7 +271,8 @@ static int check_ptr(const char* who, const char* what, const void* p, bool opti
 }
 
 // The FP32 planes of the down projection (backward: of dx), if the call splits it.
-static int64_t plane_bytes(rbk_ctx* ctx, int M, int N, int K) {
+static int64_t plane_bytes(rbk_ctx* ctx, int M, int N, int K, int b_mn) {
+    if (mid_store_serves(ctx, M, N, K, b_mn)) return 0;
     const int s = gemm_store_splits(ctx, M, N, K);
     return s > 1 ? (int64_t)s * M * N * 4 : 0;
 }
@@ -293,7 +294,7 @@ int64_t rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int backward) 
     RBK_TRY(ffn::check_sizes(who, N, D, F, RBK_ACT_SILU));
     RBK_REQUIRE(ctx, "%s: ctx is NULL", who);
     if (N == 0 || (!backward && ffn::few(N, D, F))) return 0;
-    return ffn::plane_bytes(ctx, N, D, backward ? 2 * F : F);
+    return ffn::plane_bytes(ctx, N, D, backward ? 2 * F : F, backward != 0);
 }
 
 int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
@@ -338,10 +339,10 @@ int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
         return ffn::few_rows<false>(ctx, d, st);
     }
     void* ws = a->ws;
-    const int64_t need = ffn::plane_bytes(ctx, a->N, a->D, a->F);
+    const int64_t need = ffn::plane_bytes(ctx, a->N, a->D, a->F, 0);
     RBK_TRY(ffn::check_ws(who, ws, a->ws_bytes, need));
     if (!ws && need) RBK_TRY(ctx_scratch(ctx, need, &ws));
-    RBK_TRY(glu_fwd_tiles(ctx, a->h, a->gu, a->x, a->ldx, a->wgu, a->bgu, a->N, a->D, a->F, a->act, st));
+    RBK_TRY(mid_glu_fwd(ctx, a->h, a->gu, a->x, a->ldx, a->wgu, a->bgu, a->N, a->D, a->F, a->act, st));
     rbk_gemm_desc d = {};
     d.M = a->N; d.N = a->D; d.K = a->F;
     d.A = a->h; d.lda = a->F;
@@ -351,7 +352,8 @@ int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {
     d.bias = a->bd;
     d.aux = a->residual; d.ld_aux = a->residual ? a->ldr : 0;
     d.alpha = 1.0f;
-    return gemm_store(ctx, &d, (float*)ws, st);
+    // wd is as it will be: the kernel before, of this call, began after all before it had ended and writes none of it
+    return mid_store(ctx, &d, (float*)ws, 1, st);
 }
 
 int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* a, void* stream) {
@@ -375,10 +377,10 @@ int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* a, void* stream) {
     }
     RBK_TRY(check_device(ctx, who));
     if (!a->N) return RBK_OK;
-    const int64_t need = a->dx ? ffn::plane_bytes(ctx, a->N, a->D, 2 * a->F) : 0;
+    const int64_t need = a->dx ? ffn::plane_bytes(ctx, a->N, a->D, 2 * a->F, 1) : 0;
     RBK_TRY(ffn::check_ws(who, a->ws, a->ws_bytes, need));
     cudaStream_t st = as_stream(stream);
-    RBK_TRY(glu_bwd_tiles(ctx, a->dgu, a->recompute_h ? a->h : nullptr, a->dy, a->lddy, a->wd, a->gu, a->N, a->D, a->F,
+    RBK_TRY(mid_glu_bwd(ctx, a->dgu, a->recompute_h ? a->h : nullptr, a->dy, a->lddy, a->wd, a->gu, a->N, a->D, a->F,
                           a->act, st));
     // the weight gradients before dx, which may then lie over dy or x
     rbk_gemm_desc d = {};
@@ -412,7 +414,7 @@ int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* a, void* stream) {
     e.C = a->dx; e.ldc = a->lddx;
     e.epilogue = RBK_EPI_STORE_F16;
     e.alpha = 1.0f;
-    return gemm_store(ctx, &e, (float*)ws, st);
+    return mid_store(ctx, &e, (float*)ws, !a->dwgu && !a->dwd, st);
 }
 
 }  // extern "C"

@@ -90,7 +90,7 @@ def test_dx_over_what_is_read_and_the_scratch_of_the_context(ops, over, ws):
     import ctypes as C
 
     from rbk._lib import FFN_BWD_PACK, call, lib
-    N, D, F = 600, 264, 1032
+    N, D, F = 600, 264, 3208
     c = case(N, D, F, seed=6)
     gu = (c["x"].float() @ c["wgu"].float().T).half()
     want = {k: torch.zeros(s, device="cuda") for k, s in (("dwgu", (2 * F, D)), ("dwd", (D, F)))}
@@ -117,7 +117,7 @@ def test_dx_over_what_is_read_and_the_scratch_of_the_context(ops, over, ws):
 
 def test_a_workspace_that_is_too_small_is_refused(ops):
     from rbk._lib import FFN_BWD_PACK, FFN_PACK, lib
-    N, D, F = 100, 264, 2056
+    N, D, F = 600, 264, 8712
     c = case(N, D, F, seed=7)
     gu, dgu, dx = (torch.zeros(N, k, device="cuda").half() for k in (2 * F, 2 * F, D))
     y, h, ws = torch.zeros_like(c["x"]), torch.zeros(N, F, device="cuda").half(), torch.zeros(256, device="cuda")
