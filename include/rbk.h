@@ -340,9 +340,9 @@ enum { RBK_ACT_SILU = 0, RBK_ACT_GELU = 1 /* the tanh form */ };
  * 8, every pointer 16-byte aligned, row strides (elements) multiples of 8.
  * The two projections, the activation and the product are one kernel (tcgen05
  * tiles that hold the gate's and the up projection's columns side by side), the
- * down projection is the second; up to 32 rows (64 of a narrow block), where reading
- * the weights is the cost, both are kernels that stream them.  h is rounded to half
- * once. */
+ * down projection is the second, on tiles fitted to the machine where there are few;
+ * up to 32 rows (64 of a narrow block), where reading the weights is the cost, both
+ * are kernels that stream them.  h is rounded to half once. */
 typedef struct rbk_ffn_args {
     int N, D, F;             /* N rows, 0 <= N <= 2^30; D, F <= 2^29             */
     int act;                 /* RBK_ACT_*                                        */

@@ -6,7 +6,10 @@
 // Many rows: tensor bound (6 N D F FLOP each way).  The CTA-pair GEMM of gemm.cu with epilogues of its own
 // makes h (gate and up tiles share one accumulator) and dgu; the other products are plain GEMMs.  8192 rows,
 // D 2048, F 5632: forward 430 to 490 us (the power limit moves it), backward without weight gradients 510 to 535.
+// Where those tiles are too few for the machine, smaller ones (ffn_mid.cu).
 // Few rows: the weights, 6 D F bytes, are read once and that is the cost.  The kernels below stream them.
+#include <algorithm>
+
 #include "tc.cuh"
 
 namespace rbk {
@@ -26,10 +29,13 @@ namespace ffn {
 // the loop took 22.4), by latency where they are not (D 768, F 2048: 5.0 us), and from 16 rows on also by x, which
 // every tile reads from L2 (32 rows: 26.7 us).
 
-// Which calls they serve: up to 32 rows, and up to 64 of a block whose weights are few, where the tiles' fixed
-// cost is most of their time.  Measured at 33 to 64 rows, these kernels against the tiles: D 512, F 1024: 8 us
-// against 17; D 768, F 2048: 12 against 18; D 1024, F 2816: 20 against 21; D 2048, F 5632: 44 against 33.
-static bool few(int N, int D, int F) { return N <= 32 || (N <= 64 && (int64_t)D * F <= (3 << 20)); }
+// Which calls they serve: up to 32 rows, and up to 64 of a narrow block, where the launches and waits of the tiles are
+// most of their time.  Measured at 48 rows, these kernels against the tiles: D 512, F 1024: 7.5 us against 9.8;
+// D 768, F 2048: 12.6 against 12.9; D 1024, F 2816: 21 against 16.5; D 256, F 5632: 22 against 15.  At 32 rows:
+// D 1024, F 2816: 12.3 against 15.7; D 2048, F 5632: 27 both.
+static bool few(int N, int D, int F) {
+    return N <= 32 || (N <= 64 && std::max(D, F) <= 2048 && (int64_t)D * F <= (3 << 19));
+}
 
 // WIDE: at most one tile per SM, so a CTA has all of its shared memory for what is in flight; else two CTAs share
 // an SM (1 row, D 4096, F 11264: 48.1 us; three of four warps with deeper slots 52.8), and a tile is 32 weight

@@ -15,12 +15,13 @@ namespace mid {
 
 using namespace tc;
 
+constexpr int kLong = 16;                                    // k blocks of a CTA from which on it is better off alone
 constexpr int BM = 128, BK = 64, kThreads = 320;             // a TMA warp, an MMA warp, eight that read TMEM
 constexpr int kHead = 1024;                                  // barriers
 // Shared memory of which two CTAs fit an SM (228 KB, 1 KB of each for the system), the least that one takes: a CTA
 // holds up to 256 columns of TMEM while it waits for the others of its cluster, so that no SM may take more CTAs than
 // its 512 columns serve, this kernel's or the CTA pairs' (512 columns, at least 193 KB) of another stream.
-constexpr int kHalfSm = 113 << 10;
+constexpr int kHalfSm = 113 << 10, kAllSm = 227 << 10;
 enum { kGlu = 0, kGluBwd = 1, kStore = 2 };
 
 struct Params {
@@ -259,7 +260,7 @@ int launch_s(rbk_ctx* ctx, const CUtensorMap& ta, const CUtensorMap& tb, const P
              cudaStream_t st) {
     static int configured_device = -1;   // attribute is per device; one device per process
     if (configured_device != ctx->device) {
-        RBK_CUDA(cudaFuncSetAttribute(mid_kernel<EPI, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+        RBK_CUDA(cudaFuncSetAttribute(mid_kernel<EPI, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAllSm));
         configured_device = ctx->device;
     }
     cudaLaunchConfig_t cfg = {};
@@ -292,13 +293,15 @@ int launch(rbk_ctx* ctx, int S, const CUtensorMap& ta, const CUtensorMap& tb, co
 
 // The tiles of a call, or bn 0: those of gemm.cu.  Two CTAs fit an SM; what is wanted is one round of them with the
 // widest spread, and of K parts that are still worth a cluster's exchange.  Measured, whole calls, forward:
-//   D 768, F 2048: 128 rows 21.1 -> 14.1 us, 512 rows 21.9 -> 17.9; 1024 rows 24.0 -> 21.0
-//   D 2048, F 5632: 128 rows 35.3 -> 29.1, 384 rows 49.2 -> 39.7; 640 rows stay (51.6; tiles of 192 columns 74)
-//   D 512, F 1024: 100 rows 17.6 -> 10.9, 1024 rows 18.1 -> 14.2
+//   D 768, F 2048: 100 rows 20.9 -> 13.8 us, 384 rows 21.7 -> 17.8; 1024 rows 23.8 -> 20.8
+//   D 2048, F 5632: 100 rows 34.8 -> 28.2, 384 rows 48.9 -> 38.7; 640 rows stay (50.9; tiles of 192 columns 74)
+//   D 512, F 1024: 100 rows 17.6 -> 10.9, 1024 rows 18.4 -> 14.1
 // backward (dgu, h, dx):
-//   D 768, F 2048: 128 rows 25.4 -> 17.0; 1024 rows 30.4 -> 27.1
-//   D 2048, F 5632: 100 rows 40.2 -> 32.6, 384 rows 48.6 -> 45.6; 512 rows stay (49.9; 53.3 with 64 columns)
-//   D 512, F 1024: 512 rows 22.6 -> 14.5
+//   D 768, F 2048: 100 rows 25.1 -> 15.7; 1024 rows 30.2 -> 27.0
+//   D 2048, F 5632: 100 rows 40.3 -> 32.5, 384 rows 48.2 -> 45.0; 512 rows stay (49.9; 53.3 with 64 columns)
+//   D 512, F 1024: 384 rows 22.8 -> 17.7
+// Over 96 shapes (33 to 2048 rows, D 256 to 2048, F 256 to 5632) the forward took 0.80 of its time and the backward
+// 0.76 (geometric means), the worst 1.07 (353 rows, D 760, F 3832: 27.6 us, 25.8 on the larger tiles).
 struct Plan {
     int bn, S;
 };
@@ -308,7 +311,7 @@ static Plan plan(rbk_ctx* ctx, int epi, int M, int N, int K, int b_mn) {
     const auto ctas = [&](long long cols, int bn) { return m * ((cols + bn - 1) / bn); };
     // Clusters of four do not fill the machine: 288 CTAs of them are two rounds (dx of 768 rows, D 768,
     // F 2048: 36 us and 29 with the tiles of gemm.cu), 264 are one.
-    const auto fit = [&](long long cols, int least, int most, int S) {       // the narrowest tiles that are one round
+    const auto fit = [&](long long cols, int least, int most, int S, long long slots) {   // the narrowest one-round tiles
         for (int bn = least; bn <= most; bn += 16)
             if (ctas(cols, bn) * S <= (S >= 4 ? slots * 9 / 10 : slots)) return bn;
         return 0;
@@ -327,7 +330,9 @@ static Plan plan(rbk_ctx* ctx, int epi, int M, int N, int K, int b_mn) {
     const long long m2 = (M + 2 * BM - 1) / (2 * BM);
     Plan p = {0, 1};
     if (epi == kGlu) {
-        p.bn = fit(2LL * N, kb >= 24 ? 64 : 48, 160, 1);
+        // long in K: one CTA for an SM, or two (286 rows, D 1192, F 2040, whole call: 23.7 us so, 28.1 with two)
+        if (kb >= kLong) p.bn = fit(2LL * N, 48, 256, 1, slots / 2);
+        if (!p.bn) p.bn = fit(2LL * N, kb >= 24 ? 64 : 48, 160, 1, slots);
         if (p.bn && here(p.bn, 1, ctas(2LL * N, p.bn)) > there(m2 * ((N + 127) / 128), 1)) p.bn = 0;
     } else if (epi == kGluBwd) {
         // tiles of 192 columns fill an SM alone
@@ -337,7 +342,7 @@ static Plan plan(rbk_ctx* ctx, int epi, int M, int N, int K, int b_mn) {
     } else if (!b_mn) {
         p.S = m <= 2 || kb > 48 ? 4 : 2;
         while (p.S < 8 && kb >= 32 * p.S && ctas(N, 32) * 2 * p.S <= (m <= 2 ? slots / 2 : slots)) p.S *= 2;
-        if (m <= 2 || kb <= 32 * p.S) p.bn = fit(N, m <= 2 ? 32 : 48, 80, p.S);
+        if (m <= 2 || kb <= 32 * p.S) p.bn = fit(N, m <= 2 ? 32 : 48, 80, p.S, slots);
         if (p.bn && here(p.bn, p.S, ctas(N, p.bn) * p.S) > there(m2 * ((N + 255) / 256), gemm_store_splits(ctx, M, N, K))) p.bn = 0;
     } else {
         // dx: K is twice F, and its rows of B come 64 columns at a time
@@ -361,11 +366,15 @@ int run(rbk_ctx* ctx, Params p, const Plan& pl, const void* A, int64_t lda, cons
     p.k_blocks = (p.K + BK - 1) / BK;
     p.kb_per = (p.k_blocks + pl.S - 1) / pl.S;
     p.rows_box = std::min(BM, (p.M + 7) / 8 * 8);
-    const int stage = BM * BK * 2 + p.bn * BK * 2;
-    p.stages = std::min({8, p.kb_per, std::max(3, (kHalfSm - 1024 - kHead) / stage)});
-    p.err = ctx->tickets + kGemmError;
     const int per = EPI == kGlu ? p.bn / 2 : p.bn;
     const int tiles = p.m_blocks * ((p.N + per - 1) / per);
+    const int stage = BM * BK * 2 + p.bn * BK * 2;
+    // At most one CTA for an SM, and long in K: all of its shared memory for what is in flight (629 rows, D 1736, F 864:
+    // forward 27.4 -> 21.6 us; 131 rows, D 1448, F 992 23.4 -> 18.8).  Short ones are better off beside the next
+    // kernel's (100 rows, D 768, F 2048: 13.8, and 14.9 alone).
+    const bool alone = p.kb_per >= kLong && tiles * pl.S <= (pl.S >= 4 ? ctx->num_sms * 9 / 10 : ctx->num_sms);
+    p.stages = std::min({8, p.kb_per, std::max(3, ((alone ? kAllSm : kHalfSm) - 1024 - kHead) / stage)});
+    p.err = ctx->tickets + kGemmError;
     const int smem = std::max(kHalfSm, 1024 + kHead + std::max(p.stages * stage, p.rows_box * (p.bn + 4) * 4));
     CUtensorMap ta, tb;
     RBK_TRY(make_tmap(&ta, A, p.K, p.M, lda, 64, p.rows_box));

@@ -70,6 +70,54 @@ def test_backward(ops, N, D, F, act):
     assert ops.device_error() == 0
 
 
+# Between few rows and full tiles: rows in one to sixteen blocks of 128, K in one to eight parts, rows of K that start
+# on 128 bytes and not, narrow and wide blocks.
+MIDDLE = [(34, 8, 8), (66, 768, 2048), (127, 264, 5640), (128, 512, 1024), (129, 1144, 3872), (131, 1448, 992),
+          (200, 1024, 2816), (257, 2048, 264), (286, 1192, 2040), (384, 768, 2048), (440, 672, 2088), (513, 400, 3344),
+          (630, 1736, 864), (899, 600, 408), (1025, 512, 1024), (1121, 2008, 336), (2047, 72, 264)]
+
+
+@pytest.mark.parametrize("N,D,F", MIDDLE)
+def test_middle_sizes(ops, N, D, F):
+    """Against float64; the same bits from a second call, and from dx with and without weight gradients before it."""
+    act = "gelu" if N % 2 else "silu"
+    c = case(N, D, F, N % 3 == 0, N % 4 < 2, seed=11)
+    how = dict(bgu=c["bgu"], bd=c["bd"], residual=c["residual"], act=act)
+    want = ref.fwd(c["x"], c["wgu"], c["wd"], c["bgu"], c["bd"], c["residual"], act)
+    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], **how)
+    for name, t in (("gu", gu), ("h", h), ("y", y)):
+        within(name, t, *want[name])
+    again = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], **how)
+    assert all(torch.equal(s, t) for s, t in zip(again, (y, gu, h)))
+    want = ref.bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], act)
+    dx, dgu, h = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], act=act)
+    for name, t in dict(dx=dx, dgu=dgu, h=h).items():
+        within(name, t, *want[name])
+    dwd = torch.zeros(D, F, device="cuda")
+    dx2, dgu2, h2 = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], act=act, dwd=dwd)
+    assert torch.equal(dx2, dx) and torch.equal(dgu2, dgu) and torch.equal(h2, h)
+    within("dwd", dwd, *want["dwd"])
+    assert ops.device_error() == 0
+
+
+def test_middle_sizes_on_two_streams(ops):
+    """Calls on two streams at once, whose clusters share the SMs, give what each gives alone."""
+    cases = [case(N, D, F, seed=12) for N, D, F in ((300, 768, 2048), (129, 1144, 1000))]
+    want = [ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"]) for c in cases]
+    back = [ops.gated_ffn_bwd(c["dy"], c["x"], w[1], c["wgu"], c["wd"]) for c, w in zip(cases, want)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for c, w, st in zip(cases, want, streams):
+            with torch.cuda.stream(st):
+                got.append((ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"]),
+                            ops.gated_ffn_bwd(c["dy"], c["x"], w[1], c["wgu"], c["wd"])))
+    torch.cuda.synchronize()
+    for i, (f, b) in enumerate(got):
+        assert all(torch.equal(s, t) for s, t in zip(f + b, want[i % 2] + back[i % 2]))
+
+
 def test_backward_accumulates_and_reads_the_kept_product(ops):
     N, D, F = 200, 128, 264
     c = case(N, D, F, seed=2)
