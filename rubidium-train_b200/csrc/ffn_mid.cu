@@ -18,7 +18,7 @@ namespace mid {
 
 using namespace tc;
 
-constexpr int kLong = 16;                                    // k blocks of a CTA from which on it is better off alone
+constexpr int kLong = 17;                                    // k blocks of a CTA from which on it is better off alone
 constexpr int BM = 128, BK = 64, kThreads = 320;             // a TMA warp, an MMA warp, eight that read TMEM
 constexpr int kHead = 1024;                                  // barriers
 // Shared memory of which two CTAs fit an SM (228 KB, 1 KB of each for the system), the least that one takes: a CTA
@@ -148,13 +148,17 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
             for (int i = 0; i < first; ++i) load_a(i, kb0 + i);
             int s = 0;
             uint32_t phase = 0;
-            for (int i = first; i < nk; ++i) {
+            int i = first;
+            for (; i < nk; ++i) {
                 if (!mbar_wait(empty_bar(s), phase, abort_flag)) break;
                 mbar_expect_tx(full_bar(s), tx);
                 load_b(s, kb0 + i);
                 load_a(s, kb0 + i);
                 if (++s == p.stages) { s = 0; phase ^= 1; }
             }
+            if (*abort_flag)                                 // the copies under way land before the CTA ends, or 4 ms pass
+                for (int n = max(0, i - p.stages); n < i; ++n)
+                    for (int t = 0; t < 200 && !mbar_try_suspend(full_bar(n % p.stages), n / p.stages & 1, 20000u); ++t) {}
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
     __syncwarp();
     if (warp >= 2) {
         // the tile's sums to shared memory, over the operands' slots: all MMAs have read them
-        if (mbar_wait(done_bar, 0, abort_flag)) {
+        if (__all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag) && !*abort_flag)) {
             fence_after();
             const int q = warp & 3, row = q * 32 + lane;
             if (q * 32 < rows) {
@@ -296,14 +300,14 @@ int launch(rbk_ctx* ctx, int S, const CUtensorMap& ta, const CUtensorMap& tb, co
 
 // The tiles of a call, or bn 0: those of gemm.cu.  Two CTAs fit an SM; what is wanted is one round of them with the
 // widest spread, and of K parts that are still worth a cluster's exchange.  Measured, whole calls, forward:
-//   D 768, F 2048: 100 rows 20.9 -> 13.8 us, 384 rows 21.7 -> 17.8; 1024 rows 23.8 -> 20.8
+//   D 768, F 2048: 100 rows 20.9 -> 13.8 us, 384 rows 21.6 -> 18.7; 1024 rows 23.8 -> 20.8
 //   D 2048, F 5632: 100 rows 34.8 -> 28.2, 384 rows 48.9 -> 38.7; 640 rows stay (50.9; tiles of 192 columns 74)
 //   D 512, F 1024: 100 rows 17.6 -> 10.9, 1024 rows 18.4 -> 14.1
 // backward (dgu, h, dx):
 //   D 768, F 2048: 100 rows 25.1 -> 15.7; 1024 rows 30.2 -> 27.0
 //   D 2048, F 5632: 100 rows 40.3 -> 32.5, 384 rows 48.2 -> 45.0; 512 rows stay (49.9; 53.3 with 64 columns)
 //   D 512, F 1024: 384 rows 22.8 -> 17.7
-// Over 96 shapes (33 to 2048 rows, D 256 to 2048, F 256 to 5632) the forward took 0.80 of its time and the backward
+// Over 96 shapes (33 to 2048 rows, D 256 to 2048, F 256 to 5632) the forward took 0.79 of its time and the backward
 // 0.76 (geometric means), the worst 1.07 (353 rows, D 760, F 3832: 27.6 us, 25.8 on the larger tiles).
 struct Plan {
     int bn, S;
@@ -374,8 +378,10 @@ int run(rbk_ctx* ctx, Params p, const Plan& pl, const void* A, int64_t lda, cons
     const int stage = BM * BK * 2 + p.bn * BK * 2;
     // At most one CTA for an SM, and long in K: all of its shared memory for what is in flight (629 rows, D 1736, F 864:
     // forward 27.4 -> 21.6 us; 131 rows, D 1448, F 992 23.4 -> 18.8).  Short ones are better off beside the next
-    // kernel's (100 rows, D 768, F 2048: 13.8, and 14.9 alone).
-    const bool alone = p.kb_per >= kLong && tiles * pl.S <= (pl.S >= 4 ? ctx->num_sms * 9 / 10 : ctx->num_sms);
+    // kernel's (100 rows, D 768, F 2048: 13.8, and 14.9 alone), and so are few (dx of 100 rows, D 1024, F 2816, 64 CTAs:
+    // backward 18.9, and 20.1 alone; of 200 rows, 128 CTAs: 24.4, and 22.0 alone).
+    const int ctas = tiles * pl.S, room = pl.S >= 4 ? ctx->num_sms * 9 / 10 : ctx->num_sms;
+    const bool alone = p.kb_per >= kLong && ctas <= room && (EPI != kStore || 2 * ctas > ctx->num_sms);
     p.stages = std::min({8, p.kb_per, std::max(3, ((alone ? kAllSm : kHalfSm) - 1024 - kHead) / stage)});
     p.err = ctx->tickets + kGemmError;
     const int smem = std::max(kHalfSm, 1024 + kHead + std::max(p.stages * stage, p.rows_box * (p.bn + 4) * 4));
