@@ -26,6 +26,7 @@
 #include <cfloat>
 #include <cmath>
 
+#include "index.cuh"
 #include "tc.cuh"
 
 namespace rbk {
@@ -239,12 +240,12 @@ __global__ void __launch_bounds__(kThreads, per_sm(G, T, BWD)) qk_kernel(const _
     auto next = [&](int tk) { return p.tokens - tk > stride ? tk + stride : p.tokens; };
     auto row_of = [&](int tk) { return (int)((__umulhi((uint32_t)tk, p.s_mul) + (uint32_t)tk) >> p.s_shift); };
     auto at = [&](const Heads& t, int tk) {                         // this lane's chunk a of head h0
-        tk = min(tk + sub, p.tokens - 1);
+        tk = token_at(tk, sub, p.tokens);
         const int bi = row_of(tk), si = tk - bi * p.S;
         return t.p + ((long long)bi * t.sb + (long long)si * t.ss + (long long)h0 * t.sh + l.a);
     };
     auto pos_of = [&](int tk) {
-        tk = min(tk + sub, p.tokens - 1);
+        tk = token_at(tk, sub, p.tokens);
         return p.pos ? p.pos[tk] : p.pos0 + (tk - row_of(tk) * p.S);
     };
     // whether this lane has head hd of token tk (+ sub)
