@@ -344,7 +344,8 @@ enum { RBK_ACT_SILU = 0, RBK_ACT_GELU = 1 /* the tanh form */ };
  * up to 32 rows (64 of a narrow block), where reading the weights is the cost, both
  * are kernels that stream them.  h is rounded to half once. */
 typedef struct rbk_ffn_args {
-    int N, D, F;             /* N rows, 0 <= N <= 2^30; D, F <= 2^29             */
+    int N, D, F;             /* N rows, 0 <= N <= 2^30; D, F <= 2^29; at most 2^31 - 1 tiles of
+                                128 x 128 in [N, 2F], [N, D] and [2F, D]         */
     int act;                 /* RBK_ACT_*                                        */
     const void* x; int ldx;  /* [N, D]                                           */
     const void* wgu;         /* [2F, D]: the rows of Wg, then those of Wu        */

@@ -264,6 +264,10 @@ static int check_sizes(const char* who, int N, int D, int F, int act) {
     RBK_REQUIRE(N <= (1 << 30), "%s: more than 2^30 rows", who);         // rounded up to tiles they stay an int
     RBK_REQUIRE(D > 0 && F > 0 && D % 8 == 0 && F % 8 == 0 && D <= (1 << 29) && F <= (1 << 29),
                 "%s: D and F must be positive multiples of 8, at most 2^29 (D=%d F=%d)", who, D, F);
+    // the kernels count the tiles of an output in an int
+    const auto blocks = [](int n) { return ((long long)n + 127) / 128; };
+    RBK_REQUIRE(blocks(N) * blocks(std::max(D, 2 * F)) <= 0x7fffffffLL && blocks(2 * F) * blocks(D) <= 0x7fffffffLL,
+                "%s: more than 2^31 - 1 tiles of 128 x 128 (N=%d D=%d F=%d)", who, N, D, F);
     RBK_REQUIRE(act == RBK_ACT_SILU || act == RBK_ACT_GELU, "%s: act must be RBK_ACT_SILU or RBK_ACT_GELU", who);
     return RBK_OK;
 }

@@ -1496,8 +1496,9 @@ int glu_fwd_tiles(rbk_ctx* ctx, void* h, void* gu, const void* x, int ldx, const
 
 int gemm_store_splits(rbk_ctx* ctx, int M, int N, int K) {
     using namespace gemm;
-    const int units = ((M + 2 * BM - 1) / (2 * BM)) * ((N + 255) / 256), kb = (K + BK - 1) / BK;
-    const int s = std::min(ctx->num_sms / 2 / units, kb / 8);
+    const long long units = (long long)((M + 2 * BM - 1) / (2 * BM)) * ((N + 255) / 256);   // may pass 32 bits
+    const int kb = (K + BK - 1) / BK;
+    const int s = (int)std::min<long long>(ctx->num_sms / 2 / units, kb / 8);
     // At least 16 of a tile's k blocks have to go elsewhere, or the planes and their launch cost what they save: 97
     // rows, D 344, K 1456 18.5 us split and 16.6 whole; 300 rows, D 768, K 1536 23.9 and 25.6; 256 rows, D 1024,
     // K 5632 27.8 and 45.6 (of the whole call).

@@ -257,3 +257,29 @@ def test_args_layouts_match_header(tmp_path):
                    check=True)
     got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == want
+
+
+FFN_SIZES = r"""
+import ctypes as C, sys
+from rbk import lib
+ctx = (C.c_int * 1024)(0, 148)          # a context of a device with 148 SMs: nothing else of it is looked at
+for n, d, f, back in eval(sys.argv[1]):
+    print(lib().rbk_gated_ffn_ws_bytes(ctx, n, d, f, back), lib().rbk_last_error().decode())
+"""
+
+
+def test_ffn_sizes_at_the_ends_of_their_range():
+    """A query with sizes of the documented range answers or refuses, and divides by no product that has wrapped to 0."""
+    import subprocess
+    import sys
+    from rbk._lib import PKG_ROOT
+    # (N, D, F, backward): more tiles than an int counts
+    refused = [(2 ** 30, 2 ** 29, 8, 0), (2 ** 30, 2 ** 29, 8, 1), (2 ** 30, 2 ** 29, 2 ** 29, 0), (2 ** 24, 2 ** 24, 8, 0),
+               (8, 2 ** 29, 2 ** 29, 1), (2 ** 30, 8, 2 ** 29, 0), (2 ** 22, 2 ** 23, 8, 0)]      # 2^15 * 2^16 tiles
+    taken = [(2 ** 30, 8, 8, 0), (2 ** 30, 8, 8, 1), (2 ** 22, 2 ** 22, 2 ** 21, 1), (8, 2 ** 29, 256, 1),
+             (2 ** 22, 2 ** 23 - 128, 8, 0)]
+    r = subprocess.run([sys.executable, "-c", FFN_SIZES, str(refused + taken)], cwd=PKG_ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.returncode
+    lines = r.stdout.splitlines()
+    assert all(x.startswith("-1 ") and "tiles" in x for x in lines[:len(refused)]), lines
+    assert all(int(x.split()[0]) >= 0 for x in lines[len(refused):]), lines
