@@ -88,6 +88,9 @@ struct rbk_ctx {
     // arrive at the barrier (-1: none).
     uint64_t test_tail_wait_ns = 0;
     int test_tail_withheld_cta = -1;
+    // The same for the next launch of the gated feed-forward block's smaller tiles
+    // (rbk_ctx_arm_ffn_timeout_test): the limit of its waits in ns, 0 when not armed.
+    uint64_t test_ffn_wait_ns = 0;
 };
 
 namespace rbk {

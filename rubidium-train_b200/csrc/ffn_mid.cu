@@ -38,6 +38,8 @@ struct Params {
     half* out; long long ldo;      // y or dx; kGlu, kGluBwd: h, [M, N], or NULL
     half* gu;                      // kGlu: gate | up, or NULL; kGluBwd: dgate | dup; [M, 2N]
     int* err;
+    uint64_t wait_ns;              // limit of a wait
+    int hold;                      // test of the limit: a K block whose rows of A CTA 0 does not load, or -1
 };
 
 // act(z) and act'(z), glu_act's formulas.
@@ -131,7 +133,11 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
             for (int j = 0; j < p.bn / 64; ++j) tma_load_2d(sb + 8192 * j, &tmB, full_bar(s), n0 + 64 * j, kb * BK);
         }
     };
-    auto load_a = [&](int s, int kb) { tma_load_2d(ring + s * stage_bytes, &tmA, full_bar(s), kb * BK, m0); };
+    const int held = blockIdx.x == 0 ? p.hold : -1;
+    auto load_a = [&](int s, int kb) {
+        if (kb != held) tma_load_2d(ring + s * stage_bytes, &tmA, full_bar(s), kb * BK, m0);
+    };
+    int issued = 0;                                          // K blocks whose loads thread 0 has issued
     const uint32_t tx = (p.rows_box + p.bn) * BK * 2;
 
     // Everybody but the producer waits here for what came before; bounded waits start after that.
@@ -148,17 +154,13 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
             for (int i = 0; i < first; ++i) load_a(i, kb0 + i);
             int s = 0;
             uint32_t phase = 0;
-            int i = first;
-            for (; i < nk; ++i) {
-                if (!mbar_wait(empty_bar(s), phase, abort_flag)) break;
+            for (issued = first; issued < nk; ++issued) {
+                if (!mbar_wait(empty_bar(s), phase, abort_flag, p.wait_ns)) break;
                 mbar_expect_tx(full_bar(s), tx);
-                load_b(s, kb0 + i);
-                load_a(s, kb0 + i);
+                load_b(s, kb0 + issued);
+                load_a(s, kb0 + issued);
                 if (++s == p.stages) { s = 0; phase ^= 1; }
             }
-            if (*abort_flag)                                 // the copies under way land before the CTA ends, or 4 ms pass
-                for (int n = max(0, i - p.stages); n < i; ++n)
-                    for (int t = 0; t < 200 && !mbar_try_suspend(full_bar(n % p.stages), n / p.stages & 1, 20000u); ++t) {}
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
             int s = 0;
             uint32_t phase = 0;
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait(full_bar(s), phase, abort_flag)) break;
+                if (!mbar_wait(full_bar(s), phase, abort_flag, p.wait_ns)) break;
                 fence_after();
                 const uint32_t sa = ring + s * stage_bytes, sb = sa + BM * BK * 2;
 #pragma unroll
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
     __syncwarp();
     if (warp >= 2) {
         // the tile's sums to shared memory, over the operands' slots: all MMAs have read them
-        if (__all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag) && !*abort_flag)) {
+        if (__all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag, p.wait_ns) && !*abort_flag)) {
             fence_after();
             const int q = warp & 3, row = q * 32 + lane;
             if (q * 32 < rows) {
@@ -206,6 +208,11 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
     if (S > 1) cluster_sync();
     else __syncthreads();
     fence_after();
+    // Every role has ended, so the flag is what it will be.  After a timeout the copies under way, which may be the last
+    // that were issued for each slot, land before the CTA ends, or 4 ms pass.
+    if (threadIdx.x == 0 && *abort_flag)
+        for (int n = max(0, issued - p.stages), t = 0; n < issued; ++n)
+            while (t < 200 && !mbar_try_suspend(full_bar(n % p.stages), n / p.stages & 1, 20000u)) ++t;
 
     uint32_t part[S];
 #pragma unroll
@@ -384,6 +391,9 @@ int run(rbk_ctx* ctx, Params p, const Plan& pl, const void* A, int64_t lda, cons
     const bool alone = p.kb_per >= kLong && ctas <= room && (EPI != kStore || 2 * ctas > ctx->num_sms);
     p.stages = std::min({8, p.kb_per, std::max(3, ((alone ? kAllSm : kHalfSm) - 1024 - kHead) / stage)});
     p.err = ctx->tickets + kGemmError;
+    p.wait_ns = ctx->test_ffn_wait_ns ? ctx->test_ffn_wait_ns : kWaitTimeoutNs;
+    p.hold = ctx->test_ffn_wait_ns ? p.kb_per - 1 : -1;
+    ctx->test_ffn_wait_ns = 0;                               // the test setting covers one launch
     const int smem = std::max(kHalfSm, 1024 + kHead + std::max(p.stages * stage, p.rows_box * (p.bn + 4) * 4));
     CUtensorMap ta, tb;
     RBK_TRY(make_tmap(&ta, A, p.K, p.M, lda, 64, p.rows_box));

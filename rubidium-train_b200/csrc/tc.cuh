@@ -54,13 +54,14 @@ __device__ __forceinline__ bool mbar_try_suspend(uint32_t bar, uint32_t parity, 
 // when another role already aborted.  Waiting threads sleep in try_wait
 // between checks rather than spinning, so they leave the issue slots to the
 // warps doing the work.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                          uint64_t limit_ns = kWaitTimeoutNs) {
     if (mbar_try(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     while (true) {
         if (mbar_try_suspend(bar, parity, 20000u)) return true;
         if (*abort_flag) return false;
-        if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+        if (globaltimer_ns() - t0 > limit_ns) {
             *abort_flag = 1;
             return false;
         }

@@ -125,6 +125,7 @@ _SIGS = {
     "rbk_ctx_device_error": (i32, [vp, C.POINTER(i32)]),
     "rbk_ctx_set_deterministic": (i32, [vp, i32]),
     "rbk_ctx_arm_tail_timeout_test": (i32, [vp, C.c_double, i32]),
+    "rbk_ctx_arm_ffn_timeout_test": (i32, [vp, C.c_double]),
     "rbk_model_ctx": (i32, [vp, C.POINTER(vp)]),
     "rbk_ln_fwd": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, f32, vp]),
     "rbk_ln_bwd": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp]),

@@ -283,3 +283,11 @@ def test_ffn_sizes_at_the_ends_of_their_range():
     lines = r.stdout.splitlines()
     assert all(x.startswith("-1 ") and "tiles" in x for x in lines[:len(refused)]), lines
     assert all(int(x.split()[0]) >= 0 for x in lines[len(refused):]), lines
+
+
+def test_ffn_timeout_test_refusals():
+    from rbk import lib
+    ctx = (C.c_int * 1024)(0, 148)
+    for c, limit, match in ((None, 1e-3, "null ctx"), (ctx, 1e-5, "limit_s"), (ctx, 3.0, "limit_s"),
+                            (ctx, float("nan"), "limit_s")):
+        assert lib().rbk_ctx_arm_ffn_timeout_test(c, limit) == -1 and match in lib().rbk_last_error().decode()

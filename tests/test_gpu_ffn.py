@@ -317,3 +317,26 @@ def test_refused_tensors(ops):
         ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], act="relu")
     with pytest.raises(RuntimeError, match="multiples of 8"):
         ops.gated_ffn_fwd(c["x"][:, :60], c["wgu"][:, :60].contiguous(), c["wd"][:60].contiguous())
+
+
+@pytest.mark.parametrize("N,D,F,back", [(100, 768, 2048, False), (100, 768, 2048, True), (300, 256, 2048, False)])
+def test_a_wait_that_runs_out(ops, N, D, F, back):
+    """A tile whose load never comes: its waits give up after 1 ms with copies of other slots under way, the launch
+    returns, RBK_ERR_TIMEOUT is reported, and the same call again gives the bits of a call before (backward: a
+    cluster shares K out)."""
+    from rbk._lib import call
+    c = case(N, D, F, seed=13)
+    gu = (c["x"].float() @ c["wgu"].float().T).half()
+
+    def once():
+        if back:
+            return ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"])
+        return ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"])
+
+    want = once()
+    assert ops.device_error() == 0
+    call("rbk_ctx_arm_ffn_timeout_test", ops.ctx().handle, 1e-3)
+    once()
+    assert ops.device_error() == -4                        # RBK_ERR_TIMEOUT
+    assert all(torch.equal(a, b) for a, b in zip(once(), want))
+    assert ops.device_error() == 0
