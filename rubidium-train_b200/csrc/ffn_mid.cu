@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
                         for (int k = 0; k < 16; k += 4)
                             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (c + k) * 4), "r"(r[k]),
                                          "r"(r[k + 1]), "r"(r[k + 2]), "r"(r[k + 3]) : "memory");
+                    __syncwarp();                            // the next load is the whole warp's
                 }
             }
             fence_before();
@@ -263,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
         }
     }
 
+    __syncwarp();                                            // lanes leave the loop at different times
     if (S > 1) cluster_sync();                               // the other CTAs have read this one's sums
     else __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, RBK_ERR_TIMEOUT);
