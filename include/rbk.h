@@ -394,6 +394,21 @@ int rbk_gated_ffn_bwd(rbk_ctx* ctx, const rbk_ffn_bwd_args* args, void* stream);
  * planes in a fixed order.  ws NULL: the ctx scratch (see rbk_qk_args.ws). */
 int64_t rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int backward);
 
+/* Which kernels serve a forward (backward != 0: a backward) of these sizes (N > 0): its first
+ * product (gate and up; backward: dgu) and its second (y; backward: dx).  For tests and
+ * profiles; a call chooses by itself. */
+enum {
+    RBK_FFN_ROWS = 0,        /* few rows, weights streamed; cols is 1 where a CTA has at most one tile */
+    RBK_FFN_TILES = 1,       /* one CTA for 128 rows and `cols` accumulator columns, `parts` CTAs share K */
+    RBK_FFN_PAIRS = 2        /* CTA pairs, 256 rows and columns; parts > 1: K shared out, planes in ws */
+};
+typedef struct rbk_ffn_plan {
+    struct {
+        int kernel, cols, parts;
+    } product[2];
+} rbk_ffn_plan;
+int rbk_gated_ffn_plan(rbk_ctx* ctx, int N, int D, int F, int backward, rbk_ffn_plan* plan);
+
 /* ------------------------------------------------------------------------
  * LoRA adapters, kernel level (the model level runs the same GEMMs inside
  * rbk_model_forward / _backward once rbk_model_lora_enable has been called)

@@ -133,12 +133,14 @@ int gemm_store_splits(rbk_ctx* ctx, int M, int N, int K);
 int gemm_store(rbk_ctx* ctx, const rbk_gemm_desc* d, float* ws, cudaStream_t st);
 
 // The same three with smaller tiles where those are too few (ffn_mid.cu), else the functions above.  early: B was
-// complete before the kernel before this one began.  mid_store needs no ws where mid_store_serves.
+// complete before the kernel before this one began.  mid_store needs no ws where mid_serves it.
 int mid_glu_fwd(rbk_ctx* ctx, void* h, void* gu, const void* x, int ldx, const void* wgu, const void* bgu, int N, int D,
                 int F, int act, cudaStream_t st);
 int mid_glu_bwd(rbk_ctx* ctx, void* dgu, void* h, const void* dy, int lddy, const void* wd, const void* gu, int N, int D,
                 int F, int act, cudaStream_t st);
-bool mid_store_serves(rbk_ctx* ctx, int M, int N, int K, int b_mn);
+enum MidProduct { kMidGlu = 0, kMidGluBwd = 1, kMidStore = 2 };
+// Whether the smaller tiles serve the product, and then their accumulator columns and the parts of K (or NULL).
+bool mid_serves(rbk_ctx* ctx, int product, int M, int N, int K, int b_mn, int* cols = nullptr, int* parts = nullptr);
 int mid_store(rbk_ctx* ctx, const rbk_gemm_desc* d, float* ws, int early, cudaStream_t st);
 
 // Ticket slots (see rbk_ctx::tickets).

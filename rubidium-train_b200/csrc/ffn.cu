@@ -249,10 +249,12 @@ int launch_few(rbk_ctx* ctx, const Params& p, cudaStream_t st) {
     return RBK_OK;
 }
 
+static bool few_wide(rbk_ctx* ctx, int R, bool glu) { return (R + (glu ? 7 : 15)) / (glu ? 8 : 16) <= ctx->num_sms; }
+
 template <bool GLU>
 int few_rows(rbk_ctx* ctx, const Params& p, cudaStream_t st) {
     ProfScope prof(ctx, st, kCatGemm, (GLU ? 4.0 : 2.0) * p.N * (double)p.R * p.K, 0);
-    const bool wide = (p.R + (GLU ? 7 : 15)) / (GLU ? 8 : 16) <= ctx->num_sms;
+    const bool wide = few_wide(ctx, p.R, GLU);
     if (p.N <= 8) return wide ? launch_few<1, true, GLU>(ctx, p, st) : launch_few<1, false, GLU>(ctx, p, st);
     if (p.N <= 16) return wide ? launch_few<2, true, GLU>(ctx, p, st) : launch_few<2, false, GLU>(ctx, p, st);
     if (p.N <= 32) return wide ? launch_few<4, true, GLU>(ctx, p, st) : launch_few<4, false, GLU>(ctx, p, st);
@@ -282,7 +284,7 @@ static int check_ptr(const char* who, const char* what, const void* p, bool opti
 
 // The FP32 planes of the down projection (backward: of dx), if the call splits it.
 static int64_t plane_bytes(rbk_ctx* ctx, int M, int N, int K, int b_mn) {
-    if (mid_store_serves(ctx, M, N, K, b_mn)) return 0;
+    if (mid_serves(ctx, kMidStore, M, N, K, b_mn)) return 0;
     const int s = gemm_store_splits(ctx, M, N, K);
     return s > 1 ? (int64_t)s * M * N * 4 : 0;
 }
@@ -305,6 +307,25 @@ int64_t rbk_gated_ffn_ws_bytes(rbk_ctx* ctx, int N, int D, int F, int backward) 
     RBK_REQUIRE(ctx, "%s: ctx is NULL", who);
     if (N == 0 || (!backward && ffn::few(N, D, F))) return 0;
     return ffn::plane_bytes(ctx, N, D, backward ? 2 * F : F, backward != 0);
+}
+
+int rbk_gated_ffn_plan(rbk_ctx* ctx, int N, int D, int F, int backward, rbk_ffn_plan* plan) {
+    const char* who = "rbk_gated_ffn_plan";
+    RBK_TRY(ffn::check_sizes(who, N, D, F, RBK_ACT_SILU));
+    RBK_REQUIRE(ctx && plan, "%s: ctx or plan is NULL", who);
+    RBK_REQUIRE(N > 0, "%s: no rows", who);
+    if (!backward && ffn::few(N, D, F)) {
+        for (int i = 0; i < 2; ++i) plan->product[i] = {RBK_FFN_ROWS, ffn::few_wide(ctx, i ? D : F, i == 0), 1};
+        return RBK_OK;
+    }
+    const int K = backward ? 2 * F : F;                      // of the second product
+    auto& p = plan->product;
+    p[0] = {RBK_FFN_PAIRS, 256, 1};
+    if (mid_serves(ctx, backward ? kMidGluBwd : kMidGlu, N, F, D, backward != 0, &p[0].cols, &p[0].parts))
+        p[0].kernel = RBK_FFN_TILES;
+    p[1] = {RBK_FFN_PAIRS, 256, gemm_store_splits(ctx, N, D, K)};
+    if (mid_serves(ctx, kMidStore, N, D, K, backward != 0, &p[1].cols, &p[1].parts)) p[1].kernel = RBK_FFN_TILES;
+    return RBK_OK;
 }
 
 int rbk_gated_ffn_fwd(rbk_ctx* ctx, const rbk_ffn_args* a, void* stream) {

@@ -25,7 +25,7 @@ constexpr int kHead = 1024;                                  // barriers
 // holds up to 256 columns of TMEM while it waits for the others of its cluster, so that no SM may take more CTAs than
 // its 512 columns serve, this kernel's or the CTA pairs' (512 columns, at least 193 KB) of another stream.
 constexpr int kHalfSm = 113 << 10, kAllSm = 227 << 10;
-enum { kGlu = 0, kGluBwd = 1, kStore = 2 };
+enum { kGlu = kMidGlu, kGluBwd = kMidGluBwd, kStore = kMidStore };
 
 struct Params {
     int M, N, K;                   // rows, output columns (F; store: D), inner extent
@@ -406,7 +406,12 @@ int run(rbk_ctx* ctx, Params p, const Plan& pl, const void* A, int64_t lda, cons
 
 }  // namespace mid
 
-bool mid_store_serves(rbk_ctx* ctx, int M, int N, int K, int b_mn) { return mid::plan(ctx, mid::kStore, M, N, K, b_mn).bn > 0; }
+bool mid_serves(rbk_ctx* ctx, int product, int M, int N, int K, int b_mn, int* cols, int* parts) {
+    const mid::Plan p = mid::plan(ctx, product, M, N, K, b_mn);
+    if (p.bn && cols) *cols = p.bn;
+    if (p.bn && parts) *parts = p.S;
+    return p.bn > 0;
+}
 
 int mid_glu_fwd(rbk_ctx* ctx, void* h, void* gu, const void* x, int ldx, const void* wgu, const void* bgu, int N, int D,
                 int F, int act, cudaStream_t st) {

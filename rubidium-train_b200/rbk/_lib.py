@@ -150,6 +150,7 @@ _SIGS = {
     "rbk_gated_ffn_fwd": (i32, [vp, vp, vp]),
     "rbk_gated_ffn_bwd": (i32, [vp, vp, vp]),
     "rbk_gated_ffn_ws_bytes": (i64, [vp, i32, i32, i32, i32]),
+    "rbk_gated_ffn_plan": (i32, [vp, i32, i32, i32, i32, vp]),
     "rbk_clip_grad_norm": (i32, [vp, vp, i32, f32, vp, vp, vp, vp]),
     "rbk_model_create": (i32, [C.POINTER(vp), C.POINTER(Config), C.POINTER(ModelOpts)]),
     "rbk_model_destroy": (i32, [vp]),

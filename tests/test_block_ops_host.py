@@ -291,3 +291,54 @@ def test_ffn_timeout_test_refusals():
     for c, limit, match in ((None, 1e-3, "null ctx"), (ctx, 1e-5, "limit_s"), (ctx, 3.0, "limit_s"),
                             (ctx, float("nan"), "limit_s")):
         assert lib().rbk_ctx_arm_ffn_timeout_test(c, limit) == -1 and match in lib().rbk_last_error().decode()
+
+
+def ffn_plan(N, D, F, back):
+    """The kernels of a call on 148 SMs, as rbk_gated_ffn_plan gives them."""
+    from rbk import lib
+    ctx, plan = (C.c_int * 1024)(0, 148), (C.c_int * 6)()
+    assert lib().rbk_gated_ffn_plan(ctx, N, D, F, back, plan) == 0, lib().rbk_last_error()
+    return tuple(plan[:3]), tuple(plan[3:])
+
+
+def ffn_kernels(N, D, F):
+    """The kernel instances and configurations that a forward and a backward of these sizes run."""
+    out = set()
+    for back in (0, 1):
+        for i, (kernel, cols, parts) in enumerate(ffn_plan(N, D, F, back)):
+            if kernel == 0:                                 # rows: by the rows' multiple of 8 too
+                parts = 1 if N <= 8 else 2 if N <= 16 else 4 if N <= 32 else 8
+            elif kernel == 2:
+                parts = parts > 1
+            out.add((back, i, kernel, cols, parts))
+    return out
+
+
+def test_ffn_tests_reach_every_kernel():
+    """Whatever kernel a call of 1 to 5000 rows and widths up to 5632 chooses, some size of the GPU tests chooses too."""
+    import random
+
+    import test_gpu_ffn as t
+    tested = set().union(*(ffn_kernels(*s) for s in t.SIZES + t.MIDDLE + t.REST + t.PAIRS))
+    r = random.Random(0)
+    for _ in range(60000):
+        n, d, f = (int(2 ** r.uniform(0, 12.3)), 8 * int(2 ** r.uniform(0, 9.46)), 8 * int(2 ** r.uniform(0, 9.46)))
+        missing = ffn_kernels(n, d, f) - tested
+        assert not missing, (n, d, f, missing)
+
+
+def test_ffn_plan():
+    from rbk import lib
+    rows, pairs = 0, 2
+    assert ffn_plan(1, 2048, 5632, 0) == ((rows, 0, 1), (rows, 1, 1))
+    assert ffn_plan(8192, 2048, 5632, 0) == ((pairs, 256, 1), (pairs, 256, 1))
+    for size in ((1999, 776, 2056), (600, 264, 8712)):
+        for back in (0, 1):
+            (k0, _, _), (k1, _, parts) = ffn_plan(*size, back)
+            assert k0 == k1 == pairs and parts > 1
+            ctx = (C.c_int * 1024)(0, 148)
+            assert lib().rbk_gated_ffn_ws_bytes(ctx, *size, back) == 4 * parts * size[0] * size[1]
+    plan, ctx = (C.c_int * 6)(), (C.c_int * 1024)(0, 148)
+    for args, match in (((None, 4, 64, 128, 0, plan), "NULL"), ((ctx, 4, 64, 128, 0, None), "NULL"),
+                        ((ctx, 0, 64, 128, 0, plan), "no rows"), ((ctx, 4, 60, 128, 0, plan), "multiples")):
+        assert lib().rbk_gated_ffn_plan(*args) == -1 and match in lib().rbk_last_error().decode()

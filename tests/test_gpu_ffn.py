@@ -340,3 +340,171 @@ def test_a_wait_that_runs_out(ops, N, D, F, back):
     assert ops.device_error() == -4                        # RBK_ERR_TIMEOUT
     assert all(torch.equal(a, b) for a, b in zip(once(), want))
     assert ops.device_error() == 0
+
+
+# The kernels that the sizes above do not reach; with them every kernel that a call can choose runs (a CPU test,
+# test_block_ops_host.py, holds these lists against rbk_gated_ffn_plan).
+REST = [(7, 2504, 1256), (5, 136, 1192), (12, 2504, 72), (30, 2384, 264), (61, 264, 1496), (48, 768, 2048),
+        (40, 1248, 4616), (132, 8, 4856), (140, 456, 5192), (200, 2048, 5632), (392, 8, 4760), (405, 8, 5384),
+        (287, 1064, 3952), (526, 1048, 2568), (259, 1032, 4792), (280, 1096, 5256), (264, 1040, 5688), (405, 1064, 4464),
+        (131, 1592, 8), (131, 1592, 1032), (521, 1960, 8), (933, 1208, 456), (4285, 72, 3104)]
+# Full tiles in the forward and the backward: K of the down projection in 12 parts, in 2 and whole; several tiles a pair
+# of CTAs; last tiles of 8 columns and of 128 or 256.
+PAIRS = [(600, 264, 8712), (2049, 776, 2056), (4100, 520, 2568), (4097, 776, 2560)]
+
+
+def full_tiles(ops, N, D, F):
+    """The calls of these sizes run on CTA pairs; whether their second products share K out."""
+    import ctypes as C
+
+    from rbk._lib import call
+    split = []
+    for back in (0, 1):
+        plan = (C.c_int * 6)()
+        call("rbk_gated_ffn_plan", ops.ctx().handle, N, D, F, back, plan)
+        assert plan[0] == plan[3] == 2, list(plan)
+        split.append(plan[5] > 1)
+    return split
+
+
+@pytest.mark.parametrize("N,D,F", REST)
+def test_every_other_kernel(ops, N, D, F):
+    act = "gelu" if (N + F // 8) % 2 else "silu"
+    c = case(N, D, F, N % 3 != 0, N % 4 < 2, seed=14)
+    how = dict(bgu=c["bgu"], bd=c["bd"], residual=c["residual"], act=act)
+    want = ref.fwd(c["x"], c["wgu"], c["wd"], c["bgu"], c["bd"], c["residual"], act)
+    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], **how)
+    for name, t in (("gu", gu), ("h", h), ("y", y)):
+        within(name, t, *want[name])
+    y2, _, h2 = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], save=False, **how)
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+    want = ref.bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], act)
+    dx, dgu, h = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], act=act)
+    for name, t in dict(dx=dx, dgu=dgu, h=h).items():
+        within(name, t, *want[name])
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("N,D,F", PAIRS)
+def test_full_tiles(ops, N, D, F, bias, act):
+    """Everything of a training step against float64, without and with biases and a residual; the same bits without the
+    saved projections, with y over the residual, with dgu over gu, with the kept h and without the weights' gradients."""
+    split = full_tiles(ops, N, D, F)
+    assert split == [F != 2568 and F != 2560] * 2
+    c = case(N, D, F, bias, bias, seed=15)
+    how = dict(bgu=c["bgu"], bd=c["bd"], act=act)
+    want = ref.fwd(c["x"], c["wgu"], c["wd"], c["bgu"], c["bd"], c["residual"], act)
+    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], residual=c["residual"], **how)
+    for name, t in (("gu", gu), ("h", h), ("y", y)):
+        within(name, t, *want[name])
+    over = c["residual"].clone() if bias else torch.empty_like(y)
+    y2, none, h2 = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], residual=over if bias else None, save=False, out=over, **how)
+    assert y2 is over and none is None and torch.equal(y, y2) and torch.equal(h, h2)
+    want = ref.bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], act)
+    grads = dict(dwgu=torch.zeros(2 * F, D, device="cuda"), dwd=torch.zeros(D, F, device="cuda"))
+    if bias:
+        grads.update(dbgu=torch.zeros(2 * F, device="cuda"), dbd=torch.zeros(D, device="cuda"))
+    dx, dgu, hb = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], act=act, **grads)
+    for name, t in dict(grads, dx=dx, dgu=dgu, h=hb).items():
+        within(name, t, *want[name])
+    over = gu.clone()
+    dx2, dgu2, _ = ops.gated_ffn_bwd(c["dy"], c["x"], over, c["wgu"], c["wd"], act=act, h=hb, dgu=over)
+    assert dgu2 is over and torch.equal(dgu2, dgu) and torch.equal(dx2, dx)
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("N,D,F", PAIRS[:2])
+def test_full_tiles_rows_that_are_not_finite(ops, N, D, F):
+    """A row of x or dy that is not finite spoils itself only."""
+    full_tiles(ops, N, D, F)
+    c = case(N, D, F, seed=16)
+    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"])
+    dx, dgu, _ = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"])
+    x, dy = c["x"].clone(), c["dy"].clone()
+    bad = [0, 77, 255, 256, N - 1]
+    x[bad[0::2], 5], x[bad[1::2], 0] = float("nan"), float("inf")
+    dy[bad[0::2], 0], dy[bad[1::2], 7] = float("-inf"), float("nan")
+    keep = torch.ones(N, dtype=torch.bool, device="cuda")
+    keep[bad] = False
+    for a, b in zip((y, gu, h), ops.gated_ffn_fwd(x, c["wgu"], c["wd"])):
+        assert torch.equal(a[keep], b[keep]) and not bool(b[~keep].isfinite().all(1).any())
+    dx2, dgu2, _ = ops.gated_ffn_bwd(dy, c["x"], gu, c["wgu"], c["wd"])
+    for a, b in ((dx, dx2), (dgu, dgu2)):
+        assert torch.equal(a[keep], b[keep]) and not bool(b[~keep].isfinite().all(1).any())
+
+
+def test_full_tiles_extreme_gates(ops):
+    """test_extreme_gates on CTA pairs: gates of FP16's largest size, half of the columns each way."""
+    N, D, F = PAIRS[0]
+    full_tiles(ops, N, D, F)
+    x = torch.ones(N, D, device="cuda", dtype=torch.float16)
+    wgu = torch.zeros(2 * F, D, device="cuda", dtype=torch.float16)
+    wgu[:F // 2, 0], wgu[F // 2:F, 0], wgu[F:, 0] = 60000.0, -60000.0, 0.5
+    wd = torch.zeros(D, F, device="cuda", dtype=torch.float16)
+    wd[0] = 2.0 ** -6
+    dy = torch.ones(N, D, device="cuda", dtype=torch.float16)
+    for act in ("silu", "gelu"):
+        _, gu, h = ops.gated_ffn_fwd(x, wgu, wd, act=act)
+        assert bool((h[:, :F // 2] == 30000).all()) and bool((h[:, F // 2:] == 0).all())
+        _, dgu, h2 = ops.gated_ffn_bwd(dy, x, gu, wgu, wd, act=act)
+        assert torch.equal(h, h2)
+        d = 2.0 ** -6
+        assert bool((dgu[:, :F // 2] == d * 0.5).all()) and bool((dgu[:, F // 2:F] == 0).all())
+        assert bool((dgu[:, F:F + F // 2] == d * 60000).all()) and bool((dgu[:, F + F // 2:] == 0).all())
+
+
+def test_full_tiles_rows_behind_the_last_stay(ops):
+    """Through the C entry: the rows of y, gu, h, dgu and dx from N on stay as they were."""
+    import ctypes as C
+
+    from rbk._lib import FFN_BWD_PACK, FFN_PACK, call
+    N, D, F = PAIRS[1]
+    full_tiles(ops, N, D, F)
+    c = case(N, D, F, seed=17)
+    st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    y, gu, h, dgu, dx, hb = [torch.full((N + 300, k), 9.0, device="cuda").half() for k in (D, 2 * F, F, 2 * F, D, F)]
+    call("rbk_gated_ffn_fwd", ops.ctx().handle, FFN_PACK.pack(
+        N, D, F, 1, c["x"].data_ptr(), D, c["wgu"].data_ptr(), 0, c["wd"].data_ptr(), 0, 0, 0, y.data_ptr(), D,
+        gu.data_ptr(), h.data_ptr(), 0, 0), st)
+    call("rbk_gated_ffn_bwd", ops.ctx().handle, FFN_BWD_PACK.pack(
+        N, D, F, 1, c["dy"].data_ptr(), D, c["x"].data_ptr(), D, gu.data_ptr(), c["wgu"].data_ptr(), c["wd"].data_ptr(),
+        hb.data_ptr(), 1, dgu.data_ptr(), dx.data_ptr(), D, 0, 0, 0, 0, 0, 0), st)
+    want = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], act="gelu")
+    back = ops.gated_ffn_bwd(c["dy"], c["x"], want[1], c["wgu"], c["wd"], act="gelu")
+    for got, w in zip((y, gu, h, dx, dgu, hb), want + back):
+        assert torch.equal(got[:N], w) and bool((got[N:] == 9.0).all())
+
+
+def test_full_tiles_in_graphs(ops):
+    """Two captured graphs replayed at the same time give the bits of the calls."""
+    N, D, F = PAIRS[0]
+    c = case(N, D, F, True, True, seed=18)
+
+    def both():
+        y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], bgu=c["bgu"], bd=c["bd"], residual=c["residual"])
+        return (y, gu, h) + ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"])
+
+    want = both()
+    graphs = []
+    for _ in range(2):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            both()
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=side):
+                out = both()
+        graphs.append((side, gr, out))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for side, gr, out in graphs:
+            with torch.cuda.stream(side):
+                for t in out:
+                    t.zero_()
+                gr.replay()
+    torch.cuda.synchronize()
+    for _, _, out in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert ops.device_error() == 0
