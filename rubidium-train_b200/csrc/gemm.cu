@@ -205,7 +205,7 @@ __device__ __forceinline__ void prefetch_h(uint4* pf, const half* g, int ld, int
         if (m < p.M && col < p.N) {
             const half* src = g + (size_t)m * ld + col;
             if (col + 8 <= p.N) {
-                u = __ldg(reinterpret_cast<const uint4*>(src));
+                u = *reinterpret_cast<const uint4*>(src);   // an ordinary load: the output may lie over g
             } else {
                 half h[8];
 #pragma unroll
@@ -404,8 +404,8 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(float* __restrict__ 
 }
 
 // out[m, n] = sum over the planes, in split order, + bias[n] + aux[m, n], rounded to half: 8 columns a thread.
-// The planes come from L2; 1999 x 776, two planes: about 3 us, and the GEMM before it 16 us instead of 29.
-__global__ void __launch_bounds__(256) splitk_store_kernel(half* __restrict__ out, int ldo, const float* __restrict__ part,
+// out may lie over aux.  The planes come from L2; 1999 x 776, two planes: about 3 us, and the GEMM before it 16 us instead of 29.
+__global__ void __launch_bounds__(256) splitk_store_kernel(half* out, int ldo, const float* __restrict__ part,
                                                            int M, int N, int ldp, int splits,
                                                            const half* __restrict__ bias, const half* aux, int ld_aux) {
     grid_dependency_sync();
