@@ -258,7 +258,10 @@ int few_rows(rbk_ctx* ctx, const Params& p, cudaStream_t st) {
     if (p.N <= 8) return wide ? launch_few<1, true, GLU>(ctx, p, st) : launch_few<1, false, GLU>(ctx, p, st);
     if (p.N <= 16) return wide ? launch_few<2, true, GLU>(ctx, p, st) : launch_few<2, false, GLU>(ctx, p, st);
     if (p.N <= 32) return wide ? launch_few<4, true, GLU>(ctx, p, st) : launch_few<4, false, GLU>(ctx, p, st);
-    return wide ? launch_few<8, true, GLU>(ctx, p, st) : launch_few<8, false, GLU>(ctx, p, st);
+    // 33 to 64 rows: D is at most 2048, which is 128 of the down projection's tiles
+    if constexpr (GLU)
+        if (!wide) return launch_few<8, false, GLU>(ctx, p, st);
+    return launch_few<8, true, GLU>(ctx, p, st);
 }
 
 static int check_sizes(const char* who, int N, int D, int F, int act) {

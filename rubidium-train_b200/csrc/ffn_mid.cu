@@ -1,11 +1,11 @@
 // ffn_mid.cu — the gated feed-forward block's products where the 256 x 256 tiles of gemm.cu are too few for the
 // machine: some tens to a few hundred rows, or narrow blocks.
 //
-// One CTA has 128 rows and `bn` columns of a product (EPI_GLU: bn / 2 of the gate and the same of the up
-// projection), and of K one part of S: the S CTAs of a tile are a cluster.  Each leaves its FP32 sums in its own
-// shared memory, and every CTA of the cluster adds a part of the tile from all of them, in order, through
-// distributed shared memory, applies the epilogue and stores it: one launch, no planes in global memory, and two
-// runs give the same bits.
+// One CTA has 128 rows and `bn` columns of a product (kGlu: bn / 2 of the gate and the same of the up projection),
+// and of K one part of S (gate and up: all of it; dgu: up to 2 parts; y and dx: up to 8): the S CTAs of a tile are a
+// cluster.  Each leaves its FP32 sums in its own shared memory, and every CTA of the cluster adds a part of the tile
+// from all of them, in order, through distributed shared memory, applies the epilogue and stores it: one launch, no
+// planes in global memory, and two runs give the same bits.
 // Bound by latency: the first loads, a chain of K blocks with what an SM has in flight (96 KB, 200 where one CTA has
 // it), the exchange and the drain.  100 rows, D 2048, F 5632: 28 us for the forward's two launches (floor 10.7); each
 // uses 11 to 19% of the tensor pipe and 16 to 30% of L2 and HBM.
@@ -299,12 +299,16 @@ int launch_s(rbk_ctx* ctx, const CUtensorMap& ta, const CUtensorMap& tb, const P
 template <int EPI>
 int launch(rbk_ctx* ctx, int S, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int tiles, int smem,
            cudaStream_t st) {
-    switch (S) {
-        case 1: return launch_s<EPI, 1>(ctx, ta, tb, p, tiles, smem, st);
-        case 2: return launch_s<EPI, 2>(ctx, ta, tb, p, tiles, smem, st);
-        case 4: return launch_s<EPI, 4>(ctx, ta, tb, p, tiles, smem, st);
-        default: return launch_s<EPI, 8>(ctx, ta, tb, p, tiles, smem, st);
+    // the parts of K that plan() gives: gate and up one, dgu one or two, y and dx up to eight
+    if (S == 1) return launch_s<EPI, 1>(ctx, ta, tb, p, tiles, smem, st);
+    if constexpr (EPI != kGlu)
+        if (S == 2) return launch_s<EPI, 2>(ctx, ta, tb, p, tiles, smem, st);
+    if constexpr (EPI == kStore) {
+        if (S == 4) return launch_s<EPI, 4>(ctx, ta, tb, p, tiles, smem, st);
+        if (S == 8) return launch_s<EPI, 8>(ctx, ta, tb, p, tiles, smem, st);
     }
+    set_error("mid_kernel: no instance for %d parts of K", S);
+    return RBK_ERR_INVALID;
 }
 
 // The tiles of a call, or bn 0: those of gemm.cu.  Two CTAs fit an SM; what is wanted is one round of them with the
