@@ -342,3 +342,15 @@ def test_ffn_plan():
     for args, match in (((None, 4, 64, 128, 0, plan), "NULL"), ((ctx, 4, 64, 128, 0, None), "NULL"),
                         ((ctx, 0, 64, 128, 0, plan), "no rows"), ((ctx, 4, 60, 128, 0, plan), "multiples")):
         assert lib().rbk_gated_ffn_plan(*args) == -1 and match in lib().rbk_last_error().decode()
+
+
+def test_import_without_a_cuda_build_of_torch():
+    """The package's operators import where torch has none of its CUDA functions."""
+    import subprocess
+    import sys
+    from rbk._lib import PKG_ROOT
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_get')]:\n    delattr(torch._C, n)\n"
+            "import rbk.ops, rbk.model, rbk.tokenizer\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=PKG_ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
