@@ -257,7 +257,7 @@ int rbk_adam_tail(rbk_ctx* ctx, const rbk_tail_args* args, void* stream);
 typedef struct rbk_grad {
     const void* g;
     void* out;
-    int64_t n;               /* >= 0                                              */
+    int64_t n;               /* 0 <= n < 2^40; of all tensors less than 2^44 bytes */
     int64_t half;            /* 0: FP32, 1: half                                  */
 } rbk_grad;
 

@@ -293,7 +293,7 @@ static int check(const rbk_grad* t, int count, float max_norm, const float* norm
                     "%s: tensor %d is not aligned to its type", who, i);
         RBK_REQUIRE(t[i].n < (1LL << 40), "%s: tensor %d is too large", who, i);
         chunks += t[i].n * (long long)es / kChunkBytes + 2;
-        RBK_REQUIRE(chunks < (1LL << 31), "%s: the tensors are too large", who);
+        RBK_REQUIRE(chunks < (1LL << 30), "%s: the tensors are too large", who);   // a block's next chunk fits an int
     }
     try {
         RBK_REQUIRE(disjoint(t, count), "%s: a written range overlaps another tensor", who);

@@ -193,6 +193,15 @@ def test_clip_accepts(tensors):
     assert st == -1 and "ctx is NULL" in msg
 
 
+def test_clip_counts_chunks_in_32_bits():
+    """Tensors that are only counted may be given more than once: 2^27 chunks of 16 KB each here, fewer than 2^30 in all."""
+    one = (P, None, (1 << 39) - 65536, 0)
+    st, msg = clip([one] * 8)
+    assert st == -1 and "ctx is NULL" in msg
+    st, msg = clip([(P, None, 1 << 39, 0)] * 8)
+    assert st == -1 and "too large" in msg
+
+
 def test_packed_args_are_the_structs():
     """The packed forms that the ops pass have the structs' bytes."""
     from rbk import _lib
