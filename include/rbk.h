@@ -269,7 +269,8 @@ typedef struct rbk_grad {
  * Where the norm is at most max_norm, nothing is written in place; where a gradient
  * is infinite or NaN they all pass unchanged, so the tail finds the overflow and skips
  * its step.  Squares are summed in FP64, in a fixed order: no finite gradient overflows
- * the sum, and two runs give the same bits.
+ * the sum, and two runs give the same bits.  A norm beyond FP32 is written as infinity;
+ * the gradients are clipped by it all the same.
  * Written ranges must not overlap each other or another tensor (RBK_ERR_INVALID);
  * `tensors` is a host array, read during the call only.  ws: RBK_CLIP_WS_BYTES of
  * device memory, or NULL for the ctx scratch (see rbk_qk_args.ws).

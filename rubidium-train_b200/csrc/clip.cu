@@ -15,6 +15,7 @@
 // the same stretch of memory together (each its own run of neighbours: 338 us against 323); a block searches the
 // table for its first chunk's tensor and walks on from there.  The second kernel goes backwards.
 #include <algorithm>
+#include <cfloat>
 #include <new>
 #include <vector>
 
@@ -143,13 +144,22 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
     if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
 
+// v * coef, or with TINY v * 2^-126 * coef: a factor below FP32's normal range as two in it.  What the first product
+// rounds, below 2^-126, ends below 2^-126 of that; a half is nothing there.
+template <bool TINY>
 __device__ __forceinline__ uint4 scaled(uint4 v, int half, float coef) {
     if (half) {
         float f[8];
         h8_to_f(v, f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= coef;
+        for (int j = 0; j < 8; ++j) f[j] *= TINY ? 0.0f : coef;
         return f_to_h8(f);
+    }
+    if (TINY) {
+        v.x = __float_as_uint(__uint_as_float(v.x) * FLT_MIN);
+        v.y = __float_as_uint(__uint_as_float(v.y) * FLT_MIN);
+        v.z = __float_as_uint(__uint_as_float(v.z) * FLT_MIN);
+        v.w = __float_as_uint(__uint_as_float(v.w) * FLT_MIN);
     }
     v.x = __float_as_uint(__uint_as_float(v.x) * coef);
     v.y = __float_as_uint(__uint_as_float(v.y) * coef);
@@ -183,6 +193,7 @@ __device__ __forceinline__ uint4 funnel(const uint4& v, const uint4& next, int s
 }
 // A chunk to out, scaled.  out's alignment is its own: where its 16-byte vectors lie s bytes off g's, each is put
 // together from two neighbouring vectors of g, the second from the next lane (lane 31 reads it again).
+template <bool TINY>
 __device__ __forceinline__ void store_chunk(const Tensor& t, const Chunk& k, const uint4* v, float coef) {
     const int ve = t.half ? 8 : 4, es = t.half ? 2 : 4;
     char* o = t.out + k.e * es;
@@ -214,16 +225,34 @@ __device__ __forceinline__ void store_chunk(const Tensor& t, const Chunk& k, con
             store_part(o + (long long)i * kThreads * 16, v[i], t.half, s / es, ve);
             continue;
         }
-        if ((threadIdx.x & 31) == 31) next = scaled(g[i * kThreads + 1], t.half, coef);
+        if ((threadIdx.x & 31) == 31) next = scaled<TINY>(g[i * kThreads + 1], t.half, coef);
         *reinterpret_cast<uint4*>(o + s + (long long)i * kThreads * 16) = funnel(v[i], next, s);
     }
 }
 
+// The chunks of a block, backwards.
+template <int CAP, bool TINY>
+__device__ __forceinline__ void scale_chunks(const Table<CAP>& tab, float coef) {
+    int c = tab.chunks - 1 - (int)blockIdx.x;
+    for (int k = c >= 0 ? tensor_of(tab, c) : 0; c >= 0; c -= gridDim.x) {
+        while (tab.t[k].first > c) --k;
+        const Tensor& t = tab.t[k];
+        if (!t.out || (t.out == t.g && coef == 1.0f && !TINY)) continue;
+        const Chunk ch = chunk_of(t, c);
+        uint4 v[kVec];
+        load_chunk(v, t, ch);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = scaled<TINY>(v[i], t.half, coef);
+        store_chunk<TINY>(t, ch, v, coef);
+    }
+}
+
 template <int CAP>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<CAP> tab, const double* part,
+__global__ void __launch_bounds__(kThreads, kPerSm) scale_kernel(const __grid_constant__ Table<CAP> tab, const double* part,
                                                          int parts, float max_norm, const rbk_scaler* scaler,
                                                          float* norm_out) {
     __shared__ float coef_s;
+    __shared__ int tiny_s;
     grid_dependency_sync();
     double s = 0.0;
     for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
@@ -232,23 +261,14 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
         const double norm = sqrt(s) / (scaler ? (double)scaler->scale : 1.0);
         // 1 too for a NaN (no comparison holds) and an infinite norm
         const bool bites = max_norm > 0.0f && norm > (double)max_norm && norm <= 1.7976931348623157e308;
-        coef_s = bites ? (float)((double)max_norm / norm) : 1.0f;
+        const double f = bites ? (double)max_norm / norm : 1.0;
+        tiny_s = f < (double)FLT_MIN;
+        coef_s = (float)(tiny_s ? f / (double)FLT_MIN : f);
         if (norm_out && blockIdx.x == 0) *norm_out = (float)norm;
     }
     __syncthreads();
-    const float coef = coef_s;
-    int c = tab.chunks - 1 - (int)blockIdx.x;
-    for (int k = c >= 0 ? tensor_of(tab, c) : 0; c >= 0; c -= gridDim.x) {
-        while (tab.t[k].first > c) --k;
-        const Tensor& t = tab.t[k];
-        if (!t.out || (t.out == t.g && coef == 1.0f)) continue;
-        const Chunk ch = chunk_of(t, c);
-        uint4 v[kVec];
-        load_chunk(v, t, ch);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = scaled(v[i], t.half, coef);
-        store_chunk(t, ch, v, coef);
-    }
+    if (tiny_s) scale_chunks<CAP, true>(tab, coef_s);
+    else scale_chunks<CAP, false>(tab, coef_s);
 }
 
 // Written ranges overlap nothing but the gradient they replace.

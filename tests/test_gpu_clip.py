@@ -196,3 +196,28 @@ def test_refused_tensors(ops):
             ops.clip_grad_norm(grads, 1.0, **kw)
     with pytest.raises(RuntimeError, match="overlaps"):
         ops.clip_grad_norm([g, g], 1.0)
+
+
+def test_factors_below_the_normal_range(ops):
+    """max_norm / norm below 2^-126, and below the smallest subnormal: large gradients keep all their bits.  The factor
+    is then two, each right to E, the first product to E (2^-150 among the subnormals, times a factor of at most 1), the
+    second to E (2^-150): 7 E as before, and 2^-149."""
+    for v, max_norm, scale in ((3e38, 1e-3, 1.0), (3e38, 1e-7, 1.0), (1e30, 1e-12, 1.0), (3e38, 1e-30, 2.0 ** -20),
+                               (1e20, 1e-38, 1.0)):
+        max_norm = float(torch.tensor(max_norm, dtype=torch.float32))
+        half = float(torch.tensor(max_norm / math.sqrt(2), dtype=torch.float32))
+        g = torch.full((70001,), v, device="cuda")
+        g[::3] = 1.0
+        g[1::7] = -v / 7
+        h = torch.full((33,), 2.0, device="cuda").half()
+        sc = ops.new_scaler(scale=scale)
+        want = math.sqrt(float((g.double() ** 2).sum()) + 33 * 4.0)
+        f = max_norm / (want / scale)
+        assert f < 2.0 ** -126
+        out = [torch.empty_like(g), torch.ones_like(h), torch.full((g.numel() + 9,), 5.0, device="cuda")[9:]]
+        ops.clip_grad_norm([g, h, g], half, scaler=sc, out=[out[0], out[1], None])
+        ops.clip_grad_norm([g, h], max_norm, scaler=sc, out=[out[2], None])
+        lim = 7 * E * (g.double() * f).abs() + 2.0 ** -149
+        f2 = half / (math.sqrt(2 * float((g.double() ** 2).sum()) + 33 * 4.0) / scale)
+        assert bool(((out[0].double() - g.double() * f2).abs() <= lim).all()) and bool((out[1] == 0).all())
+        assert bool(((out[2].double() - g.double() * f).abs() <= lim).all())
