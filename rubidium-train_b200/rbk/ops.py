@@ -342,6 +342,8 @@ def _heads(t, name, shape):
     st = t.stride()
     if (t.dtype is _F16 and t.shape == shape and t.get_device() == _dev() and len(st) == 4
             and (st[3] == 1 or shape[3] == 1)):
+        if (st[0] | st[1] | st[2]) & 7:                     # the stride of an axis of size 1 says nothing
+            st = [s if n > 1 else 0 for s, n in zip(st, shape)]
         return t.data_ptr(), st[0], st[1], st[2]
     _refuse(t, _F16, name, shape, "heads [B, S, H, dh] with contiguous channels, a")
 

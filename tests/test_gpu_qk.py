@@ -272,3 +272,22 @@ def test_refused_tensors(ops):
         ops.qk_norm_rope_fwd(q, None, out=(q[:, :1].expand(1, 4, 2, 64), None))
     with pytest.raises(RuntimeError, match="rot"):
         ops.qk_norm_rope_fwd(q, None, rot=24)
+
+
+def test_strides_of_axes_of_size_one(ops):
+    """Nothing is read by the stride of an axis of size 1, so any will do: torch gives such axes what it likes."""
+    x = torch.randn(3, 64, device="cuda").half()
+    g = (1 + torch.randn(64, device="cuda")).half()
+    for shape, rows in (((1, 3, 1, 64), (0, 64, 0)), ((1, 1, 3, 64), (0, 0, 64)), ((3, 1, 1, 64), (64, 0, 0))):
+        strides = [s if n > 1 else 13 for s, n in zip(rows, shape)] + [1]
+        odd = torch.as_strided(x, shape, strides)
+        y, dq = torch.as_strided(torch.zeros_like(x), shape, strides), torch.as_strided(torch.zeros_like(x), shape, strides)
+        plain = x.view(shape)
+        want, _ = ops.qk_norm_rope_fwd(plain, None, g)
+        ops.qk_norm_rope_fwd(odd, None, g, out=(y, None))
+        assert torch.equal(y, want)
+        wdq, _, wg, _ = ops.qk_norm_rope_bwd(plain, None, plain, None, g)
+        _, _, dg, _ = ops.qk_norm_rope_bwd(odd, None, odd, None, g, out=(dq, None))
+        assert torch.equal(dq, wdq) and torch.equal(dg, wg)
+    with pytest.raises(RuntimeError, match="multiples of 8"):
+        ops.qk_norm_rope_fwd(torch.as_strided(x, (1, 2, 1, 64), (0, 65, 0, 1)), None)
