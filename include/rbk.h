@@ -275,7 +275,13 @@ typedef struct rbk_grad {
  * `tensors` is a host array, read during the call only.  ws: RBK_CLIP_WS_BYTES of
  * device memory, or NULL for the ctx scratch (see rbk_qk_args.ws).
  * rbk_adam_tail's own max_norm clips each tensor by itself, as the reference does
- * (src/model.cu:493-523); this is the norm over all of them, for it to follow. */
+ * (src/model.cu:493-523); this is the norm over all of them, for it to follow.
+ * The norm is that of the elements given to this call, on this device.  Under data
+ * parallelism the gradients have to be whole and reduced first, the same on every rank,
+ * as they are after rbk_model_backward with the plain all-reduce.  It is NOT for the
+ * sharded optimizer (rbk_dp_opts.shard_optimizer): a rank then holds the reduced slice
+ * of each bucket beside unreduced ones, so the ranks would clip by different factors;
+ * there rbk_adam_tail's per-tensor max_norm is the clip that is right on every rank. */
 #define RBK_CLIP_WS_BYTES (16 << 10)
 int rbk_clip_grad_norm(rbk_ctx* ctx, const rbk_grad* tensors, int count, float max_norm, const rbk_scaler* scaler,
                        float* norm, void* ws, void* stream);

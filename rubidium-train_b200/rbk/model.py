@@ -124,6 +124,11 @@ class RubidiumTransformer:
     def loss_buffer(self):
         return self._bufs[BUF_LOSS]
 
+    @property
+    def scaler_buffer(self):
+        """The device's rbk_scaler (int32 [8]), as ops.clip_grad_norm takes it."""
+        return self._scaler
+
     def tensor(self, name: str, which: str = "p32") -> torch.Tensor:
         off, r, c = self._names[name]
         buf = {"p16": BUF_P16, "p32": BUF_P32, "grad": BUF_GRAD, "m": BUF_M, "v": BUF_V}[which]

@@ -209,7 +209,8 @@ def clip_grad_norm(grads, max_norm, scaler=None, out=None):
 
     grads: contiguous FP32 or half tensors.  scaler: a new_scaler() buffer (None: no loss scale).  out: a tensor for each
     of its gradient's type and size, or None in a place to count that gradient and not write it.  max_norm <= 0: only
-    the norm is computed (and `out` is a copy)."""
+    the norm is computed (and `out` is a copy).  The norm is over what this call is given: not for a model with the
+    sharded optimizer (dp_init(shard=True)), whose ranks hold different slices of the reduced gradients."""
     dev, n = _dev(), len(grads)
     f32, f16 = torch.float32, torch.float16
     T = torch.Tensor

@@ -221,3 +221,23 @@ def test_factors_below_the_normal_range(ops):
         f2 = half / (math.sqrt(2 * float((g.double() ** 2).sum()) + 33 * 4.0) / scale)
         assert bool(((out[0].double() - g.double() * f2).abs() <= lim).all()) and bool((out[1] == 0).all())
         assert bool(((out[2].double() - g.double() * f).abs() <= lim).all())
+
+
+def test_model_step_clipped_by_the_global_norm(ops):
+    """Between a model's backward and its optimizer step, by public means: the arena's gradients, the model's scaler.
+    The step is the one of gradients scaled by hand: m = 0.1 g / scale * factor, the factor right to 7 E, the tail's
+    division and product to 3 E more."""
+    from rbk.model import ModelConfig, RubidiumTransformer
+    m = RubidiumTransformer(ModelConfig(V=512, T=64, D=128, H=2, L=2, FF=256), max_batch=2, max_seq=64)
+    m.init_weights(seed=5)
+    tok = torch.randint(0, 512, (2, 64), device="cuda", dtype=torch.int32)
+    m.forward(tok, tok, 2, 64)
+    m.backward(tok, tok, 2, 64)
+    g, scale = m.grad.double(), m.loss_scale
+    want = float(g.norm()) / scale
+    norm = ops.clip_grad_norm([m.grad], want / 4, scaler=m.scaler_buffer)
+    assert abs(float(norm) - want) <= 2 * E * want
+    m.optimizer_step(1, 1e-3)
+    got, v = m._bufs[3].double(), 0.1 * g / scale / 4
+    assert bool(((got - v).abs() <= 10 * E * v.abs() + 2.0 ** -149).all()) and float(got.norm()) > 0
+    assert m.scaler().skipped == 0
