@@ -483,15 +483,15 @@ def gated_ffn_fwd(x, wgu, wd, bgu=None, bd=None, residual=None, act="silu", save
 
 
 def gated_ffn_bwd(dy, x, gu, wgu, wd, act="silu", h=None, want_dx=True, dwgu=None, dbgu=None, dwd=None, dbd=None,
-                  dgu=None):
+                  dgu=None, out=None):
     """Its backward (rbk_gated_ffn_bwd) from the saved gu.  h: the forward's, or None to have it computed again.
     dwgu [2F, D], dbgu [2F], dwd [D, F], dbd [D]: FP32, accumulate; those left out are not computed.  dgu: may be gu.
-    Returns (dx or None, dgu, h)."""
+    x: may be None without dwgu, which alone reads it.  out: dx, may be dy or x.  Returns (dx or None, dgu, h)."""
     shape, dev = dy.shape, dy.device
     N, D = shape
     F = wd.shape[1]
     pdy, lddy = _rows(dy, "dy", shape)
-    px, ldx = _rows(x, "x", shape)
+    px, ldx = (0, 0) if x is None else _rows(x, "x", shape)
     pgu = _here(gu, _F16, "gu", (N, 2 * F))
     pwgu, pwd = _here(wgu, _F16, "wgu", (2 * F, D)), _here(wd, _F16, "wd", (D, F))
     recompute = h is None
@@ -506,15 +506,19 @@ def gated_ffn_bwd(dy, x, gu, wgu, wd, act="silu", h=None, want_dx=True, dwgu=Non
     else:
         pdgu = _here(dgu, _F16, "dgu", (N, 2 * F))
     handle = ctx().handle
-    dx, pdx, ws, pws, nws = None, 0, None, 0, 0
+    dx, pdx, lddx, ws, pws, nws = None, 0, D, None, 0, 0
     if want_dx:
-        dx = torch.empty_like(dy)
-        pdx = dx.data_ptr()
+        if out is None:
+            dx = torch.empty_like(dy)                       # contiguous, whatever dy's row stride
+            pdx = dx.data_ptr()
+        else:
+            dx = out
+            pdx, lddx = _rows(dx, "out", shape)
         ws, pws, nws = _ffn_ws(handle, N, D, F, 1, dev)
     p1 = 0 if dwgu is None else _here(dwgu, _F32, "dwgu", (2 * F, D))
     p2 = 0 if dbgu is None else _here(dbgu, _F32, "dbgu", (2 * F,))
     p3 = 0 if dwd is None else _here(dwd, _F32, "dwd", (D, F))
     p4 = 0 if dbd is None else _here(dbd, _F32, "dbd", (D,))
     call("rbk_gated_ffn_bwd", handle, FFN_BWD_PACK.pack(N, D, F, _ACTS[act], pdy, lddy, px, ldx, pgu, pwgu, pwd, ph,
-                                                        recompute, pdgu, pdx, D, p1, p2, p3, p4, pws, nws), _s())
+                                                        recompute, pdgu, pdx, lddx, p1, p2, p3, p4, pws, nws), _s())
     return dx, dgu, h

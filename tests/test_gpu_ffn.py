@@ -508,3 +508,28 @@ def test_full_tiles_in_graphs(ops):
     for _, _, out in graphs:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("N", [5, 100, 2100])
+def test_backward_without_x_and_into_given_rows(ops, N):
+    """dx and dgu need no x; dx may go over dy or x, with weight gradients too, or into rows of its own stride."""
+    D, F = 136, 2056
+    c = case(N, D, F, seed=19)
+    gu = (c["x"].float() @ c["wgu"].float().T).half()
+    grads = [dict(dwgu=torch.zeros(2 * F, D, device="cuda"), dwd=torch.zeros(D, F, device="cuda")) for _ in range(3)]
+    dx, dgu, h = ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"], **grads[0])
+    dx2, dgu2, h2 = ops.gated_ffn_bwd(c["dy"], None, gu, c["wgu"], c["wd"])
+    assert torch.equal(dx, dx2) and torch.equal(dgu, dgu2) and torch.equal(h, h2)
+    for i, over in ((1, "dy"), (2, "x")):
+        t = {k: c[k].clone() for k in ("dy", "x")}
+        dx3, _, _ = ops.gated_ffn_bwd(t["dy"], t["x"], gu, c["wgu"], c["wd"], out=t[over], **grads[i])
+        assert dx3 is t[over] and torch.equal(dx3, dx)
+        # FP32 additions in another order where K is shared out: twice the bound of one sum
+        for k, a, b in (("dwgu", dgu, c["x"]), ("dwd", c["dy"], h)):
+            lim = 2 * (N + 1) * ref.E * (a.double().abs().T @ b.double().abs())
+            assert bool(((grads[i][k] - grads[0][k]).double().abs() <= lim).all())
+    wide = torch.full((N, D + 24), 9.0, device="cuda", dtype=torch.float16)
+    ops.gated_ffn_bwd(c["dy"], None, gu, c["wgu"], c["wd"], out=wide[:, 8:8 + D])
+    assert torch.equal(wide[:, 8:8 + D], dx) and bool((wide[:, :8] == 9).all()) and bool((wide[:, 8 + D:] == 9).all())
+    with pytest.raises(RuntimeError, match="x is NULL"):
+        ops.gated_ffn_bwd(c["dy"], None, gu, c["wgu"], c["wd"], dwgu=grads[0]["dwgu"])
