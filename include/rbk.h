@@ -102,8 +102,8 @@ int rbk_ctx_set_deterministic(rbk_ctx* ctx, int on);
 int rbk_ctx_arm_tail_timeout_test(rbk_ctx* ctx, double limit_s, int withheld_cta);
 /* Test only, in the same way: of the next rbk_gated_ffn_* launch on this context whose
  * tiles have 128 rows (some tens to some hundred rows; the setting is cleared when it is
- * used), the waits give up after limit_s seconds (1e-4 .. 2) and the first CTA leaves out
- * one load.  The launch returns with wrong outputs and rbk_ctx_device_error reports
+ * used), the waits give up after limit_s seconds (1e-4 .. 2) and wait for more bytes than
+ * are loaded.  The launch returns with wrong outputs and rbk_ctx_device_error reports
  * RBK_ERR_TIMEOUT; the next launch runs normally. */
 int rbk_ctx_arm_ffn_timeout_test(rbk_ctx* ctx, double limit_s);
 

@@ -30,6 +30,7 @@ enum { kGlu = kMidGlu, kGluBwd = kMidGluBwd, kStore = kMidStore };
 struct Params {
     int M, N, K;                   // rows, output columns (F; store: D), inner extent
     int bn, m_blocks, k_blocks, kb_per, stages, rows_box;
+    uint32_t tx;                   // bytes of a K block's loads
     int b_mn;                      // B(n, k) is contiguous in n
     int early;                     // B may be read before the kernel before this one has ended
     int act;
@@ -39,7 +40,6 @@ struct Params {
     half* gu;                      // kGlu: gate | up, or NULL; kGluBwd: dgate | dup; [M, 2N]
     int* err;
     uint64_t wait_ns;              // limit of a wait
-    int hold;                      // test of the limit: a K block whose rows of A CTA 0 does not load, or -1
 };
 
 // act(z) and act'(z), glu_act's formulas.
@@ -133,12 +133,8 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
             for (int j = 0; j < p.bn / 64; ++j) tma_load_2d(sb + 8192 * j, &tmB, full_bar(s), n0 + 64 * j, kb * BK);
         }
     };
-    const int held = blockIdx.x == 0 ? p.hold : -1;
-    auto load_a = [&](int s, int kb) {
-        if (kb != held) tma_load_2d(ring + s * stage_bytes, &tmA, full_bar(s), kb * BK, m0);
-    };
+    auto load_a = [&](int s, int kb) { tma_load_2d(ring + s * stage_bytes, &tmA, full_bar(s), kb * BK, m0); };
     int issued = 0;                                          // K blocks whose loads thread 0 has issued
-    const uint32_t tx = (p.rows_box + p.bn) * BK * 2;
 
     // Everybody but the producer waits here for what came before; bounded waits start after that.
     if (warp != 0 || lane != 0) grid_dependency_sync();
@@ -147,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
             const int nk = kb1 - kb0, first = min(nk, p.stages);
             if (!p.early) grid_dependency_sync();
             for (int i = 0; i < first; ++i) {
-                mbar_expect_tx(full_bar(i), tx);
+                mbar_expect_tx(full_bar(i), p.tx);
                 load_b(i, kb0 + i);
             }
             if (p.early) grid_dependency_sync();
@@ -156,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
             uint32_t phase = 0;
             for (issued = first; issued < nk; ++issued) {
                 if (!mbar_wait(empty_bar(s), phase, abort_flag, p.wait_ns)) break;
-                mbar_expect_tx(full_bar(s), tx);
+                mbar_expect_tx(full_bar(s), p.tx);
                 load_b(s, kb0 + issued);
                 load_a(s, kb0 + issued);
                 if (++s == p.stages) { s = 0; phase ^= 1; }
@@ -194,12 +190,10 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
                     uint32_t r[16];
                     tmem_ld16(t + c, r);
                     tmem_wait_ld();
-                    if (row < p.rows_box)
 #pragma unroll
-                        for (int k = 0; k < 16; k += 4)
-                            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (c + k) * 4), "r"(r[k]),
-                                         "r"(r[k + 1]), "r"(r[k + 2]), "r"(r[k + 3]) : "memory");
-                    __syncwarp();                            // the next load is the whole warp's
+                    for (int k = 0; k < 16; k += 4)          // a warp's 32 rows have room, those behind the last too
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (c + k) * 4), "r"(r[k]),
+                                     "r"(r[k + 1]), "r"(r[k + 2]), "r"(r[k + 3]) : "memory");
                 }
             }
             fence_before();
@@ -209,11 +203,6 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
     if (S > 1) cluster_sync();
     else __syncthreads();
     fence_after();
-    // Every role has ended, so the flag is what it will be.  After a timeout the copies under way, which may be the last
-    // that were issued for each slot, land before the CTA ends, or 4 ms pass.
-    if (threadIdx.x == 0 && *abort_flag)
-        for (int n = max(0, issued - p.stages), t = 0; n < issued; ++n)
-            while (t < 200 && !mbar_try_suspend(full_bar(n % p.stages), n / p.stages & 1, 20000u)) ++t;
 
     uint32_t part[S];
 #pragma unroll
@@ -267,7 +256,13 @@ __global__ void __launch_bounds__(kThreads, 2) mid_kernel(const __grid_constant_
     __syncwarp();                                            // lanes leave the loop at different times
     if (S > 1) cluster_sync();                               // the other CTAs have read this one's sums
     else __syncthreads();
-    if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, RBK_ERR_TIMEOUT);
+    // Every role has ended, so the flag is what it will be.  After a timeout the copies under way, which may be the last
+    // that were issued for each slot, land before the CTA ends, or 4 ms pass.
+    if (threadIdx.x == 0 && *abort_flag) {
+        for (int n = max(0, issued - p.stages), t = 0; n < issued; ++n)
+            while (t < 200 && !mbar_try_suspend(full_bar(n % p.stages), n / p.stages & 1, 20000u)) ++t;
+        atomicExch(p.err, RBK_ERR_TIMEOUT);
+    }
     if (warp == 1) tmem_free(tmem, cols);
 }
 
@@ -398,9 +393,9 @@ int run(rbk_ctx* ctx, Params p, const Plan& pl, const void* A, int64_t lda, cons
     p.stages = std::min({8, p.kb_per, std::max(3, ((alone ? kAllSm : kHalfSm) - 1024 - kHead) / stage)});
     p.err = ctx->tickets + kGemmError;
     p.wait_ns = ctx->test_ffn_wait_ns ? ctx->test_ffn_wait_ns : kWaitTimeoutNs;
-    p.hold = ctx->test_ffn_wait_ns ? p.kb_per - 1 : -1;
+    p.tx = (p.rows_box + p.bn) * BK * 2 + (ctx->test_ffn_wait_ns ? 16 : 0);   // armed: more than will come
     ctx->test_ffn_wait_ns = 0;                               // the test setting covers one launch
-    const int smem = std::max(kHalfSm, 1024 + kHead + std::max(p.stages * stage, p.rows_box * (p.bn + 4) * 4));
+    const int smem = std::max(kHalfSm, 1024 + kHead + std::max(p.stages * stage, (p.rows_box + 31) / 32 * 32 * (p.bn + 4) * 4));
     CUtensorMap ta, tb;
     RBK_TRY(make_tmap(&ta, A, p.K, p.M, lda, 64, p.rows_box));
     if (p.b_mn) RBK_TRY(make_tmap(&tb, B, p.N, p.K, ldb, 64, 64));

@@ -14,6 +14,9 @@ namespace rbk {
 
 // tk + sub, or the last of `tokens` (> 0) where that is at or behind the end: tk <= tokens, sub 0 or 1.
 // tokens may be 2^31 - 1, so tk + sub alone may not fit an int.
-RBK_HD constexpr int token_at(int tk, int sub, int tokens) { return tk < tokens - sub ? tk + sub : tokens - 1; }
+RBK_HD constexpr int token_at(int tk, int sub, int tokens) {
+    const int last = tokens - 1 - sub;
+    return (tk < last ? tk : last) + sub;
+}
 
 }  // namespace rbk

@@ -321,9 +321,9 @@ def test_refused_tensors(ops):
 
 @pytest.mark.parametrize("N,D,F,back", [(100, 768, 2048, False), (100, 768, 2048, True), (300, 256, 2048, False)])
 def test_a_wait_that_runs_out(ops, N, D, F, back):
-    """A tile whose load never comes: its waits give up after 1 ms with copies of other slots under way, the launch
-    returns, RBK_ERR_TIMEOUT is reported, and the same call again gives the bits of a call before (backward: a
-    cluster shares K out)."""
+    """Tiles whose loads never complete: the waits give up after 1 ms with every slot's copies issued, the launch returns,
+    RBK_ERR_TIMEOUT is reported, and the same call again gives the bits of a call before (backward: a cluster shares
+    K out)."""
     from rbk._lib import call
     c = case(N, D, F, seed=13)
     gu = (c["x"].float() @ c["wgu"].float().T).half()
