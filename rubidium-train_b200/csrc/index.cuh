@@ -13,10 +13,10 @@
 namespace rbk {
 
 // tk + sub, or the last of `tokens` (> 0) where that is at or behind the end: tk <= tokens, sub 0 or 1.
-// tokens may be 2^31 - 1, so tk + sub alone may not fit an int.
+// tokens may be 2^31 - 1, so tk + sub may not fit an int, but fits 32 bits without a sign.
 RBK_HD constexpr int token_at(int tk, int sub, int tokens) {
-    const int last = tokens - 1 - sub;
-    return (tk < last ? tk : last) + sub;
+    const uint32_t at = (uint32_t)tk + (uint32_t)sub, last = (uint32_t)tokens - 1u;
+    return (int)(at < last ? at : last);
 }
 
 }  // namespace rbk
