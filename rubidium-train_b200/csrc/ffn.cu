@@ -5,7 +5,8 @@
 //
 // Many rows: tensor bound (6 N D F FLOP each way).  The CTA-pair GEMM of gemm.cu with epilogues of its own
 // makes h (gate and up tiles share one accumulator) and dgu; the other products are plain GEMMs.  8192 rows,
-// D 2048, F 5632: forward 430 to 490 us (the power limit moves it), backward without weight gradients 510 to 535.
+// D 2048, F 5632: forward 425 to 510 us (280 + 142 its two kernels alone; the power limit does the rest), backward without
+// weight gradients 500 to 560 (174 + 280), with them 1010 to 1050 (283 + 147 more); in a stream of calls 498 and 552.
 // Where those tiles are too few for the machine, smaller ones (ffn_mid.cu).
 // Few rows: the weights, 6 D F bytes, are read once and that is the cost.  The kernels below stream them.
 #include <algorithm>
@@ -26,8 +27,9 @@ namespace ffn {
 // A lane copies its vectors of the next DEPTH - 1 rounds, across tiles, into slots of its own with cp.async and
 // waits for its own copies only: the weights stream without registers or barriers.  Bound by HBM where the weights
 // are large (1 row, D 2048, F 5632: 14.6 us for both kernels, 69 MB, 4740 GB/s with two ramps; plain loads in
-// the loop took 22.4), by latency where they are not (D 768, F 2048: 5.0 us), and from 16 rows on also by x, which
-// every tile reads from L2 (32 rows: 26.7 us).
+// the loop took 22.4), by latency where they are not (D 768, F 2048: 5.5 us), and from 16 rows on also by x, which
+// every tile reads from L2 (32 rows: 26.7 us), and by SMs without work: 21 rows, D 1000, F 2664 are 167 tiles of gate and
+// up on 148 SMs and 63 of the down projection (13.8 us, floor 2.5).
 
 // Which calls they serve: up to 32 rows, and up to 64 of a narrow block, where the launches and waits of the tiles are
 // most of their time.  Measured at 48 rows, these kernels against the tiles: D 512, F 1024: 7.5 us against 9.8;
@@ -38,7 +40,7 @@ static bool few(int N, int D, int F) {
 }
 
 // WIDE: at most one tile per SM, so a CTA has all of its shared memory for what is in flight; else two CTAs share
-// an SM (1 row, D 4096, F 11264: 48.1 us; three of four warps with deeper slots 52.8), and a tile is 32 weight
+// an SM (1 row, D 4096, F 11264: 48 to 49.5 us; three of four warps with deeper slots 52.8), and a tile is 32 weight
 // rows where x, which comes from L2 for each, is more than the weights (16 rows n, D 1888, F 4312: 21.5 us with 16
 // weight rows, 16.6 with 32).
 template <int NT, bool WIDE>

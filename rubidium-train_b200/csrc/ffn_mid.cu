@@ -350,7 +350,12 @@ static Plan plan(rbk_ctx* ctx, int epi, int M, int N, int K, int b_mn) {
         if (!p.bn) p.bn = fit(2LL * N, kb >= 24 ? 64 : 48, 160, 1, slots);
         if (p.bn && here(p.bn, 1, ctas(2LL * N, p.bn)) > there(m2 * ((N + 127) / 128), 1)) p.bn = 0;
     } else if (epi == kGluBwd) {
-        // tiles of 192 columns fill an SM alone
+        // One round of two CTAs an SM with two parts of K; else one round of CTAs alone in an SM (192 columns); else one of
+        // two an SM with K whole.  Whole backwards, 64 columns x 2 parts | 192 x 2 | 64 whole | CTA pairs:
+        //   100 rows, D 1024, F 2048:  18.0 | 21.7 | 20.0 | 26.4        200 rows, D 2048, F 4736:  35.4 | 36.5 | 37.0 | 41.0
+        //   200 rows, D 2048, F 5632:  45.7 | 39.3 | 42.2 | 44.1        300 rows, D 1024, F 4736:  36.5 | 34.5 | 30.4 | 33.8
+        // Over 119 shapes (100 to 1500 rows, D 256 to 4096) within 0.2% of the best of the four on average, the worst
+        // 14% off it (200 rows, D 256, F 5632: 25.9, 22.6 with 64 columns in two parts, two rounds).
         if (2 * ctas(N, 64) <= slots) p = {64, 2};
         else if (4 * ctas(N, 192) <= slots) p = {192, 2};
         else if (ctas(N, 64) <= slots) p = {64, 1};
@@ -360,7 +365,13 @@ static Plan plan(rbk_ctx* ctx, int epi, int M, int N, int K, int b_mn) {
         if (m <= 2 || kb <= 32 * p.S) p.bn = fit(N, m <= 2 ? 32 : 48, 80, p.S, slots);
         if (p.bn && here(p.bn, p.S, ctas(N, p.bn) * p.S) > there(m2 * ((N + 255) / 256), gemm_store_splits(ctx, M, N, K))) p.bn = 0;
     } else {
-        // dx: K is twice F, and its rows of B come 64 columns at a time
+        // dx: K is twice F, and its rows of B come 64 columns at a time.  t tiles.  Two parts where K is short and the
+        // tiles many; eight where they are few and K is worth the exchange; four between; CTA pairs, which share K out
+        // over planes, where K is long or the tiles are enough for them.  Whole backwards, 2 | 4 | 8 parts | CTA pairs:
+        //   t 64, 500 rows, D 1024, F 1024:  17.4 | 20.1 | 33.3 | 20.5     t 8, 100 rows, D 512, F 2304:  20.8 | 15.9 | 14.9 | 17.4
+        //   t 48, 300 rows, D 1024, F 2560:  26.9 | 24.5 | 35.5 | 25.6     t 48, 300 rows, D 1024, F 5632:  43.8 | 34.4 | 45.9 | 32.1
+        // Over 143 shapes (t 8 to 144, 8 to 176 k blocks) within 2% of the best of the four on average and 0.94 of the
+        // pairs' time; the worst 19% off it (t 24, 200 rows, D 768, F 1792: 20.3, and 17.0 with four parts).
         const long long t = ctas(N, 64);
         if (kb <= 32 && 8 * t > slots) {
             if (2 * t <= slots) p = {64, 2};

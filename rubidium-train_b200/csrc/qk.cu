@@ -10,8 +10,11 @@
 //
 // Memory bound: 4 bytes per element forward, 6 backward, each touched once.  16384 tokens, 16 + 16 heads of
 // 128: forward 45.7 us = 5880 GB/s, backward 65.4 us = 6160 GB/s (0.91 and 0.95 of a copy's rate); 16384
-// tokens, 12 + 12 heads of 64: backward 27.5 us = 5490 GB/s; 32 tokens forward: 2.8 us, a launch.  Few heads
-// and odd widths are bound by their instructions: 65740 tokens, 3 + 3 heads of 80, backward 54 us = 3500 GB/s.
+// tokens, 12 + 12 heads of 64: backward 27.5 us = 5490 GB/s; 32 tokens forward: 2.8 us, a launch.  These are replays
+// from a graph; a stream of calls, whose clock is lower, takes 50.6, 73.7 and 31.4 us (0.82, 0.85 and 0.75 of a copy's
+// rate): three in five issue slots are taken.  Few heads and odd widths are bound by their instructions: 65740 tokens,
+// 3 + 3 heads of 80, backward 54 us = 3500 GB/s, and its 128 registers spill 16 bytes (the backwards of 3, 5, 6, 10 and
+// 16 lanes all spill, 4 to 48 bytes, of 2, 4 and 8 lanes some, 4 to 12).
 // Layout: a head is split over G lanes (dh / 16, or the next of 8, 10 and 16), a lane holding two
 // 16-byte chunks of it, chosen so that both members of every rotated pair are in the
 // same lane: no exchange is needed for the rotation.  A warp, or each half of one (T = 2,
