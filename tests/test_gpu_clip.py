@@ -241,3 +241,18 @@ def test_model_step_clipped_by_the_global_norm(ops):
     got, v = m._bufs[3].double(), 0.1 * g / scale / 4
     assert bool(((got - v).abs() <= 10 * E * v.abs() + 2.0 ** -149).all()) and float(got.norm()) > 0
     assert m.scaler().skipped == 0
+
+
+def test_more_elements_than_32_bits_count(ops):
+    """A tensor of 2^32 + 5 halves, clipped in place: its ends count and are scaled, its neighbours stay."""
+    n = 2 ** 32 + 5
+    buf = torch.zeros(n + 16, device="cuda", dtype=torch.float16)
+    g = buf[3:3 + n]
+    at = [0, 1, 2 ** 31 - 1, 2 ** 31, 2 ** 32 - 1, 2 ** 32, n - 1]
+    g[at] = 16.0
+    buf[:3], buf[3 + n:] = 5.0, 5.0
+    want = 16.0 * math.sqrt(len(at))
+    norm = ops.clip_grad_norm([g], want / 4)
+    assert abs(float(norm) - want) <= 5 * E * want
+    assert bool((g[at] == 4.0).all()) and int(torch.count_nonzero(g)) == len(at)
+    assert bool((buf[:3] == 5).all()) and bool((buf[3 + n:] == 5).all())

@@ -533,3 +533,25 @@ def test_backward_without_x_and_into_given_rows(ops, N):
     assert torch.equal(wide[:, 8:8 + D], dx) and bool((wide[:, :8] == 9).all()) and bool((wide[:, 8 + D:] == 9).all())
     with pytest.raises(RuntimeError, match="x is NULL"):
         ops.gated_ffn_bwd(c["dy"], None, gu, c["wgu"], c["wd"], dwgu=grads[0]["dwgu"])
+
+
+def test_offsets_beyond_32_bits(ops):
+    """gate | up, h and dgu of more than 2^31 elements: the last rows are right, forward and backward."""
+    N, D, F = 1100000, 64, 2056
+    g = torch.Generator(device="cuda").manual_seed(20)
+    c = dict(wgu=(torch.randn(2 * F, D, device="cuda", generator=g) * D ** -0.5).half(),
+             wd=(torch.randn(D, F, device="cuda", generator=g) * F ** -0.5).half(),
+             x=torch.randn(N, D, device="cuda", generator=g).half(), dy=torch.randn(N, D, device="cuda", generator=g).half())
+    full_tiles(ops, N, D, F)
+    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"])
+    assert h.numel() > 2 ** 31
+    for rows in (slice(0, 200), slice(N - 300, N)):
+        want = ref.fwd(c["x"][rows], c["wgu"], c["wd"], None, None, None, "silu")
+        for name, t in (("gu", gu), ("h", h), ("y", y)):
+            within(name, t[rows], *want[name])
+    dx, dgu, h2 = ops.gated_ffn_bwd(c["dy"], None, gu, c["wgu"], c["wd"])
+    for rows in (slice(0, 200), slice(N - 300, N)):
+        want = ref.bwd(c["dy"][rows], c["x"][rows], gu[rows], c["wgu"], c["wd"], "silu")
+        for name, t in (("dgu", dgu), ("h", h2), ("dx", dx)):
+            within(name, t[rows], *want[name])
+    assert ops.device_error() == 0
