@@ -256,3 +256,5 @@ def test_more_elements_than_32_bits_count(ops):
     assert abs(float(norm) - want) <= 5 * E * want
     assert bool((g[at] == 4.0).all()) and int(torch.count_nonzero(g)) == len(at)
     assert bool((buf[:3] == 5).all()) and bool((buf[3 + n:] == 5).all())
+    del buf, g
+    torch.cuda.empty_cache()

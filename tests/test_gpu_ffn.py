@@ -555,3 +555,5 @@ def test_offsets_beyond_32_bits(ops):
         for name, t in (("dgu", dgu), ("h", h2), ("dx", dx)):
             within(name, t[rows], *want[name])
     assert ops.device_error() == 0
+    del gu, h, dgu, h2
+    torch.cuda.empty_cache()

@@ -291,3 +291,22 @@ def test_strides_of_axes_of_size_one(ops):
         assert torch.equal(dq, wdq) and torch.equal(dg, wg)
     with pytest.raises(RuntimeError, match="multiples of 8"):
         ops.qk_norm_rope_fwd(torch.as_strided(x, (1, 2, 1, 64), (0, 65, 0, 1)), None)
+
+
+def test_as_many_tokens_as_are_taken(ops):
+    """2^31 - 1 tokens of one head of 8, two tokens a warp, with listed positions: the last tokens are those of a short
+    call, the rest (zeros) stays zero."""
+    n, last = 2 ** 31 - 1, 300
+    if torch.cuda.get_device_properties(0).total_memory < 64 << 30:
+        pytest.skip("needs 43 GB")
+    q = torch.zeros(1, n, 1, 8, device="cuda", dtype=torch.float16)
+    q[0, -last:] = torch.randn(last, 1, 8, device="cuda").half()
+    pos = torch.arange(n, device="cuda", dtype=torch.int32).view(1, n)
+    g = (1 + torch.randn(8, device="cuda")).half()
+    want, _ = ops.qk_norm_rope_fwd(q[:, -last:].clone(), None, g, positions=pos[:, -last:].clone(), rot=8, interleaved=True)
+    ops.qk_norm_rope_fwd(q, None, g, positions=pos, rot=8, interleaved=True, out=(q, None))
+    assert torch.equal(q[:, -last:], want)
+    for part in q.view(-1)[:-8 * last].split(1 << 30):
+        assert not bool(part.any())
+    del q, pos, part
+    torch.cuda.empty_cache()
