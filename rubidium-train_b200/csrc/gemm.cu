@@ -25,6 +25,7 @@
 // RBK_ERR_TIMEOUT, drains, frees TMEM and returns.
 // No cluster multicast is used anywhere.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "tc.cuh"
@@ -1396,7 +1397,7 @@ int launch_pair(rbk_ctx* ctx, const rbk_gemm_desc* d, Params& p, cudaStream_t st
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    static int configured_device = -1, max_pairs = 0;
+    static std::atomic<int> configured_device{-1}, max_pairs{0};   // another thread may be here: the device last
     if (configured_device != ctx->device) {
         RBK_CUDA(cudaFuncSetAttribute(gemm_pair_kernel<EPI, ROW>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         cfg.gridDim = dim3(ctx->num_sms & ~1);
@@ -1405,7 +1406,7 @@ int launch_pair(rbk_ctx* ctx, const rbk_gemm_desc* d, Params& p, cudaStream_t st
         max_pairs = n > 0 ? n : ctx->num_sms / 2;
         configured_device = ctx->device;
     }
-    const int pairs = p.units < max_pairs ? p.units : max_pairs;
+    const int pairs = std::min(p.units, max_pairs.load());
     cfg.gridDim = dim3(2 * pairs);
     cfg.numAttrs = set_pdl(attr, 1);
     RBK_CUDA(cudaLaunchKernelEx(&cfg, gemm_pair_kernel<EPI, ROW>, ta, tb, tc_, tx, tp, p));
@@ -1430,7 +1431,7 @@ int launch_glu(rbk_ctx* ctx, const CUtensorMap& ta, const CUtensorMap& tb, const
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    static int configured_device = -1, max_pairs = 0;
+    static std::atomic<int> configured_device{-1}, max_pairs{0};   // another thread may be here: the device last
     if (configured_device != ctx->device) {
         RBK_CUDA(cudaFuncSetAttribute(gemm_pair_kernel<EPI, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         cfg.gridDim = dim3(ctx->num_sms & ~1);
@@ -1439,7 +1440,7 @@ int launch_glu(rbk_ctx* ctx, const CUtensorMap& ta, const CUtensorMap& tb, const
         max_pairs = n > 0 ? n : ctx->num_sms / 2;
         configured_device = ctx->device;
     }
-    cfg.gridDim = dim3(2 * (p.units < max_pairs ? p.units : max_pairs));
+    cfg.gridDim = dim3(2 * std::min(p.units, max_pairs.load()));
     cfg.numAttrs = set_pdl(attr, 1);
     RBK_CUDA(cudaLaunchKernelEx(&cfg, gemm_pair_kernel<EPI, false>, ta, tb, tg, tu, th, p));
     RBK_LAUNCHED("gemm_pair_kernel (gated)");

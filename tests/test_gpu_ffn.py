@@ -557,3 +557,33 @@ def test_offsets_beyond_32_bits(ops):
     assert ops.device_error() == 0
     del gu, h, dgu, h2
     torch.cuda.empty_cache()
+
+
+def test_full_tiles_from_threads(ops):
+    """Four host threads with their own contexts and streams, whose first calls of the pair kernels may meet."""
+    import threading
+    N, D, F = PAIRS[0]
+    full_tiles(ops, N, D, F)
+    c = case(N, D, F, True, True, seed=21)
+    got, wrong = [None] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], bgu=c["bgu"], bd=c["bd"], residual=c["residual"])
+                    got[i] = (y, gu, h) + ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                             # a thread's exception is not pytest's
+            wrong.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    y, gu, h = ops.gated_ffn_fwd(c["x"], c["wgu"], c["wd"], bgu=c["bgu"], bd=c["bd"], residual=c["residual"])
+    want = (y, gu, h) + ops.gated_ffn_bwd(c["dy"], c["x"], gu, c["wgu"], c["wd"])
+    assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
